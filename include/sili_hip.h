@@ -560,6 +560,202 @@ int sili_memcpy_h2d_ordered(sili_layer *layer, void *dst, const void *src, size_
  * kernel on the stream, which writes the host pages directly. */
 int sili_memcpy_d2h_ordered(sili_layer *layer, void *dst, const void *src, size_t bytes);
 
+/* ---- operators between the layers ---------------------------------------
+ * What a transformer block needs beside its linear layers: the bookkeeping of
+ * requests, rotary positions, the norms around a block, and attention over a
+ * cache held in 4 bits.  No counterpart in the reference (a layer library).
+ * Every pointer in the argument structs is a device pointer unless its comment
+ * says host; strides count elements.  The calls run on `stream` (NULL: HIP's
+ * default stream) of the calling thread's current device, allocate nothing,
+ * wait for nothing, keep nothing between calls, and may be recorded into a
+ * graph.  Sums, softmax statistics and norms are held in fp32; results are
+ * rounded once, to `dtype`. */
+enum { SILI_F32 = 0, SILI_BF16 = 1, SILI_F16 = 2 };
+
+/* Block tables, slot maps and positions of a step, from request lengths.
+ * Request r has cached_lens[r] tokens in the cache, held by the first
+ * ceil(cached_lens[r] / page_size) entries of its block_table row, and brings
+ * new_lens[r] tokens.  The step's further pages are taken from free_pages in
+ * request order (page i of the step is free_pages[i]) and written into the
+ * table; the other entries stay.  The new tokens of all requests lie one after
+ * another: q_start[r] is the first of request r, kv_lens[r] = cached + new;
+ * token t at position p of request r has slots[t] = block_table[r][p /
+ * page_size] * page_size + p % page_size.  Tokens from the total to max_tokens
+ * get slot -1 (which sili_kv4_append skips) and position 0.
+ * status[0]: pages taken; status[1]: 0, or the sum of SILI_SLOTS_* for what
+ * did not fit: a table entry without a page becomes -1 and its tokens get slot
+ * -1; tokens past max_tokens are left out.  Negative lengths count as 0. */
+enum {
+    SILI_SLOTS_NO_PAGE = 1,    /* free_pages is too short */
+    SILI_SLOTS_TABLE_FULL = 2, /* a request needs more than table_width pages */
+    SILI_SLOTS_TOKENS_FULL = 4,/* more than max_tokens new tokens */
+    SILI_SLOTS_BAD_LENGTH = 8, /* a negative length, or cached + new past 2^31 - 1 (new is cut) */
+    SILI_SLOTS_BAD_PAGE = 16   /* a page that new tokens need is negative, or has slots past 2^31 - 1 */
+};
+typedef struct {
+    const int32_t *cached_lens, *new_lens;  /* [requests] */
+    int64_t requests, page_size;
+    const int32_t *free_pages;              /* [n_free] */
+    int64_t n_free;
+    int32_t *block_table;                   /* [requests][table_width], in and out */
+    int64_t table_width, max_tokens;
+    int32_t *q_start;                       /* [requests + 1] */
+    int32_t *kv_lens;                       /* [requests] */
+    int32_t *positions, *slots;             /* [max_tokens] */
+    int32_t *status;                        /* [2] */
+} sili_request_slots_args;
+int sili_request_slots(const sili_request_slots_args *args, void *stream);
+
+/* Rotary positions of q and k [tokens][heads][head_dim] (k_heads 0: q alone).
+ * The first rot_dim channels of a head are turned in pairs, by the angle
+ * positions[t] * phase_steps[i] / 2^64 turns for pair i:
+ *     x1' = scale (x1 cos - x2 sin),  x2' = scale (x2 cos + x1 sin)
+ * layout SILI_ROTARY_HALF pairs channels (i, i + rot_dim / 2), _INTERLEAVED
+ * (2 i, 2 i + 1); the channels from rot_dim on are copied.  inverse != 0 turns
+ * the other way: the gradient of the forward turn with the same arguments.
+ * The angle is held as a 64-bit fraction of a turn, exact modulo 1, so a
+ * position of 10^6 is as accurate as position 1.  Outputs may be the inputs
+ * (same strides), and may not overlap them otherwise. */
+enum { SILI_ROTARY_HALF = 0, SILI_ROTARY_INTERLEAVED = 1 };
+typedef struct {
+    int32_t dtype, layout, inverse;
+    float scale;
+    int64_t tokens, head_dim, rot_dim, q_heads, k_heads;
+    const int32_t *positions;    /* [tokens] */
+    const uint64_t *phase_steps; /* [rot_dim / 2] */
+    const void *q, *k;
+    int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+    void *q_out, *k_out;
+    int64_t q_out_token_stride, q_out_head_stride, k_out_token_stride, k_out_head_stride;
+} sili_rotary_args;
+int sili_rotary(const sili_rotary_args *args, void *stream);
+
+/* Phase steps for sili_rotary, on the host: pair i turns by base^(-2 i /
+ * rot_dim) radians a position, stretched for contexts longer than the
+ * original_len positions a model was trained on:
+ *   SILI_ROTARY_PLAIN   as it is
+ *   SILI_ROTARY_LINEAR  all divided by factor
+ *   SILI_ROTARY_BANDS   with n the turns a pair makes over original_len: kept
+ *                       for n >= high, divided by factor for n <= low, a ramp
+ *                       linear in n between; scale = 0.1 ln(factor) + 1
+ *   SILI_ROTARY_BASE    base * factor^(rot_dim / (rot_dim - 2)) for base
+ * steps: host uint64 [rot_dim / 2]; *scale: the factor for
+ * sili_rotary_args.scale (1 but for BANDS). */
+enum { SILI_ROTARY_PLAIN = 0, SILI_ROTARY_LINEAR = 1, SILI_ROTARY_BANDS = 2, SILI_ROTARY_BASE = 3 };
+int sili_rotary_steps(int64_t rot_dim, double base, int scaling, double factor, double original_len, double low,
+                      double high, uint64_t *steps, float *scale);
+
+/* The norm after a block, its gate and residual scale, and the norm before the
+ * next block, in one pass over [tokens][width] (width <= 32768):
+ *     n = w_post ? u rsqrt(mean u^2 + eps) w_post : u       (block output u)
+ *     y = x_scale x + u_scale (gate ? gate n : n)           (residual stream x)
+ *     h = y rsqrt(mean y^2 + eps) w_pre                     (next block's input)
+ * x NULL: no residual term.  w_pre NULL: h and rstd_pre are not computed.
+ * gate: one row for all tokens (gate_stride 0) or a row a token.  h is taken
+ * from y before its rounding.  rstd_post / rstd_pre [tokens]: the two
+ * reciprocal norms, for the backward pass; may be NULL.  y may be x, h may be
+ * u (same strides). */
+typedef struct {
+    int32_t dtype;
+    float u_scale, x_scale, eps;
+    int64_t tokens, width;
+    const void *u, *x, *gate;
+    int64_t u_stride, x_stride, gate_stride;
+    const float *w_post, *w_pre; /* [width] */
+    void *y, *h;
+    int64_t y_stride, h_stride;
+    float *rstd_post, *rstd_pre;
+} sili_block_norm_args;
+int sili_block_norm_forward(const sili_block_norm_args *args, void *stream);
+
+/* Its gradients.  args as in the forward pass, whose y (unless w_pre is NULL),
+ * rstd_post and rstd_pre are read; x, h and eps are not.  dy, dh: upstream
+ * gradients of y and h; either may be NULL (zero), dh is when w_pre is.  du, dx
+ * (NULL: not wanted) in dtype.  dgate: fp32 [width], summed over the tokens,
+ * for a shared gate (dgate_stride 0 as gate_stride), else rows in dtype; NULL:
+ * not wanted.  dw_post, dw_pre: fp32 [width], NULL: not wanted.  Sums over
+ * tokens are taken in an order that depends on the shape alone: the same call
+ * gives the same bits.  workspace: device memory of
+ * sili_block_norm_workspace(args) bytes; calls that overlap need one each. */
+typedef struct {
+    const void *dy, *dh;
+    int64_t dy_stride, dh_stride;
+    void *du, *dx, *dgate;
+    int64_t du_stride, dx_stride, dgate_stride;
+    float *dw_post, *dw_pre;
+    void *workspace;
+    size_t workspace_bytes;
+} sili_block_norm_grads;
+int sili_block_norm_backward(const sili_block_norm_args *args, const sili_block_norm_grads *grads, void *stream);
+int sili_block_norm_workspace(const sili_block_norm_args *args, size_t *bytes);
+
+/* A paged cache of keys and values in 4 bits.  Per token and kv head one fp32
+ * scale amax / 6 and head_dim E2M1 codes, fp4_encode(x * (6 / amax)), the
+ * layers' own codec (nearest, ties away from zero).  A head whose amax is below
+ * 2^-120 is stored as zeros; one with a NaN or an infinity gets a NaN scale and
+ * reads as NaN.  Bytes hold channel 2b in the low and 2b + 1 in the high
+ * nibble:
+ *   k       [n_pages][kv_heads][page_size][head_dim / 2]
+ *   v       [n_pages][kv_heads][page_size / 16][head_dim / 2][16 tokens]
+ *   k_scale [n_pages][kv_heads][page_size], v_scale likewise
+ * head_dim 64, 128 or 256; page_size a multiple of 16; k, v and the scales
+ * 16-byte aligned. */
+typedef struct {
+    uint8_t *k, *v;
+    float *k_scale, *v_scale;
+    int64_t n_pages, kv_heads, head_dim, page_size;
+} sili_kv4_cache;
+
+/* sili_kv4_append writes rows k, v [tokens][kv_heads][head_dim] of `dtype` to
+ * slots[t] = page * page_size + offset; sili_kv4_read writes the values stored
+ * at slots[t] to them.  A slot outside the cache is skipped by append (padding)
+ * and reads as zeros.  Distinct tokens take distinct slots. */
+typedef struct {
+    sili_kv4_cache cache;
+    int32_t dtype;
+    int64_t tokens;
+    const int32_t *slots; /* [tokens] */
+    void *k, *v;
+    int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+} sili_kv4_rows_args;
+int sili_kv4_append(const sili_kv4_rows_args *args, void *stream);
+int sili_kv4_read(const sili_kv4_rows_args *args, void *stream);
+
+/* Attention over the cache: out = softmax(scale q k^T) v for the query tokens
+ * q_start[r] .. q_start[r + 1] - 1 of each request r, whose keys are the first
+ * kv_lens[r] tokens of its block_table row (the new tokens appended already).
+ * q_heads is a multiple of kv_heads; query head h reads kv head h / (q_heads /
+ * kv_heads).  causal: query i of n sits at position p = kv_lens[r] - n + i and
+ * sees keys up to p, with window > 0 only the last `window` of them.  A row
+ * that sees no key gets out = 0 and lse = -infinity.  lse [tokens][q_heads]
+ * (natural logarithm of the softmax sum), may be NULL.
+ * max_new and max_len bound the requests' query tokens and key counts (host
+ * values; they size the grid): queries past max_new are not computed, keys past
+ * max_len not seen.  A table entry outside the cache hides its page's keys.
+ * fp32 inputs are multiplied in two bf16 parts each (16 significant bits),
+ * bf16 inputs exactly; codes are exact in bf16.  workspace: device memory of
+ * sili_kv4_attend_workspace(args) bytes, 16-byte aligned; calls that overlap
+ * need one each. */
+typedef struct {
+    sili_kv4_cache cache;
+    int32_t dtype, causal;
+    int64_t requests, tokens, q_heads;
+    const int32_t *q_start;     /* [requests + 1] */
+    const int32_t *kv_lens;     /* [requests] */
+    const int32_t *block_table; /* [requests][table_width] */
+    int64_t table_width, max_new, max_len, window;
+    float scale;
+    const void *q;
+    int64_t q_token_stride, q_head_stride;
+    void *out;
+    int64_t out_token_stride, out_head_stride;
+    float *lse;
+    void *workspace;
+    size_t workspace_bytes;
+} sili_kv4_attend_args;
+int sili_kv4_attend(const sili_kv4_attend_args *args, void *stream);
+int sili_kv4_attend_workspace(const sili_kv4_attend_args *args, size_t *bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,6 +1,7 @@
 // capi.hip -- the extern "C" boundary (include/sili_hip.h) and the layer's
 // host-side orchestration of the kernels.
 #include "../../include/sili_hip.h"
+#include "block_ops.hpp"
 #include "layer.hpp"
 #include "wave.hpp"
 
@@ -1802,6 +1803,77 @@ int sili_dense_to_top_k_csr(const float *x, int64_t rows, int64_t cols, int64_t 
     return guarded([&] {
         if (!nnz) throw_error(SILI_ERR_INVALID, "dense_to_top_k_csr: nnz is NULL");
         dense_to_top_k_csr_device(x, rows, cols, k, ptrs, indices, values, nnz, reinterpret_cast<hipStream_t>(stream));
+    });
+}
+
+int sili_request_slots(const sili_request_slots_args *args, void *stream) {
+    return guarded([&] {
+        if (!args) throw_error(SILI_ERR_INVALID, "request_slots: NULL arguments");
+        request_slots(*args, reinterpret_cast<hipStream_t>(stream));
+    });
+}
+
+int sili_rotary(const sili_rotary_args *args, void *stream) {
+    return guarded([&] {
+        if (!args) throw_error(SILI_ERR_INVALID, "rotary: NULL arguments");
+        rotary(*args, reinterpret_cast<hipStream_t>(stream));
+    });
+}
+
+int sili_block_norm_forward(const sili_block_norm_args *args, void *stream) {
+    return guarded([&] {
+        if (!args) throw_error(SILI_ERR_INVALID, "block_norm_forward: NULL arguments");
+        block_norm_forward(*args, reinterpret_cast<hipStream_t>(stream));
+    });
+}
+
+int sili_block_norm_backward(const sili_block_norm_args *args, const sili_block_norm_grads *grads, void *stream) {
+    return guarded([&] {
+        if (!args || !grads) throw_error(SILI_ERR_INVALID, "block_norm_backward: NULL arguments");
+        block_norm_backward(*args, *grads, reinterpret_cast<hipStream_t>(stream));
+    });
+}
+
+int sili_kv4_append(const sili_kv4_rows_args *args, void *stream) {
+    return guarded([&] {
+        if (!args) throw_error(SILI_ERR_INVALID, "kv4_append: NULL arguments");
+        kv4_append(*args, reinterpret_cast<hipStream_t>(stream));
+    });
+}
+
+int sili_kv4_read(const sili_kv4_rows_args *args, void *stream) {
+    return guarded([&] {
+        if (!args) throw_error(SILI_ERR_INVALID, "kv4_read: NULL arguments");
+        kv4_read(*args, reinterpret_cast<hipStream_t>(stream));
+    });
+}
+
+int sili_kv4_attend(const sili_kv4_attend_args *args, void *stream) {
+    return guarded([&] {
+        if (!args) throw_error(SILI_ERR_INVALID, "kv4_attend: NULL arguments");
+        kv4_attend(*args, reinterpret_cast<hipStream_t>(stream));
+    });
+}
+
+int sili_block_norm_workspace(const sili_block_norm_args *args, size_t *bytes) {
+    return guarded([&] {
+        if (!args || !bytes) throw_error(SILI_ERR_INVALID, "block_norm_workspace: NULL arguments");
+        *bytes = block_norm_workspace(*args);
+    });
+}
+
+int sili_kv4_attend_workspace(const sili_kv4_attend_args *args, size_t *bytes) {
+    return guarded([&] {
+        if (!args || !bytes) throw_error(SILI_ERR_INVALID, "kv4_attend_workspace: NULL arguments");
+        *bytes = kv4_attend_workspace(*args);
+    });
+}
+
+int sili_rotary_steps(int64_t rot_dim, double base, int scaling, double factor, double original_len, double low,
+                      double high, uint64_t *steps, float *scale) {
+    return guarded([&] {
+        if (!steps || !scale) throw_error(SILI_ERR_INVALID, "rotary_steps: NULL arguments");
+        rotary_steps(rot_dim, base, scaling, factor, original_len, low, high, steps, scale);
     });
 }
 
