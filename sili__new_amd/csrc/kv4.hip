@@ -93,76 +93,442 @@ __device__ __forceinline__ int64_t request_of(const int32_t *start, int64_t n, i
     return lo;
 }
 
-// One wave a (query token, query head).  Per step of 64 keys: a lane takes the
-// score of one key; the running maximum and sum are updated; then a lane takes
-// a channel pair of the values.
-template <typename T>
-__global__ __launch_bounds__(64) void k_kv4_attend(sili_kv4_attend_args a) {
-    __shared__ float s_q[256], s_p[64];
-    __shared__ int64_t s_v[64];
-    const sili_kv4_cache &c = a.cache;
-    const int lane = threadIdx.x, d = (int)c.head_dim;
-    const int64_t t = blockIdx.x, qh = blockIdx.y, h = qh / (a.q_heads / c.kv_heads);
-    if (t < a.q_start[0] || t >= a.q_start[a.requests]) return;
-    const int64_t r = request_of(a.q_start, a.requests, t);
-    const int64_t n_new = a.q_start[r + 1] - a.q_start[r], i = t - a.q_start[r];
-    if (i >= a.max_new) return;
-    const int64_t kv = a.kv_lens[r], last = kv - n_new + i;
-    int64_t end = min(min(kv, a.max_len), a.table_width * c.page_size), begin = 0;
-    if (a.causal) {
-        end = min(end, last + 1);
-        if (a.window > 0) begin = max((int64_t)0, last + 1 - a.window);
-    }
-    const T *q = (const T *)a.q + t * a.q_token_stride + qh * a.q_head_stride;
-    for (int k = lane; k < d; k += 64) s_q[k] = (float)q[k] * a.scale;
-    __syncthreads();
-    float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int64_t base = begin; base < end; base += 64) {
-        const int64_t j = base + lane;
-        float s = -INFINITY, vs = 0.0f;
-        int64_t vb = -1;
-        if (j < end) {
-            const int64_t page = a.block_table[r * a.table_width + j / c.page_size];
-            const int at = (int)(j % c.page_size);
-            if (page >= 0 && page < c.n_pages) {
-                const int64_t head = page * c.kv_heads + h;
-                const uint32_t *codes = reinterpret_cast<const uint32_t *>(c.k + k_byte(c, head, at, 0));
-                float dot = 0.0f;
-                for (int w = 0; w < d / 8; ++w) {
-                    const uint32_t x = codes[w];
+// ---- attention -----------------------------------------------------------------
+//
+// Rows of a (request, kv head) are its query tokens times the group of query
+// heads that share the kv head: row = token * group + head in group.  A wave
+// takes 16 NT of them against 64 keys a step, on the bf16 matrix cores:
+//
+//   S^T = K q^T    16 keys x 16 rows a tile, codes x q, four tiles a step
+//   p   = exp2(c (k_scale S - m)),   l += p
+//   O^T += V^T (v_scale p)^T         16 channels x 16 rows a tile
+//
+// E2M1 codes are exact in bf16, and the two scales of a key multiply its score
+// and its weight in fp32, so the cache's values lose nothing; q and p enter in
+// one bf16 part or two (the second the rest of the first), 8 or 16 significant
+// bits.  In both products the row is the lane's column (lane % 16), and with
+//     tile x row of K  ->  key 16 (row / 4) + 4 x + row % 4
+// the lane's four results of the four score tiles are the keys 16 g .. 16 g +
+// 15, g = lane / 16: the very k indices its share of the second product's right
+// operand holds, so no score moves between lanes.  The left operands come from
+// memory as the lane needs them: 32 channels of a K row are 16 bytes, and 16
+// keys of a V channel pair are 16 bytes.
+//
+// The running maximum m is raised only when a score passes it by 2^8 (in exp2's
+// argument 8): until then weights stay below 2^8 and nothing has to be rescaled.
+constexpr int WAVES = 4;
+constexpr float SLACK = 8.0f;
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+
+__device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){x, y}, bf16x2));
+}
+__device__ __forceinline__ float bf16_lo(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t w) { return __builtin_bit_cast(float, w & 0xFFFF0000u); }
+// Two codes (byte SEL of w) to bf16.
+template <int SEL>
+__device__ __forceinline__ uint32_t codes(uint32_t w) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, SEL));
+}
+// Eight codes of a dword: eight consecutive channels.
+__device__ __forceinline__ u32x4 codes8(uint32_t w) { return (u32x4){codes<0>(w), codes<1>(w), codes<2>(w), codes<3>(w)}; }
+// Four keys of a channel pair (a dword of V) to the even and the odd channel.
+__device__ __forceinline__ void codes_by_channel(uint32_t w, uint32_t (&even)[2], uint32_t (&odd)[2]) {
+    const uint32_t a = codes<0>(w), b = codes<1>(w), c = codes<2>(w), d = codes<3>(w);
+    even[0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+    odd[0] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    even[1] = __builtin_amdgcn_perm(d, c, 0x05040100u);
+    odd[1] = __builtin_amdgcn_perm(d, c, 0x07060302u);
+}
+__device__ __forceinline__ float lanes_max(float v) {  // over the four lanes of a row
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float lanes_sum(float v) {
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
+}
+
+// How a launch cuts the work, set on the host.
+struct AttendPlan {
+    int32_t groups_per_page;  // page_size / 16
+    int32_t page_shift;       // its logarithm, or -1
+    int32_t splits, chunk;    // keys a split takes (a multiple of 64 WAVES or of 64)
+    int32_t few, many;        // takes requests of more than `few` rows, up to `many`
+    float c;                  // |scale| log2(e)
+    bool negative;            // scale < 0: the sign goes to q
+    float *part_o;            // [tokens * q_heads][splits][D], unnormalised
+    float2 *part_ml;          // [tokens * q_heads][splits]: m c, l
+};
+
+// Keys that query i of n sees, [begin, end).
+struct KeyRange {
+    int32_t base, cap, window;  // keys before the first query, keys there are
+    bool causal;
+    __device__ __forceinline__ int32_t end(int32_t i) const { return causal ? min(cap, base + i + 1) : cap; }
+    __device__ __forceinline__ int32_t begin(int32_t i) const { return window > 0 ? max(0, base + i + 1 - window) : 0; }
+};
+
+// BY_KEYS: the block's waves share 16 NT rows and take every fourth step of
+// keys each; their results are joined in LDS.  Otherwise each wave has rows of
+// its own.
+template <typename T, int D, int NT, bool BY_KEYS>
+__global__ __launch_bounds__(64 * WAVES) void k_attend(sili_kv4_attend_args a, AttendPlan pl) {
+    constexpr int QP = sizeof(T) == 2 && __is_same(T, __bf16) ? 1 : 2;  // parts of q
+    constexpr int PP = sizeof(T) == 4 ? 2 : 1;                          // parts of p
+    constexpr int KS = D / 32;   // steps of 32 channels
+    constexpr int CT = D / 32;   // blocks of 32 output channels
+    extern __shared__ float s_join[];
+    const sili_kv4_cache &cache = a.cache;
+    const int wave = (int)uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, r16 = lane & 15;
+    const int H = (int)cache.kv_heads, group = (int)(a.q_heads / H);
+    const int h = blockIdx.x % H, tile = blockIdx.x / H, split = blockIdx.y, req = blockIdx.z;
+    const int32_t q0 = a.q_start[req];
+    const int32_t n_all = a.q_start[req + 1] - q0, n = min(n_all, (int32_t)a.max_new);
+    const int32_t n_rows = n * group;
+    const int32_t first = (BY_KEYS ? tile : tile * WAVES + wave) * (16 * NT);
+    if (q0 < 0 || n_rows <= pl.few || n_rows > pl.many) return;
+    if (first >= n_rows) return;  // BY_KEYS: the whole block
+    const int32_t kv = a.kv_lens[req];
+    KeyRange kr;
+    kr.base = kv - n_all;
+    kr.window = (int32_t)a.window;
+    kr.causal = a.causal != 0;
+    kr.cap = cache.n_pages == 0 ? 0 : (int32_t)min(min((int64_t)kv, a.max_len), a.table_width * cache.page_size);
+    const int32_t i_first = first / group, i_last = min(first + 16 * NT - 1, n_rows - 1) / group;
+    const int32_t lo = kr.begin(i_first) & ~63, hi = kr.end(i_last);
+    const int32_t all_end = kr.end(i_first), all_begin = kr.begin(i_last);  // what every row sees
+    const int32_t c0 = lo + split * pl.chunk, c1 = min(hi, c0 + pl.chunk);
+
+    // this lane's rows
+    int32_t end[NT], begin[NT];
+    u32x4 q[NT][KS][QP];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) dot += fp4_decode((x >> (4 * e)) & 15u) * s_q[8 * w + e];
-                }
-                s = dot * c.k_scale[head * c.page_size + at];
-                vs = c.v_scale[head * c.page_size + at];
-                vb = v_byte(c, head, at, 0);
+    for (int t = 0; t < NT; ++t) {
+        const int32_t row = min(first + 16 * t + r16, n_rows - 1), i = row / group;
+        end[t] = kr.end(i);
+        begin[t] = kr.begin(i);
+        const int64_t token = q0 + i;
+        const T *src = (const T *)a.q + (token < a.tokens ? token * a.q_token_stride : 0) +
+                       (h * group + (row - i * group)) * a.q_head_stride + g * (D / 4);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = pl.negative ? -(float)src[8 * s + j] : (float)src[8 * s + j];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t w = pack_bf16(x[2 * j], x[2 * j + 1]);
+                q[t][s][0][j] = w;
+                if (QP == 2) q[t][s][QP - 1][j] = pack_bf16(x[2 * j] - bf16_lo(w), x[2 * j + 1] - bf16_hi(w));
             }
         }
-        const float m_new = fmaxf(m, wave_max(s));
-        // no key seen yet: exp(-inf - -inf) would be NaN
-        const float ref = m_new == -INFINITY ? 0.0f : m_new;
-        const float keep = __expf(m - ref), p = vb >= 0 ? __expf(s - ref) : 0.0f;
-        l = l * keep + wave_sum(p);
-        m = m_new;
-        s_p[lane] = vb >= 0 ? p * vs : 0.0f;
-        s_v[lane] = vb;
-        __syncthreads();
-        for (int e = 0; e < 4; ++e) o[e] *= keep;
-        for (int b = lane, e = 0; b < d / 2; b += 64, e += 2)
-            for (int k = 0; k < 64; ++k) {
-                if (s_v[k] < 0) continue;
-                const uint32_t x = c.v[s_v[k] + 16 * b];
-                o[e] += s_p[k] * fp4_decode(x & 15u);
-                o[e + 1] += s_p[k] * fp4_decode(x >> 4);
+    }
+
+    float m[NT], l[NT];  // m in units of c; l this lane's keys only
+    f32x4 o[NT][CT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        m[t] = -INFINITY;
+        l[t] = 0.0f;
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) o[t][ct][0] = o[t][ct][1] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    const int32_t *table = a.block_table + (int64_t)req * a.table_width;
+    const int32_t stride = BY_KEYS ? 64 * WAVES : 64;
+    for (int32_t key = c0 + (BY_KEYS ? 64 * wave : 0); key < c1; key += stride) {
+        // the 16 keys of this lane group: where they lie, in groups of 16
+        const int32_t mine = (key >> 4) + g;
+        const bool there = 16 * mine < kr.cap;
+        const int32_t pi = pl.page_shift >= 0 ? mine >> pl.page_shift : mine / pl.groups_per_page;
+        const int32_t page = there ? table[pi] : -1;
+        const bool held = page >= 0 && page < cache.n_pages;
+        const int32_t at = ((held ? page : 0) * H + h) * pl.groups_per_page + (held ? mine - pi * pl.groups_per_page : 0);
+        const int32_t kat = __shfl(at, (r16 >> 2) << 4, 64);
+        const uint8_t *kp = cache.k + ((int64_t)kat * 16 + (r16 & 3)) * (D / 2) + g * (D / 8);
+        const uint8_t *vp = cache.v + (int64_t)at * (16 * (D / 2)) + r16 * 16;
+        uint32_t kw[4][KS];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const uint8_t *p = kp + 4 * x * (D / 2);
+            if constexpr (D == 64) {
+                const uint2 w = *reinterpret_cast<const uint2 *>(p);
+                kw[x][0] = w.x;
+                kw[x][1] = w.y;
+            } else {
+#pragma unroll
+                for (int s = 0; s < KS; s += 4) {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(p + 4 * s);
+                    kw[x][s] = w.x;
+                    kw[x][s + 1] = w.y;
+                    kw[x][s + 2] = w.z;
+                    kw[x][s + 3] = w.w;
+                }
             }
+        }
+        float4 ks[4], vs[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            ks[x] = reinterpret_cast<const float4 *>(cache.k_scale + (int64_t)at * 16)[x];
+            vs[x] = reinterpret_cast<const float4 *>(cache.v_scale + (int64_t)at * 16)[x];
+        }
+        uint4 vw[CT];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) vw[ct] = *reinterpret_cast<const uint4 *>(vp + ct * 256);
+
+        f32x4 sc[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) sc[t][x] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const u32x4 kk = codes8(kw[x][s]);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    sc[t][x] = mma(kk, q[t][s][0], sc[t][x]);
+                    if (QP == 2) sc[t][x] = mma(kk, q[t][s][QP - 1], sc[t][x]);
+                }
+            }
+        // wave-uniform: every row sees every key of the step
+        const bool whole = key >= all_begin && key + 64 <= all_end && __all(held);
+        u32x4 p[NT][2][PP];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            float v[16], w[16];  // scores, then weights, of keys 16 g + 0 .. 15
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                v[4 * x] = sc[t][x][0] * ks[x].x;
+                v[4 * x + 1] = sc[t][x][1] * ks[x].y;
+                v[4 * x + 2] = sc[t][x][2] * ks[x].z;
+                v[4 * x + 3] = sc[t][x][3] * ks[x].w;
+            }
+            if (!whole) {
+                const int32_t from = held ? begin[t] - (key + 16 * g) : 16, to = end[t] - (key + 16 * g);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] = j >= from && j < to ? v[j] : -INFINITY;
+            }
+            float top = v[0];
+#pragma unroll
+            for (int j = 1; j < 16; ++j) top = fmaxf(top, v[j]);
+            top *= pl.c;
+            if (__any(top > m[t] + SLACK)) {
+                const float up = fmaxf(m[t], lanes_max(top));
+                // a row without a key so far keeps m = -inf, and factor 1 on its zeros
+                const float keep = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[t] - up);
+                m[t] = up;
+                l[t] *= keep;
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct) {
+                    o[t][ct][0] *= keep;
+                    o[t][ct][1] *= keep;
+                }
+            }
+            const float ref = m[t] == -INFINITY ? 0.0f : m[t];
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(v[j], pl.c, -ref));
+                sum += w[j];
+            }
+            l[t] += sum;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                w[4 * x] *= vs[x].x;
+                w[4 * x + 1] *= vs[x].y;
+                w[4 * x + 2] *= vs[x].z;
+                w[4 * x + 3] *= vs[x].w;
+            }
+            if (!whole) {
+                // a key that this row does not see may hold anything
+#pragma unroll
+                for (int j = 0; j < 16; ++j) w[j] = v[j] == -INFINITY ? 0.0f : w[j];
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float x = w[8 * e + 2 * j], y = w[8 * e + 2 * j + 1];
+                    const uint32_t b = pack_bf16(x, y);
+                    p[t][e][0][j] = b;
+                    if (PP == 2) p[t][e][PP - 1][j] = pack_bf16(x - bf16_lo(b), y - bf16_hi(b));
+                }
+        }
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                uint32_t e0[2], o0[2], e1[2], o1[2];
+                codes_by_channel(e ? vw[ct].z : vw[ct].x, e0, o0);
+                codes_by_channel(e ? vw[ct].w : vw[ct].y, e1, o1);
+                const u32x4 even = {e0[0], e0[1], e1[0], e1[1]}, odd = {o0[0], o0[1], o1[0], o1[1]};
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int y = 0; y < PP; ++y) {
+                        o[t][ct][0] = mma(even, p[t][e][y], o[t][ct][0]);
+                        o[t][ct][1] = mma(odd, p[t][e][y], o[t][ct][1]);
+                    }
+            }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) l[t] = lanes_sum(l[t]);
+
+    // lane: row r16, channels 32 ct + 8 g + 2 i + (even, odd)
+    if (BY_KEYS) {
+        constexpr int ROWS = 16 * NT;
+        float *s_o = s_join, *s_m = s_join + WAVES * ROWS * D, *s_l = s_m + WAVES * ROWS;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            if (first + 16 * t + r16 >= n_rows) continue;
+            float *dst = s_o + (wave * ROWS + 16 * t + r16) * D + 8 * g;
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    dst[32 * ct + 2 * i] = o[t][ct][0][i];
+                    dst[32 * ct + 2 * i + 1] = o[t][ct][1][i];
+                }
+            if (g == 0) {
+                s_m[wave * ROWS + 16 * t + r16] = m[t];
+                s_l[wave * ROWS + 16 * t + r16] = l[t];
+            }
+        }
         __syncthreads();
+        const int rows = min(ROWS, n_rows - first);
+        for (int at = threadIdx.x; at < rows * (D / 4); at += 64 * WAVES) {
+            const int row = at / (D / 4), ch = 4 * (at - row * (D / 4));
+            float mm = -INFINITY, ll = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int w = 0; w < WAVES; ++w) mm = fmaxf(mm, s_m[w * ROWS + row]);
+            for (int w = 0; w < WAVES; ++w) {
+                const float mw = s_m[w * ROWS + row];
+                const float f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - mm);
+                if (f == 0.0f && s_l[w * ROWS + row] == 0.0f) continue;
+                ll += f * s_l[w * ROWS + row];
+                const float4 x = *reinterpret_cast<const float4 *>(s_o + (w * ROWS + row) * D + ch);
+                acc[0] += f * x.x;
+                acc[1] += f * x.y;
+                acc[2] += f * x.z;
+                acc[3] += f * x.w;
+            }
+            const int64_t token = q0 + (first + row) / group;
+            const int64_t qh = h * group + (first + row) % group;
+            if (token >= a.tokens) continue;
+            if (pl.splits > 1) {
+                const int64_t slot = (token * a.q_heads + qh) * pl.splits + split;
+                if (ll != 0.0f) *reinterpret_cast<float4 *>(pl.part_o + slot * D + ch) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+                if (ch == 0) pl.part_ml[slot] = make_float2(mm, ll);
+            } else {
+                const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
+                T *out = (T *)a.out + token * a.out_token_stride + qh * a.out_head_stride + ch;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) out[j] = (T)(acc[j] * inv);
+                if (a.lse && ch == 0)
+                    a.lse[token * a.q_heads + qh] = ll != 0.0f ? (mm + __builtin_amdgcn_logf(ll)) * 0.69314718f : -INFINITY;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int32_t row = first + 16 * t + r16;
+            const int64_t token = q0 + row / group, qh = h * group + row % group;
+            if (row >= n_rows || token >= a.tokens) continue;
+            if (pl.splits > 1) {
+                const int64_t slot = (token * a.q_heads + qh) * pl.splits + split;
+                float *dst = pl.part_o + slot * D + 8 * g;
+                if (l[t] != 0.0f)
+#pragma unroll
+                    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            dst[32 * ct + 2 * i] = o[t][ct][0][i];
+                            dst[32 * ct + 2 * i + 1] = o[t][ct][1][i];
+                        }
+                if (g == 0) pl.part_ml[slot] = make_float2(m[t], l[t]);
+            } else {
+                const float inv = l[t] != 0.0f ? 1.0f / l[t] : 0.0f;
+                T *out = (T *)a.out + token * a.out_token_stride + qh * a.out_head_stride + 8 * g;
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        out[32 * ct + 2 * i] = (T)(o[t][ct][0][i] * inv);
+                        out[32 * ct + 2 * i + 1] = (T)(o[t][ct][1][i] * inv);
+                    }
+                if (a.lse && g == 0)
+                    a.lse[token * a.q_heads + qh] = l[t] != 0.0f ? (m[t] + __builtin_amdgcn_logf(l[t])) * 0.69314718f : -INFINITY;
+            }
+        }
     }
-    T *out = (T *)a.out + t * a.out_token_stride + qh * a.out_head_stride;
-    for (int b = lane, e = 0; b < d / 2; b += 64, e += 2) {
-        out[2 * b] = (T)(l != 0.0f ? o[e] / l : 0.0f);
-        out[2 * b + 1] = (T)(l != 0.0f ? o[e + 1] / l : 0.0f);
+}
+
+// Joins the splits of a row: a block a (token, query head); D / 4 threads share
+// a split's channels, and the block's thread groups take every GROUPS-th split.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void k_attend_join(sili_kv4_attend_args a, AttendPlan pl) {
+    constexpr int GROUPS = 256 / (D / 4);
+    __shared__ float4 s_acc[256];
+    __shared__ float s_w[4], s_l[4];
+    const int64_t id = blockIdx.x, token = id / a.q_heads, qh = id - token * a.q_heads;
+    if (token < a.q_start[0] || token >= a.q_start[a.requests]) return;
+    const int64_t req = request_of(a.q_start, a.requests, token);
+    const int32_t q0 = a.q_start[req], n = min(a.q_start[req + 1] - q0, (int32_t)a.max_new);
+    const int64_t rows = n * (a.q_heads / a.cache.kv_heads);
+    if (token - q0 >= n || rows <= pl.few || rows > pl.many) return;
+    const float2 *ml = pl.part_ml + id * pl.splits;
+    float m = -INFINITY;
+    for (int s = threadIdx.x; s < pl.splits; s += 256) m = fmaxf(m, ml[s].x);
+    m = wave_max(m);
+    if ((threadIdx.x & 63) == 0) s_w[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(s_w[0], s_w[1]), fmaxf(s_w[2], s_w[3]));
+    const int part = threadIdx.x / (D / 4), ch = 4 * (threadIdx.x % (D / 4));
+    float l = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int s = part; s < pl.splits; s += GROUPS) {
+        const float2 x = ml[s];
+        if (x.y == 0.0f) continue;  // no key, and no sums written
+        const float f = __builtin_amdgcn_exp2f(x.x - m);
+        const float4 v = *reinterpret_cast<const float4 *>(pl.part_o + (id * pl.splits + s) * D + ch);
+        l += f * x.y;
+        acc.x += f * v.x;
+        acc.y += f * v.y;
+        acc.z += f * v.z;
+        acc.w += f * v.w;
     }
-    if (a.lse && lane == 0) a.lse[t * a.q_heads + qh] = l != 0.0f ? m + __logf(l) : -INFINITY;
+    s_acc[threadIdx.x] = acc;
+    __shared__ float s_sum[GROUPS];
+    if (ch == 0) s_sum[part] = l;
+    __syncthreads();
+    if (part != 0) return;
+    l = 0.0f;
+    acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int k = 0; k < GROUPS; ++k) {
+        const float4 v = s_acc[k * (D / 4) + threadIdx.x];
+        l += s_sum[k];
+        acc.x += v.x;
+        acc.y += v.y;
+        acc.z += v.z;
+        acc.w += v.w;
+    }
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    T *out = (T *)a.out + token * a.out_token_stride + qh * a.out_head_stride + ch;
+    out[0] = (T)(acc.x * inv);
+    out[1] = (T)(acc.y * inv);
+    out[2] = (T)(acc.z * inv);
+    out[3] = (T)(acc.w * inv);
+    if (a.lse && ch == 0) a.lse[id] = l != 0.0f ? (m + __builtin_amdgcn_logf(l)) * 0.69314718f : -INFINITY;
 }
 
 void check_cache(const sili_kv4_cache &c, const char *what) {
@@ -199,7 +565,9 @@ void check_attend(const sili_kv4_attend_args &a) {
     require(a.requests >= 0 && a.requests <= 65535, "kv4_attend: requests out of range");
     require(a.tokens >= 0 && a.tokens < (int64_t(1) << 31), "kv4_attend: tokens out of range");
     require(a.q_heads >= 1 && a.q_heads % a.cache.kv_heads == 0, "kv4_attend: q_heads is no multiple of kv_heads");
-    require(a.q_heads <= 65535, "kv4_attend: too many query heads");
+    require(a.q_heads <= 65535 && a.tokens * a.q_heads <= INT32_MAX, "kv4_attend: too many query heads");
+    require(a.cache.n_pages * (a.cache.page_size / 16) * a.cache.kv_heads <= INT32_MAX, "kv4_attend: cache too large");
+    require(a.max_new * (a.q_heads / a.cache.kv_heads) <= INT32_MAX, "kv4_attend: too many rows");
     require(a.table_width >= 0 && a.max_new >= 0 && a.max_len >= 0, "kv4_attend: negative size");
     require(a.max_len < (int64_t(1) << 31) && a.max_new < (int64_t(1) << 31), "kv4_attend: bound out of range");
     require(a.window >= 0 && (a.window == 0 || a.causal), "kv4_attend: a window needs the causal mask");
@@ -210,9 +578,87 @@ void check_attend(const sili_kv4_attend_args &a) {
 void kv4_append(const sili_kv4_rows_args &a, hipStream_t st) { rows<true>(a, st, "kv4_append"); }
 void kv4_read(const sili_kv4_rows_args &a, hipStream_t st) { rows<false>(a, st, "kv4_read"); }
 
+
+namespace {
+
+// Requests of up to FEW_ROWS rows have their keys shared by a block's waves, a
+// row tile of 16 each; larger ones give each wave rows of its own.
+constexpr int32_t FEW_ROWS = 64;
+constexpr int NT_MANY = 2;
+
+struct Launch {
+    bool on = false;
+    int64_t tiles = 0;  // row tiles of a (request, kv head)
+    AttendPlan plan{};
+};
+
+// The two launches of a call (few rows, many rows).  Keys are split until the
+// blocks fill the GPU, a split not below 256 keys.
+void plan_attend(const sili_kv4_attend_args &a, Launch (&out)[2]) {
+    const int64_t group = a.q_heads / a.cache.kv_heads, rows = a.max_new * group;
+    const int64_t gpp = a.cache.page_size / 16;
+    for (int k = 0; k < 2; ++k) {
+        Launch &L = out[k];
+        AttendPlan &p = L.plan;
+        p.groups_per_page = (int32_t)gpp;
+        p.page_shift = (gpp & (gpp - 1)) == 0 ? (int32_t)__builtin_ctzll((unsigned long long)gpp) : -1;
+        // a scale of zero leaves all scores equal; c > 0 keeps hidden ones at -inf
+        p.c = std::max(std::fabs(a.scale) * 1.44269504f, 0x1p-100f);
+        p.negative = a.scale < 0.0f;
+        p.few = k == 0 ? 0 : FEW_ROWS;
+        p.many = k == 0 ? FEW_ROWS : INT32_MAX;
+        L.on = k == 0 || rows > FEW_ROWS;
+        const int64_t tile_rows = k == 0 ? 16 : 16 * NT_MANY * WAVES;
+        L.tiles = (std::min<int64_t>(rows, p.many) + tile_rows - 1) / tile_rows;
+        // keys a row tile can reach: its rows' windows, aligned to 64
+        int64_t reach = a.max_len;
+        if (a.window > 0) reach = std::min(reach, a.window + (tile_rows - 1) / group + 1 + 63);
+        const int64_t step = k == 0 ? 64 * WAVES : 64;
+        const int64_t blocks = std::max<int64_t>(1, a.requests * a.cache.kv_heads * L.tiles);
+        const int64_t want = std::clamp<int64_t>(2048 / blocks, 1, std::max<int64_t>(1, (reach + 255) / 256));
+        p.chunk = (int32_t)std::max<int64_t>(step, ((reach + want - 1) / want + step - 1) / step * step);
+        p.splits = (int32_t)std::max<int64_t>(1, (reach + p.chunk - 1) / p.chunk);
+        if (!L.on) p.splits = 1;
+    }
+}
+
+size_t part_bytes(const sili_kv4_attend_args &a, const Launch &L) {
+    if (!L.on || L.plan.splits == 1) return 0;
+    return (size_t)a.tokens * (size_t)a.q_heads * (size_t)L.plan.splits * ((size_t)a.cache.head_dim * sizeof(float) + sizeof(float2));
+}
+
+template <typename T, int D>
+void run_attend(const sili_kv4_attend_args &a, Launch (&L)[2], hipStream_t st) {
+    char *work = static_cast<char *>(a.workspace);
+    for (int k = 0; k < 2; ++k) {
+        if (!L[k].on) continue;
+        AttendPlan &p = L[k].plan;
+        const int64_t parts = a.tokens * a.q_heads * p.splits;
+        if (p.splits > 1) {
+            p.part_o = reinterpret_cast<float *>(work);
+            p.part_ml = reinterpret_cast<float2 *>(work + parts * D * sizeof(float));
+            work += part_bytes(a, L[k]);
+        }
+        const int64_t x = L[k].tiles * a.cache.kv_heads;
+        require(x <= INT32_MAX && p.splits <= 65535, "kv4_attend: too many rows or keys");
+        const dim3 grid((unsigned)x, (unsigned)p.splits, (unsigned)a.requests);
+        if (k == 0) {
+            const uint32_t lds = WAVES * 16 * (D + 2) * sizeof(float);
+            launch(k_attend<T, D, 1, true>, grid, dim3(64 * WAVES), lds, st, a, p);
+        } else {
+            launch(k_attend<T, D, NT_MANY, false>, grid, dim3(64 * WAVES), 0, st, a, p);
+        }
+        if (p.splits > 1) launch(k_attend_join<T, D>, dim3((unsigned)(a.tokens * a.q_heads)), dim3(256), 0, st, a, p);
+    }
+}
+
+}  // namespace
+
 size_t kv4_attend_workspace(const sili_kv4_attend_args &a) {
     check_attend(a);
-    return 0;
+    Launch L[2];
+    plan_attend(a, L);
+    return part_bytes(a, L[0]) + part_bytes(a, L[1]);
 }
 
 void kv4_attend(const sili_kv4_attend_args &a, hipStream_t st) {
@@ -220,8 +666,18 @@ void kv4_attend(const sili_kv4_attend_args &a, hipStream_t st) {
     if (a.tokens == 0 || a.requests == 0 || a.max_new == 0) return;
     require(a.q && a.out && a.q_start && a.kv_lens, "kv4_attend: NULL buffer");
     require(a.block_table || a.table_width == 0, "kv4_attend: NULL block_table");
+    Launch L[2];
+    plan_attend(a, L);
+    const size_t need = part_bytes(a, L[0]) + part_bytes(a, L[1]);
+    require(need == 0 || (a.workspace && aligned(a.workspace, 16) && a.workspace_bytes >= need),
+            "kv4_attend: workspace too small or not 16-byte aligned");
     with_dtype(a.dtype, [&](auto z) {
-        launch(k_kv4_attend<decltype(z)>, dim3((unsigned)a.tokens, (unsigned)a.q_heads), dim3(64), 0, st, a);
+        using T = decltype(z);
+        switch (a.cache.head_dim) {
+            case 64: run_attend<T, 64>(a, L, st); break;
+            case 128: run_attend<T, 128>(a, L, st); break;
+            default: run_attend<T, 256>(a, L, st); break;
+        }
     });
     SILI_HIP(hipGetLastError());
 }
