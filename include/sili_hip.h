@@ -732,8 +732,9 @@ int sili_kv4_read(const sili_kv4_rows_args *args, void *stream);
  * max_new and max_len bound the requests' query tokens and key counts (host
  * values; they size the grid): queries past max_new are not computed, keys past
  * max_len not seen.  A table entry outside the cache hides its page's keys.
- * fp32 inputs are multiplied in two bf16 parts each (16 significant bits),
- * bf16 inputs exactly; codes are exact in bf16.  workspace: device memory of
+ * Products run on the bf16 matrix cores: the codes are exact there, q and the
+ * softmax weights enter in as many bf16 parts as their type has bits (fp32 three,
+ * f16 two, bf16 one or two), and sums are fp32.  workspace: device memory of
  * sili_kv4_attend_workspace(args) bytes, 16-byte aligned; calls that overlap
  * need one each. */
 typedef struct {

@@ -8,6 +8,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <utility>
 
 namespace sili {
 
@@ -82,17 +83,6 @@ __global__ __launch_bounds__(ROWS_TPB) void k_kv4_rows(sili_kv4_rows_args a) {
     }
 }
 
-// The request of query token t: the last that begins at or before it.
-__device__ __forceinline__ int64_t request_of(const int32_t *start, int64_t n, int64_t t) {
-    int64_t lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (start[mid] <= t) lo = mid;
-        else hi = mid;
-    }
-    return lo;
-}
-
 // ---- attention -----------------------------------------------------------------
 //
 // Rows of a (request, kv head) are its query tokens times the group of query
@@ -116,7 +106,6 @@ __device__ __forceinline__ int64_t request_of(const int32_t *start, int64_t n, i
 //
 // The running maximum m is raised only when a score passes it by 2^8 (in exp2's
 // argument 8): until then weights stay below 2^8 and nothing has to be rescaled.
-constexpr int WAVES = 4;
 constexpr float SLACK = 8.0f;
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
@@ -148,6 +137,13 @@ __device__ __forceinline__ void codes_by_channel(uint32_t w, uint32_t (&even)[2]
     even[1] = __builtin_amdgcn_perm(d, c, 0x05040100u);
     odd[1] = __builtin_amdgcn_perm(d, c, 0x07060302u);
 }
+// x[j] *= what lane j of this row of 16 lanes holds (DPP row_newbcast, folded
+// into the product).
+template <int... J>
+__device__ __forceinline__ void times_row(float (&x)[16], float s, std::integer_sequence<int, J...>) {
+    ((x[J] *= dpp_f32<0x150 + J>(s)), ...);
+}
+__device__ __forceinline__ void times_scales(float (&x)[16], float s) { times_row(x, s, std::make_integer_sequence<int, 16>{}); }
 __device__ __forceinline__ float lanes_max(float v) {  // over the four lanes of a row
     v = fmaxf(v, __shfl_xor(v, 16, 64));
     return fmaxf(v, __shfl_xor(v, 32, 64));
@@ -157,17 +153,75 @@ __device__ __forceinline__ float lanes_sum(float v) {
     return v + __shfl_xor(v, 32, 64);
 }
 
+// bf16 parts of q: 24 bits of fp32, all 11 of f16, all 8 of bf16.
+template <typename T>
+constexpr int q_parts() { return sizeof(T) == 4 ? 3 : __is_same(T, __bf16) ? 1 : 2; }
+// ... of p: 24 bits for fp32, 16 for f16.  bf16 takes one where the matrix
+// cores' time counts (its rounding is as large as the output's own, together
+// 1.4 times that), two where memory bounds the kernel.
+template <typename T, bool BY_KEYS>
+constexpr int p_parts() { return sizeof(T) == 4 ? 3 : __is_same(T, __bf16) && !BY_KEYS ? 1 : 2; }
+// x, y in N parts: part k the bf16 nearest to what the parts before leave.
+template <int N>
+__device__ __forceinline__ void split_bf16(float x, float y, uint32_t (&part)[N]) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        part[k] = pack_bf16(x, y);
+        x -= bf16_lo(part[k]);
+        y -= bf16_hi(part[k]);
+    }
+}
+
+// The part of this lane's column: take[k] is all ones for part k's columns.
+template <int N>
+__device__ __forceinline__ uint32_t pick(const uint32_t (&part)[N], const uint32_t (&take)[N]) {
+    uint32_t w = part[0] & take[0];
+#pragma unroll
+    for (int k = 1; k < N; ++k) w |= part[k] & take[k];
+    return w;
+}
+// Sum over the CP columns of a row, 16 / CP lanes apart in their 16.
+template <int CP>
+__device__ __forceinline__ float columns_sum(float v) {
+    if (CP >= 2) v += dpp_f32<DPP_ROW_ROR8>(v);
+    if (CP >= 4) v += dpp_f32<DPP_ROW_ROR4>(v);
+    return v;
+}
+
 // How a launch cuts the work, set on the host.
 struct AttendPlan {
+    int32_t kv_heads, group;  // query heads a kv head
+    uint32_t group_inv;       // floor(2^32 / group), at most 2^32 - 1
+    int32_t n_pages, most;    // pages of the cache; keys that max_len and the table allow
+    bool q_packed, out_packed;  // rows of q in 16-byte pieces; of out in pieces of 4 elements
     int32_t groups_per_page;  // page_size / 16
     int32_t page_shift;       // its logarithm, or -1
-    int32_t splits, chunk;    // keys a split takes (a multiple of 64 WAVES or of 64)
+    int32_t splits, chunk;    // keys a split takes: a multiple of a block's step
+    int32_t waves;            // of a block whose waves share rows
+    int32_t join_rows;        // rows such a block joins at most
+    int32_t columns;          // columns a row takes
     int32_t few, many;        // takes requests of more than `few` rows, up to `many`
     float c;                  // |scale| log2(e)
     bool negative;            // scale < 0: the sign goes to q
     float *part_o;            // [tokens * q_heads][splits][D], unnormalised
     float2 *part_ml;          // [tokens * q_heads][splits]: m c, l
 };
+
+// The query token of a row: row / group (the estimate is at most one too low).
+__device__ __forceinline__ int32_t token_of(const AttendPlan &pl, int32_t row) {
+    const int32_t q = (int32_t)__umulhi((uint32_t)row, pl.group_inv);
+    return q + (row - q * pl.group >= pl.group ? 1 : 0);
+}
+// Four channels of an output row.
+template <typename T>
+__device__ __forceinline__ void store4(T *out, const float (&x)[4], bool packed) {
+    if (packed) {
+        store_pack<T, 4>(out, x);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) out[j] = (T)x[j];
+    }
+}
 
 // Keys that query i of n sees, [begin, end).
 struct KeyRange {
@@ -177,58 +231,103 @@ struct KeyRange {
     __device__ __forceinline__ int32_t begin(int32_t i) const { return window > 0 ? max(0, base + i + 1 - window) : 0; }
 };
 
+// Registers allow this many waves on a SIMD.
+template <typename T, int D, bool BY_KEYS>
+constexpr int waves_per_simd() {
+    if (!BY_KEYS) return 1;
+    return (D == 64 ? 4 : D == 128 ? 3 : 2) - (__is_same(T, __bf16) ? 0 : 1);
+}
+
 // BY_KEYS: the block's waves share 16 NT rows and take every fourth step of
 // keys each; their results are joined in LDS.  Otherwise each wave has rows of
 // its own.
-template <typename T, int D, int NT, bool BY_KEYS>
-__global__ __launch_bounds__(64 * WAVES) void k_attend(sili_kv4_attend_args a, AttendPlan pl) {
-    constexpr int QP = sizeof(T) == 2 && __is_same(T, __bf16) ? 1 : 2;  // parts of q
-    constexpr int PP = sizeof(T) == 4 ? 2 : 1;                          // parts of p
+//
+// CP > 1: with 16 / CP rows at most, the parts of q and p go to the columns that
+// would be empty instead of to products of their own: column r + (16 / CP) k
+// holds part k of row r.  Scores are summed over a row's columns (rotations
+// within 16 lanes), so every one of them holds the row's weights and takes its
+// own part of them; the outputs are summed once, at the end.
+template <typename T, int D, int NT, bool BY_KEYS, int WAVES, int CP = 1>
+__global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, BY_KEYS>())) void k_attend(sili_kv4_attend_args a, AttendPlan pl) {
+    constexpr int QP = q_parts<T>(), PP = p_parts<T, BY_KEYS>();
     constexpr int KS = D / 32;   // steps of 32 channels
     constexpr int CT = D / 32;   // blocks of 32 output channels
+    constexpr int RT = 16 / CP;  // rows of a tile
+    constexpr int QM = CP > 1 ? 1 : QP, PM = CP > 1 ? 1 : PP;  // products each
+    static_assert(CP == 1 || (BY_KEYS && NT == 1 && CP >= QP && CP >= PP), "parts fit the columns");
     extern __shared__ float s_join[];
     const sili_kv4_cache &cache = a.cache;
     const int wave = (int)uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, r16 = lane & 15;
-    const int H = (int)cache.kv_heads, group = (int)(a.q_heads / H);
+    const int my_row = r16 % RT, my_part = r16 / RT;
+    const int H = pl.kv_heads, group = pl.group;
     const int h = blockIdx.x % H, tile = blockIdx.x / H, split = blockIdx.y, req = blockIdx.z;
+    const int32_t *table = a.block_table + (int64_t)req * a.table_width;
+    const int32_t stride = BY_KEYS ? 64 * WAVES : 64;
+    // the page of the first step, asked for before the lengths are here (the
+    // table has the entry whatever they say)
+    int32_t key = split * pl.chunk + (BY_KEYS ? 64 * wave : 0);
+    auto entry = [&](int32_t k) {
+        const int32_t mine = (k >> 4) + g;
+        return table[pl.page_shift >= 0 ? mine >> pl.page_shift : mine / pl.groups_per_page];
+    };
+    int32_t page = -1;
+    if (a.window == 0 && key + 16 * g < pl.most) page = entry(key);
+
     const int32_t q0 = a.q_start[req];
     const int32_t n_all = a.q_start[req + 1] - q0, n = min(n_all, (int32_t)a.max_new);
+    const int32_t kv = a.kv_lens[req];
     const int32_t n_rows = n * group;
-    const int32_t first = (BY_KEYS ? tile : tile * WAVES + wave) * (16 * NT);
+    const int32_t first = (BY_KEYS ? tile : tile * WAVES + wave) * (RT * NT);
     if (q0 < 0 || n_rows <= pl.few || n_rows > pl.many) return;
     if (first >= n_rows) return;  // BY_KEYS: the whole block
-    const int32_t kv = a.kv_lens[req];
     KeyRange kr;
     kr.base = kv - n_all;
     kr.window = (int32_t)a.window;
     kr.causal = a.causal != 0;
-    kr.cap = cache.n_pages == 0 ? 0 : (int32_t)min(min((int64_t)kv, a.max_len), a.table_width * cache.page_size);
-    const int32_t i_first = first / group, i_last = min(first + 16 * NT - 1, n_rows - 1) / group;
+    kr.cap = min(kv, pl.most);
+    const int32_t i_first = token_of(pl, first), i_last = token_of(pl, min(first + RT * NT - 1, n_rows - 1));
     const int32_t lo = kr.begin(i_first) & ~63, hi = kr.end(i_last);
     const int32_t all_end = kr.end(i_first), all_begin = kr.begin(i_last);  // what every row sees
     const int32_t c0 = lo + split * pl.chunk, c1 = min(hi, c0 + pl.chunk);
 
+    uint32_t take_q[QP], take_p[PP];  // CP > 1: the part this lane's column holds
+#pragma unroll
+    for (int k = 0; k < QP; ++k) take_q[k] = my_part == k ? ~0u : 0u;
+#pragma unroll
+    for (int k = 0; k < PP; ++k) take_p[k] = my_part == k ? ~0u : 0u;
+
     // this lane's rows
     int32_t end[NT], begin[NT];
-    u32x4 q[NT][KS][QP];
+    u32x4 q[NT][KS][QM];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const int32_t row = min(first + 16 * t + r16, n_rows - 1), i = row / group;
+        const int32_t row = min(first + 16 * t + my_row, n_rows - 1), i = token_of(pl, row);
         end[t] = kr.end(i);
         begin[t] = kr.begin(i);
         const int64_t token = q0 + i;
         const T *src = (const T *)a.q + (token < a.tokens ? token * a.q_token_stride : 0) +
                        (h * group + (row - i * group)) * a.q_head_stride + g * (D / 4);
+        float xs[KS][8];
+        if (pl.q_packed) {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) load_pack<T, 8>(src + 8 * s, xs[s]);
+        } else {
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) xs[s][j] = (float)src[8 * s + j];
+        }
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             float x[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = pl.negative ? -(float)src[8 * s + j] : (float)src[8 * s + j];
+            for (int j = 0; j < 8; ++j) x[j] = pl.negative ? -xs[s][j] : xs[s][j];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const uint32_t w = pack_bf16(x[2 * j], x[2 * j + 1]);
-                q[t][s][0][j] = w;
-                if (QP == 2) q[t][s][QP - 1][j] = pack_bf16(x[2 * j] - bf16_lo(w), x[2 * j + 1] - bf16_hi(w));
+                uint32_t part[QP];
+                split_bf16<QP>(x[2 * j], x[2 * j + 1], part);
+#pragma unroll
+                for (int k = 0; k < QM; ++k) q[t][s][k][j] = CP > 1 && QP > 1 ? pick<QP>(part, take_q) : part[k];
             }
         }
     }
@@ -243,20 +342,23 @@ __global__ __launch_bounds__(64 * WAVES) void k_attend(sili_kv4_attend_args a, A
         for (int ct = 0; ct < CT; ++ct) o[t][ct][0] = o[t][ct][1] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    const int32_t *table = a.block_table + (int64_t)req * a.table_width;
-    const int32_t stride = BY_KEYS ? 64 * WAVES : 64;
-    for (int32_t key = c0 + (BY_KEYS ? 64 * wave : 0); key < c1; key += stride) {
-        // the 16 keys of this lane group: where they lie, in groups of 16
-        const int32_t mine = (key >> 4) + g;
-        const bool there = 16 * mine < kr.cap;
-        const int32_t pi = pl.page_shift >= 0 ? mine >> pl.page_shift : mine / pl.groups_per_page;
-        const int32_t page = there ? table[pi] : -1;
-        const bool held = page >= 0 && page < cache.n_pages;
-        const int32_t at = ((held ? page : 0) * H + h) * pl.groups_per_page + (held ? mine - pi * pl.groups_per_page : 0);
+    // The keys of a step as this lane needs them, loaded a step ahead: a part's
+    // registers take the next step's as soon as this one's are used.
+    uint32_t kw[4][KS];
+    float ks, vs;  // scales of key 16 g + r16: the products take them from their lane
+    uint4 vw[CT];
+    bool held;   // the 16 keys of this lane group are in the cache
+    int32_t at;  // where they lie, in groups of 16 keys
+    auto page_of = [&](int32_t k) -> int32_t { return k + 16 * g < kr.cap ? entry(k) : -1; };
+    auto locate = [&](int32_t k) {
+        const int32_t mine = (k >> 4) + g;
+        held = page >= 0 && page < pl.n_pages && k + 16 * g < kr.cap;
+        const int32_t in_page = pl.page_shift >= 0 ? mine & (pl.groups_per_page - 1) : mine % pl.groups_per_page;
+        at = held ? (page * H + h) * pl.groups_per_page + in_page : h * pl.groups_per_page;
+    };
+    auto load_k = [&] {
         const int32_t kat = __shfl(at, (r16 >> 2) << 4, 64);
         const uint8_t *kp = cache.k + ((int64_t)kat * 16 + (r16 & 3)) * (D / 2) + g * (D / 8);
-        const uint8_t *vp = cache.v + (int64_t)at * (16 * (D / 2)) + r16 * 16;
-        uint32_t kw[4][KS];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
             const uint8_t *p = kp + 4 * x * (D / 2);
@@ -275,16 +377,25 @@ __global__ __launch_bounds__(64 * WAVES) void k_attend(sili_kv4_attend_args a, A
                 }
             }
         }
-        float4 ks[4], vs[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            ks[x] = reinterpret_cast<const float4 *>(cache.k_scale + (int64_t)at * 16)[x];
-            vs[x] = reinterpret_cast<const float4 *>(cache.v_scale + (int64_t)at * 16)[x];
-        }
-        uint4 vw[CT];
+    };
+    auto load_v = [&] {
+        ks = cache.k_scale[(int64_t)at * 16 + r16];
+        vs = cache.v_scale[(int64_t)at * 16 + r16];
+        const uint8_t *vp = cache.v + (int64_t)at * (16 * (D / 2)) + r16 * 16;
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) vw[ct] = *reinterpret_cast<const uint4 *>(vp + ct * 256);
-
+    };
+    if (a.window > 0) {
+        key += lo;
+        page = page_of(key);
+    }
+    if (key < c1) {
+        locate(key);
+        load_k();
+        load_v();
+        page = page_of(key + stride);
+    }
+    for (; key < c1; key += stride) {
         f32x4 sc[NT][4];
 #pragma unroll
         for (int t = 0; t < NT; ++t)
@@ -296,26 +407,30 @@ __global__ __launch_bounds__(64 * WAVES) void k_attend(sili_kv4_attend_args a, A
             for (int s = 0; s < KS; ++s) {
                 const u32x4 kk = codes8(kw[x][s]);
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    sc[t][x] = mma(kk, q[t][s][0], sc[t][x]);
-                    if (QP == 2) sc[t][x] = mma(kk, q[t][s][QP - 1], sc[t][x]);
-                }
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int k = 0; k < QM; ++k) sc[t][x] = mma(kk, q[t][s][k], sc[t][x]);
             }
         // wave-uniform: every row sees every key of the step
-        const bool whole = key >= all_begin && key + 64 <= all_end && __all(held);
-        u32x4 p[NT][2][PP];
+        const bool here = held, whole = key >= all_begin && key + 64 <= all_end && __all(here);
+        const bool more = key + stride < c1;
+        if (more) {
+            locate(key + stride);
+            load_k();
+            page = page_of(key + 2 * stride);
+        }
+        u32x4 p[NT][2][PM];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             float v[16], w[16];  // scores, then weights, of keys 16 g + 0 .. 15
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                v[4 * x] = sc[t][x][0] * ks[x].x;
-                v[4 * x + 1] = sc[t][x][1] * ks[x].y;
-                v[4 * x + 2] = sc[t][x][2] * ks[x].z;
-                v[4 * x + 3] = sc[t][x][3] * ks[x].w;
+            for (int j = 0; j < 16; ++j) {
+                v[j] = sc[t][j >> 2][j & 3];
+                if (QP > 1) v[j] = columns_sum<CP>(v[j]);
             }
+            times_scales(v, ks);
             if (!whole) {
-                const int32_t from = held ? begin[t] - (key + 16 * g) : 16, to = end[t] - (key + 16 * g);
+                const int32_t from = here ? begin[t] - (key + 16 * g) : 16, to = end[t] - (key + 16 * g);
 #pragma unroll
                 for (int j = 0; j < 16; ++j) v[j] = j >= from && j < to ? v[j] : -INFINITY;
             }
@@ -343,13 +458,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_attend(sili_kv4_attend_args a, A
                 sum += w[j];
             }
             l[t] += sum;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                w[4 * x] *= vs[x].x;
-                w[4 * x + 1] *= vs[x].y;
-                w[4 * x + 2] *= vs[x].z;
-                w[4 * x + 3] *= vs[x].w;
-            }
+            times_scales(w, vs);
             if (!whole) {
                 // a key that this row does not see may hold anything
 #pragma unroll
@@ -359,10 +468,10 @@ __global__ __launch_bounds__(64 * WAVES) void k_attend(sili_kv4_attend_args a, A
             for (int e = 0; e < 2; ++e)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float x = w[8 * e + 2 * j], y = w[8 * e + 2 * j + 1];
-                    const uint32_t b = pack_bf16(x, y);
-                    p[t][e][0][j] = b;
-                    if (PP == 2) p[t][e][PP - 1][j] = pack_bf16(x - bf16_lo(b), y - bf16_hi(b));
+                    uint32_t part[PP];
+                    split_bf16<PP>(w[8 * e + 2 * j], w[8 * e + 2 * j + 1], part);
+#pragma unroll
+                    for (int k = 0; k < PM; ++k) p[t][e][k][j] = CP > 1 ? pick<PP>(part, take_p) : part[k];
                 }
         }
 #pragma unroll
@@ -376,29 +485,38 @@ __global__ __launch_bounds__(64 * WAVES) void k_attend(sili_kv4_attend_args a, A
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
-                    for (int y = 0; y < PP; ++y) {
+                    for (int y = 0; y < PM; ++y) {
                         o[t][ct][0] = mma(even, p[t][e][y], o[t][ct][0]);
                         o[t][ct][1] = mma(odd, p[t][e][y], o[t][ct][1]);
                     }
             }
+        if (more) load_v();
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t) l[t] = lanes_sum(l[t]);
 
     // lane: row r16, channels 32 ct + 8 g + 2 i + (even, odd)
     if (BY_KEYS) {
-        constexpr int ROWS = 16 * NT;
+        const int ROWS = pl.join_rows;
         float *s_o = s_join, *s_m = s_join + WAVES * ROWS * D, *s_l = s_m + WAVES * ROWS;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            if (first + 16 * t + r16 >= n_rows) continue;
+            f32x4 sum[CT][2];
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    sum[ct][0][i] = columns_sum<CP>(o[t][ct][0][i]);
+                    sum[ct][1][i] = columns_sum<CP>(o[t][ct][1][i]);
+                }
+            if (first + 16 * t + r16 >= n_rows || r16 >= RT) continue;
             float *dst = s_o + (wave * ROWS + 16 * t + r16) * D + 8 * g;
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    dst[32 * ct + 2 * i] = o[t][ct][0][i];
-                    dst[32 * ct + 2 * i + 1] = o[t][ct][1][i];
+                    dst[32 * ct + 2 * i] = sum[ct][0][i];
+                    dst[32 * ct + 2 * i + 1] = sum[ct][1][i];
                 }
             if (g == 0) {
                 s_m[wave * ROWS + 16 * t + r16] = m[t];
@@ -406,24 +524,28 @@ __global__ __launch_bounds__(64 * WAVES) void k_attend(sili_kv4_attend_args a, A
             }
         }
         __syncthreads();
-        const int rows = min(ROWS, n_rows - first);
+        const int rows = min(RT * NT, n_rows - first);
         for (int at = threadIdx.x; at < rows * (D / 4); at += 64 * WAVES) {
             const int row = at / (D / 4), ch = 4 * (at - row * (D / 4));
-            float mm = -INFINITY, ll = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            for (int w = 0; w < WAVES; ++w) mm = fmaxf(mm, s_m[w * ROWS + row]);
+            float f[WAVES], mm = -INFINITY, ll = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
             for (int w = 0; w < WAVES; ++w) {
-                const float mw = s_m[w * ROWS + row];
-                const float f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - mm);
-                if (f == 0.0f && s_l[w * ROWS + row] == 0.0f) continue;
-                ll += f * s_l[w * ROWS + row];
-                const float4 x = *reinterpret_cast<const float4 *>(s_o + (w * ROWS + row) * D + ch);
-                acc[0] += f * x.x;
-                acc[1] += f * x.y;
-                acc[2] += f * x.z;
-                acc[3] += f * x.w;
+                f[w] = s_m[w * ROWS + row];
+                mm = fmaxf(mm, f[w]);
             }
-            const int64_t token = q0 + (first + row) / group;
-            const int64_t qh = h * group + (first + row) % group;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) {
+                // a wave without keys has m = -inf and zeros
+                f[w] = f[w] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(f[w] - mm);
+                ll += f[w] * s_l[w * ROWS + row];
+                const float4 x = *reinterpret_cast<const float4 *>(s_o + (w * ROWS + row) * D + ch);
+                acc[0] += f[w] * x.x;
+                acc[1] += f[w] * x.y;
+                acc[2] += f[w] * x.z;
+                acc[3] += f[w] * x.w;
+            }
+            const int32_t i = token_of(pl, first + row);
+            const int64_t token = q0 + i, qh = h * group + (first + row - i * group);
             if (token >= a.tokens) continue;
             if (pl.splits > 1) {
                 const int64_t slot = (token * a.q_heads + qh) * pl.splits + split;
@@ -431,9 +553,9 @@ __global__ __launch_bounds__(64 * WAVES) void k_attend(sili_kv4_attend_args a, A
                 if (ch == 0) pl.part_ml[slot] = make_float2(mm, ll);
             } else {
                 const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
-                T *out = (T *)a.out + token * a.out_token_stride + qh * a.out_head_stride + ch;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) out[j] = (T)(acc[j] * inv);
+                for (int j = 0; j < 4; ++j) acc[j] *= inv;
+                store4<T>((T *)a.out + token * a.out_token_stride + qh * a.out_head_stride + ch, acc, pl.out_packed);
                 if (a.lse && ch == 0)
                     a.lse[token * a.q_heads + qh] = ll != 0.0f ? (mm + __builtin_amdgcn_logf(ll)) * 0.69314718f : -INFINITY;
             }
@@ -442,7 +564,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_attend(sili_kv4_attend_args a, A
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const int32_t row = first + 16 * t + r16;
-            const int64_t token = q0 + row / group, qh = h * group + row % group;
+            const int32_t qi = token_of(pl, row);
+            const int64_t token = q0 + qi, qh = h * group + (row - qi * group);
             if (row >= n_rows || token >= a.tokens) continue;
             if (pl.splits > 1) {
                 const int64_t slot = (token * a.q_heads + qh) * pl.splits + split;
@@ -460,12 +583,15 @@ __global__ __launch_bounds__(64 * WAVES) void k_attend(sili_kv4_attend_args a, A
                 const float inv = l[t] != 0.0f ? 1.0f / l[t] : 0.0f;
                 T *out = (T *)a.out + token * a.out_token_stride + qh * a.out_head_stride + 8 * g;
 #pragma unroll
-                for (int ct = 0; ct < CT; ++ct)
+                for (int ct = 0; ct < CT; ++ct) {
+                    float x[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        out[32 * ct + 2 * i] = (T)(o[t][ct][0][i] * inv);
-                        out[32 * ct + 2 * i + 1] = (T)(o[t][ct][1][i] * inv);
+                        x[2 * (i & 1)] = o[t][ct][0][i] * inv;
+                        x[2 * (i & 1) + 1] = o[t][ct][1][i] * inv;
+                        if (i & 1) store4<T>(out + 32 * ct + 2 * (i - 1), x, pl.out_packed);
                     }
+                }
                 if (a.lse && g == 0)
                     a.lse[token * a.q_heads + qh] = l[t] != 0.0f ? (m[t] + __builtin_amdgcn_logf(l[t])) * 0.69314718f : -INFINITY;
             }
@@ -473,19 +599,22 @@ __global__ __launch_bounds__(64 * WAVES) void k_attend(sili_kv4_attend_args a, A
     }
 }
 
-// Joins the splits of a row: a block a (token, query head); D / 4 threads share
-// a split's channels, and the block's thread groups take every GROUPS-th split.
+// Joins the splits of a row: a block a (row, kv head, request); D / 4 threads
+// share a split's channels, and the block's thread groups take every GROUPS-th
+// split.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void k_attend_join(sili_kv4_attend_args a, AttendPlan pl) {
     constexpr int GROUPS = 256 / (D / 4);
     __shared__ float4 s_acc[256];
-    __shared__ float s_w[4], s_l[4];
-    const int64_t id = blockIdx.x, token = id / a.q_heads, qh = id - token * a.q_heads;
-    if (token < a.q_start[0] || token >= a.q_start[a.requests]) return;
-    const int64_t req = request_of(a.q_start, a.requests, token);
-    const int32_t q0 = a.q_start[req], n = min(a.q_start[req + 1] - q0, (int32_t)a.max_new);
-    const int64_t rows = n * (a.q_heads / a.cache.kv_heads);
-    if (token - q0 >= n || rows <= pl.few || rows > pl.many) return;
+    __shared__ float s_w[4], s_sum[GROUPS];
+    const int32_t row = blockIdx.x, h = blockIdx.y, req = blockIdx.z;
+    const int32_t group = pl.group;
+    const int32_t q0 = a.q_start[req], n_rows = min(a.q_start[req + 1] - q0, (int32_t)a.max_new) * group;
+    if (q0 < 0 || n_rows <= pl.few || n_rows > pl.many || row >= n_rows) return;
+    const int32_t i = token_of(pl, row);
+    const int64_t token = q0 + i, qh = h * group + (row - i * group);
+    if (token >= a.tokens) return;
+    const int64_t id = token * a.q_heads + qh;
     const float2 *ml = pl.part_ml + id * pl.splits;
     float m = -INFINITY;
     for (int s = threadIdx.x; s < pl.splits; s += 256) m = fmaxf(m, ml[s].x);
@@ -494,13 +623,15 @@ __global__ __launch_bounds__(256) void k_attend_join(sili_kv4_attend_args a, Att
     __syncthreads();
     m = fmaxf(fmaxf(s_w[0], s_w[1]), fmaxf(s_w[2], s_w[3]));
     const int part = threadIdx.x / (D / 4), ch = 4 * (threadIdx.x % (D / 4));
+    const float *src = pl.part_o + id * pl.splits * D + ch;
     float l = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
     for (int s = part; s < pl.splits; s += GROUPS) {
         const float2 x = ml[s];
-        if (x.y == 0.0f) continue;  // no key, and no sums written
-        const float f = __builtin_amdgcn_exp2f(x.x - m);
-        const float4 v = *reinterpret_cast<const float4 *>(pl.part_o + (id * pl.splits + s) * D + ch);
+        // a split without keys has written no sums
+        const float4 v = x.y != 0.0f ? *reinterpret_cast<const float4 *>(src + (int64_t)s * D) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const float f = x.y != 0.0f ? __builtin_amdgcn_exp2f(x.x - m) : 0.0f;
         l += f * x.y;
         acc.x += f * v.x;
         acc.y += f * v.y;
@@ -508,7 +639,6 @@ __global__ __launch_bounds__(256) void k_attend_join(sili_kv4_attend_args a, Att
         acc.w += f * v.w;
     }
     s_acc[threadIdx.x] = acc;
-    __shared__ float s_sum[GROUPS];
     if (ch == 0) s_sum[part] = l;
     __syncthreads();
     if (part != 0) return;
@@ -523,11 +653,8 @@ __global__ __launch_bounds__(256) void k_attend_join(sili_kv4_attend_args a, Att
         acc.w += v.w;
     }
     const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-    T *out = (T *)a.out + token * a.out_token_stride + qh * a.out_head_stride + ch;
-    out[0] = (T)(acc.x * inv);
-    out[1] = (T)(acc.y * inv);
-    out[2] = (T)(acc.z * inv);
-    out[3] = (T)(acc.w * inv);
+    const float x[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+    store4<T>((T *)a.out + token * a.out_token_stride + qh * a.out_head_stride + ch, x, pl.out_packed);
     if (a.lse && ch == 0) a.lse[id] = l != 0.0f ? (m + __builtin_amdgcn_logf(l)) * 0.69314718f : -INFINITY;
 }
 
@@ -584,7 +711,7 @@ namespace {
 // Requests of up to FEW_ROWS rows have their keys shared by a block's waves, a
 // row tile of 16 each; larger ones give each wave rows of its own.
 constexpr int32_t FEW_ROWS = 64;
-constexpr int NT_MANY = 2;
+constexpr int NT_MANY = 2, WAVES_MANY = 4;
 
 struct Launch {
     bool on = false;
@@ -592,14 +719,30 @@ struct Launch {
     AttendPlan plan{};
 };
 
-// The two launches of a call (few rows, many rows).  Keys are split until the
-// blocks fill the GPU, a split not below 256 keys.
+int waves_of(const sili_kv4_attend_args &a) {
+    const bool bf = a.dtype == SILI_BF16;
+    switch (a.cache.head_dim) {
+        case 64: return 4 * (bf ? waves_per_simd<__bf16, 64, true>() : waves_per_simd<float, 64, true>());
+        case 128: return 4 * (bf ? waves_per_simd<__bf16, 128, true>() : waves_per_simd<float, 128, true>());
+        default: return 4 * (bf ? waves_per_simd<__bf16, 256, true>() : waves_per_simd<float, 256, true>());
+    }
+}
+
+// The two launches of a call (few rows, many rows).
 void plan_attend(const sili_kv4_attend_args &a, Launch (&out)[2]) {
     const int64_t group = a.q_heads / a.cache.kv_heads, rows = a.max_new * group;
     const int64_t gpp = a.cache.page_size / 16;
     for (int k = 0; k < 2; ++k) {
         Launch &L = out[k];
         AttendPlan &p = L.plan;
+        p.kv_heads = (int32_t)a.cache.kv_heads;
+        p.group = (int32_t)group;
+        p.group_inv = group == 1 ? ~0u : (uint32_t)((uint64_t(1) << 32) / (uint64_t)group);
+        p.n_pages = (int32_t)a.cache.n_pages;
+        p.most = p.n_pages == 0 ? 0 : (int32_t)std::min(a.max_len, a.table_width * a.cache.page_size);
+        const int64_t es = dtype_size(a.dtype);
+        p.q_packed = aligned(a.q, (size_t)(8 * es)) && a.q_token_stride % 8 == 0 && a.q_head_stride % 8 == 0;
+        p.out_packed = aligned(a.out, (size_t)(4 * es)) && a.out_token_stride % 4 == 0 && a.out_head_stride % 4 == 0;
         p.groups_per_page = (int32_t)gpp;
         p.page_shift = (gpp & (gpp - 1)) == 0 ? (int32_t)__builtin_ctzll((unsigned long long)gpp) : -1;
         // a scale of zero leaves all scores equal; c > 0 keeps hidden ones at -inf
@@ -608,14 +751,24 @@ void plan_attend(const sili_kv4_attend_args &a, Launch (&out)[2]) {
         p.few = k == 0 ? 0 : FEW_ROWS;
         p.many = k == 0 ? FEW_ROWS : INT32_MAX;
         L.on = k == 0 || rows > FEW_ROWS;
-        const int64_t tile_rows = k == 0 ? 16 : 16 * NT_MANY * WAVES;
+        const int parts = a.dtype == SILI_F32 ? 4 : 2;
+        p.columns = k == 0 && rows <= 16 / parts ? parts : 1;
+        const int64_t tile_rows = k == 0 ? 16 / p.columns : 16 * NT_MANY * WAVES_MANY;
         L.tiles = (std::min<int64_t>(rows, p.many) + tile_rows - 1) / tile_rows;
+        p.join_rows = (int32_t)std::min<int64_t>(16, rows);
         // keys a row tile can reach: its rows' windows, aligned to 64
         int64_t reach = a.max_len;
         if (a.window > 0) reach = std::min(reach, a.window + (tile_rows - 1) / group + 1 + 63);
-        const int64_t step = k == 0 ? 64 * WAVES : 64;
         const int64_t blocks = std::max<int64_t>(1, a.requests * a.cache.kv_heads * L.tiles);
-        const int64_t want = std::clamp<int64_t>(2048 / blocks, 1, std::max<int64_t>(1, (reach + 255) / 256));
+        // few blocks: as many waves in one as a CU holds, so that fewer splits
+        // are left to join (40 heads of 131071 keys, 8 blocks a split: 31 + 5
+        // us against 31 + 7 with 4 waves; 320 blocks of 2048 keys: 24 us
+        // against 22.6, a second round of blocks)
+        const int wide = waves_of(a);
+        p.waves = blocks <= 128 ? wide : 4;
+        const int64_t step = k == 0 ? 64 * p.waves : 64;
+        const int64_t fill = k == 0 ? 256 * (wide / p.waves) : 2048;
+        const int64_t want = std::clamp<int64_t>(fill / blocks, 1, std::max<int64_t>(1, (reach + 255) / 256));
         p.chunk = (int32_t)std::max<int64_t>(step, ((reach + want - 1) / want + step - 1) / step * step);
         p.splits = (int32_t)std::max<int64_t>(1, (reach + p.chunk - 1) / p.chunk);
         if (!L.on) p.splits = 1;
@@ -643,12 +796,23 @@ void run_attend(const sili_kv4_attend_args &a, Launch (&L)[2], hipStream_t st) {
         require(x <= INT32_MAX && p.splits <= 65535, "kv4_attend: too many rows or keys");
         const dim3 grid((unsigned)x, (unsigned)p.splits, (unsigned)a.requests);
         if (k == 0) {
-            const uint32_t lds = WAVES * 16 * (D + 2) * sizeof(float);
-            launch(k_attend<T, D, 1, true>, grid, dim3(64 * WAVES), lds, st, a, p);
+            constexpr int WIDE = 4 * waves_per_simd<T, D, true>();
+            const uint32_t lds = p.waves * p.join_rows * (D + 2) * sizeof(float);
+            constexpr int PARTS = sizeof(T) == 4 ? 4 : 2;
+            const dim3 block(64 * p.waves);
+            if (p.columns > 1) {
+                if (p.waves == WIDE) launch(k_attend<T, D, 1, true, WIDE, PARTS>, grid, block, lds, st, a, p);
+                else launch(k_attend<T, D, 1, true, 4, PARTS>, grid, block, lds, st, a, p);
+            } else {
+                if (p.waves == WIDE) launch(k_attend<T, D, 1, true, WIDE>, grid, block, lds, st, a, p);
+                else launch(k_attend<T, D, 1, true, 4>, grid, block, lds, st, a, p);
+            }
         } else {
-            launch(k_attend<T, D, NT_MANY, false>, grid, dim3(64 * WAVES), 0, st, a, p);
+            launch(k_attend<T, D, NT_MANY, false, WAVES_MANY>, grid, dim3(64 * WAVES_MANY), 0, st, a, p);
         }
-        if (p.splits > 1) launch(k_attend_join<T, D>, dim3((unsigned)(a.tokens * a.q_heads)), dim3(256), 0, st, a, p);
+        const int64_t rows = std::min<int64_t>(a.max_new * (a.q_heads / a.cache.kv_heads), p.many);
+        if (p.splits > 1)
+            launch(k_attend_join<T, D>, dim3((unsigned)rows, (unsigned)a.cache.kv_heads, (unsigned)a.requests), dim3(256), 0, st, a, p);
     }
 }
 
