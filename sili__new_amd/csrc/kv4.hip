@@ -231,11 +231,12 @@ struct KeyRange {
     __device__ __forceinline__ int32_t begin(int32_t i) const { return window > 0 ? max(0, base + i + 1 - window) : 0; }
 };
 
-// Registers allow this many waves on a SIMD.
-template <typename T, int D, bool BY_KEYS>
+// Registers allow this many waves on a SIMD without spilling.
+template <typename T, int D, bool BY_KEYS, int CP>
 constexpr int waves_per_simd() {
     if (!BY_KEYS) return 1;
-    return (D == 64 ? 4 : D == 128 ? 3 : 2) - (__is_same(T, __bf16) ? 0 : 1);
+    constexpr bool lean = __is_same(T, __bf16) || (CP > 1 && D < 256);  // no more than two parts in registers
+    return (D == 64 ? 4 : D == 128 ? 3 : 2) - (lean ? 0 : 1);
 }
 
 // BY_KEYS: the block's waves share 16 NT rows and take every fourth step of
@@ -248,7 +249,7 @@ constexpr int waves_per_simd() {
 // within 16 lanes), so every one of them holds the row's weights and takes its
 // own part of them; the outputs are summed once, at the end.
 template <typename T, int D, int NT, bool BY_KEYS, int WAVES, int CP = 1>
-__global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, BY_KEYS>())) void k_attend(sili_kv4_attend_args a, AttendPlan pl) {
+__global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, BY_KEYS, CP>())) void k_attend(sili_kv4_attend_args a, AttendPlan pl) {
     constexpr int QP = q_parts<T>(), PP = p_parts<T, BY_KEYS>();
     constexpr int KS = D / 32;   // steps of 32 channels
     constexpr int CT = D / 32;   // blocks of 32 output channels
@@ -719,13 +720,19 @@ struct Launch {
     AttendPlan plan{};
 };
 
-int waves_of(const sili_kv4_attend_args &a) {
-    const bool bf = a.dtype == SILI_BF16;
-    switch (a.cache.head_dim) {
-        case 64: return 4 * (bf ? waves_per_simd<__bf16, 64, true>() : waves_per_simd<float, 64, true>());
-        case 128: return 4 * (bf ? waves_per_simd<__bf16, 128, true>() : waves_per_simd<float, 128, true>());
-        default: return 4 * (bf ? waves_per_simd<__bf16, 256, true>() : waves_per_simd<float, 256, true>());
-    }
+// Waves of a CU that run the few-rows kernel at once.
+int waves_of(int dtype, int64_t head_dim, int columns) {
+    int n = 0;
+    with_dtype(dtype, [&](auto z) {
+        using T = decltype(z);
+        auto of = [&](auto d) {
+            constexpr int D = decltype(d)::value;
+            return 4 * (columns > 1 ? waves_per_simd<T, D, true, 2>() : waves_per_simd<T, D, true, 1>());
+        };
+        n = head_dim == 64 ? of(std::integral_constant<int, 64>{}) : head_dim == 128 ? of(std::integral_constant<int, 128>{})
+                                                                                     : of(std::integral_constant<int, 256>{});
+    });
+    return n;
 }
 
 // The two launches of a call (few rows, many rows).
@@ -764,10 +771,13 @@ void plan_attend(const sili_kv4_attend_args &a, Launch (&out)[2]) {
         // are left to join (40 heads of 131071 keys, 8 blocks a split: 31 + 5
         // us against 31 + 7 with 4 waves; 320 blocks of 2048 keys: 24 us
         // against 22.6, a second round of blocks)
-        const int wide = waves_of(a);
+        const int wide = waves_of(a.dtype, a.cache.head_dim, p.columns);
         p.waves = blocks <= 128 ? wide : 4;
         const int64_t step = k == 0 ? 64 * p.waves : 64;
-        const int64_t fill = k == 0 ? 256 * (wide / p.waves) : 2048;
+        // splits until every CU has a wave on each SIMD as often as registers
+        // allow; fp32, which the vector units bound, twice at most (320 blocks
+        // of 2048 keys: 22.7 us, with a second split 21.4 + 4.7 to join)
+        const int64_t fill = k == 0 ? 256 * std::max(1, std::min(wide, a.dtype == SILI_F32 ? 8 : wide) / p.waves) : 2048;
         const int64_t want = std::clamp<int64_t>(fill / blocks, 1, std::max<int64_t>(1, (reach + 255) / 256));
         p.chunk = (int32_t)std::max<int64_t>(step, ((reach + want - 1) / want + step - 1) / step * step);
         p.splits = (int32_t)std::max<int64_t>(1, (reach + p.chunk - 1) / p.chunk);
@@ -796,12 +806,12 @@ void run_attend(const sili_kv4_attend_args &a, Launch (&L)[2], hipStream_t st) {
         require(x <= INT32_MAX && p.splits <= 65535, "kv4_attend: too many rows or keys");
         const dim3 grid((unsigned)x, (unsigned)p.splits, (unsigned)a.requests);
         if (k == 0) {
-            constexpr int WIDE = 4 * waves_per_simd<T, D, true>();
-            const uint32_t lds = p.waves * p.join_rows * (D + 2) * sizeof(float);
             constexpr int PARTS = sizeof(T) == 4 ? 4 : 2;
+            constexpr int WIDE = 4 * waves_per_simd<T, D, true, 1>(), WIDE_P = 4 * waves_per_simd<T, D, true, PARTS>();
+            const uint32_t lds = p.waves * p.join_rows * (D + 2) * sizeof(float);
             const dim3 block(64 * p.waves);
             if (p.columns > 1) {
-                if (p.waves == WIDE) launch(k_attend<T, D, 1, true, WIDE, PARTS>, grid, block, lds, st, a, p);
+                if (p.waves == WIDE_P) launch(k_attend<T, D, 1, true, WIDE_P, PARTS>, grid, block, lds, st, a, p);
                 else launch(k_attend<T, D, 1, true, 4, PARTS>, grid, block, lds, st, a, p);
             } else {
                 if (p.waves == WIDE) launch(k_attend<T, D, 1, true, WIDE>, grid, block, lds, st, a, p);
