@@ -18,66 +18,105 @@ __device__ __forceinline__ float wave_max(float v) {
     for (int d = 32; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, 64));
     return v;
 }
-__device__ __forceinline__ float wave_sum(float v) {
-    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
+
+// ---- rows ------------------------------------------------------------------------
+// Bound by memory: 4.25 bits stored a channel beside the row's own. A thread takes
+// 8 channels of a (token, kv head), k's and v's: 16 or 32 bytes a load, a dword of
+// k codes, four bytes of v codes.  The bytes of 16 tokens share their 16-byte runs
+// of v codes, so a block takes one head of as many tokens as its threads cover:
+// their bytes meet in one L2 (a block of one token's heads, whose neighbours run on
+// other XCDs, wrote 2048 tokens of 40 heads in 42 us).
+constexpr int ROWS_TPB = 256;
+
+// Maximum over the aligned group of N lanes.
+template <int N>
+__device__ __forceinline__ float group_max(float v) {
+#pragma unroll
+    for (int d = 1; d < N; d <<= 1) v = fmaxf(v, __shfl_xor(v, d, 64));
     return v;
 }
 
-// Byte b of a stored head (channels 2b, 2b + 1) in the k and v code arrays;
-// head: index of (page, kv head).
-__device__ __forceinline__ int64_t k_byte(const sili_kv4_cache &c, int64_t head, int slot, int b) {
-    return (head * c.page_size + slot) * (c.head_dim / 2) + b;
-}
-__device__ __forceinline__ int64_t v_byte(const sili_kv4_cache &c, int64_t head, int slot, int b) {
-    return ((head * (c.page_size / 16) + slot / 16) * (c.head_dim / 2) + b) * 16 + slot % 16;
+template <typename T>
+__device__ __forceinline__ void load8(const T *p, bool packed, float (&x)[8]) {
+    if (packed) {
+        load_pack<T, 8>(p, x);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = (float)p[j];
+    }
 }
 
-constexpr int ROWS_TPB = 256;
+// Codes of eight channels (channel j in nibble j), and the head's scale.
+template <int N>
+__device__ __forceinline__ uint32_t encode8(const float (&x)[8], float &scale) {
+    float top = 0.0f, sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        top = fmaxf(top, fabsf(x[j]));
+        sum += x[j] * 0.0f;  // 0, or NaN for what is not finite
+    }
+    const float bad = sum != 0.0f || sum != sum ? INFINITY : 0.0f;
+    top = group_max<N>(fmaxf(top, bad));
+    const bool finite = top < INFINITY, zero = !finite || top < 0x1p-120f;
+    const float inv = zero ? 0.0f : 6.0f / top;
+    uint32_t w = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w |= fp4_encode(x[j] * inv) << (4 * j);
+    scale = !finite ? __builtin_nanf("") : zero ? 0.0f : top / 6.0f;
+    return zero ? 0u : w;
+}
 
-// One wave a (token, kv head): k's head, then v's.
-template <typename T, bool WRITE>
-__global__ __launch_bounds__(ROWS_TPB) void k_kv4_rows(sili_kv4_rows_args a) {
-    const int64_t id = (int64_t)blockIdx.x * (ROWS_TPB / 64) + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
+template <typename T, int D, bool WRITE>
+__global__ __launch_bounds__(ROWS_TPB) void k_kv4_rows(sili_kv4_rows_args a, bool packed) {
+    constexpr int N = D / 8;  // threads of a head
     const sili_kv4_cache &c = a.cache;
-    if (id >= a.tokens * c.kv_heads) return;
-    const int64_t t = id / c.kv_heads, h = id - t * c.kv_heads;
-    const int64_t slot = a.slots[t];
-    const bool held = slot >= 0 && slot < c.n_pages * c.page_size;
+    const uint32_t H = (uint32_t)c.kv_heads, h = blockIdx.x % H;
+    const uint32_t t = blockIdx.x / H * (ROWS_TPB / N) + threadIdx.x / N, sub = threadIdx.x % N;
+    if (t >= (uint32_t)a.tokens) return;
+    const int32_t slot = a.slots[t];
+    const uint32_t ps = (uint32_t)c.page_size;
+    const bool held = slot >= 0 && (int64_t)slot < c.n_pages * c.page_size;
     if (WRITE && !held) return;
-    const int64_t page = held ? slot / c.page_size : 0;
-    const int at = held ? (int)(slot - page * c.page_size) : 0;
-    const int64_t head = page * c.kv_heads + h;
-    const int pairs = (int)c.head_dim / 2;
-    for (int which = 0; which < 2; ++which) {
-        T *row = which ? (T *)a.v + t * a.v_token_stride + h * a.v_head_stride
-                       : (T *)a.k + t * a.k_token_stride + h * a.k_head_stride;
-        uint8_t *codes = which ? c.v : c.k;
-        float *scales = (which ? c.v_scale : c.k_scale) + head * c.page_size + at;
-        if (WRITE) {
-            float top = 0.0f;
-            bool bad = false;
-            for (int b = lane; b < pairs; b += 64) {
-                const float x = fabsf((float)row[2 * b]), y = fabsf((float)row[2 * b + 1]);
-                bad |= !(x < INFINITY) || !(y < INFINITY);
-                top = fmaxf(top, fmaxf(x, y));
-            }
-            top = wave_max(top);
-            bad = __any(bad);
-            const bool zero = top < 0x1p-120f || bad;
-            const float inv = zero ? 0.0f : 6.0f / top;
-            for (int b = lane; b < pairs; b += 64) {
-                const uint32_t lo = zero ? 0u : fp4_encode((float)row[2 * b] * inv);
-                const uint32_t hi = zero ? 0u : fp4_encode((float)row[2 * b + 1] * inv);
-                codes[which ? v_byte(c, head, at, b) : k_byte(c, head, at, b)] = (uint8_t)(lo | hi << 4);
-            }
-            if (lane == 0) *scales = bad ? __builtin_nanf("") : zero ? 0.0f : top / 6.0f;
-        } else {
-            const float scale = held ? *scales : 0.0f;
-            for (int b = lane; b < pairs; b += 64) {
-                const uint32_t byte = held ? codes[which ? v_byte(c, head, at, b) : k_byte(c, head, at, b)] : 0u;
-                row[2 * b] = (T)(fp4_decode(byte & 15u) * scale);
-                row[2 * b + 1] = (T)(fp4_decode(byte >> 4) * scale);
+    const uint32_t page = held ? (uint32_t)slot / ps : 0u, at = held ? (uint32_t)slot - page * ps : 0u;
+    const int64_t first = ((int64_t)page * H + h) * ps;  // this head's first slot in the page
+    T *k = (T *)a.k + t * a.k_token_stride + h * a.k_head_stride + 8 * sub;
+    T *v = (T *)a.v + t * a.v_token_stride + h * a.v_head_stride + 8 * sub;
+    uint32_t *kc = reinterpret_cast<uint32_t *>(c.k + (first + at) * (D / 2)) + sub;
+    uint8_t *vc = c.v + (first + (at & ~15u)) * (D / 2) + 64 * sub + (at & 15u);  // channel pair 4 sub, key at % 16
+    float *ks = c.k_scale + first + at, *vs = c.v_scale + first + at;
+    if (WRITE) {
+        float x[8], y[8], sk, sv;
+        load8<T>(k, packed, x);
+        load8<T>(v, packed, y);
+        *kc = encode8<N>(x, sk);
+        const uint32_t w = encode8<N>(y, sv);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) vc[16 * j] = (uint8_t)(w >> (8 * j));
+        if (sub == 0) {
+            *ks = sk;
+            *vs = sv;
+        }
+    } else {
+        uint32_t w[2] = {0, 0};
+        float s[2] = {0.0f, 0.0f};
+        if (held) {
+            w[0] = *kc;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[1] |= (uint32_t)vc[16 * j] << (8 * j);
+            s[0] = *ks;
+            s[1] = *vs;
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            T *out = r ? v : k;
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = fp4_decode((w[r] >> (4 * j)) & 15u) * s[r];
+            if (packed) {
+                store_pack<T, 8>(out, x);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) out[j] = (T)x[j];
             }
         }
     }
@@ -679,10 +718,21 @@ void rows(const sili_kv4_rows_args &a, hipStream_t st, const char *what) {
     require(a.tokens >= 0 && a.tokens < (int64_t(1) << 31), "kv4 rows: tokens out of range");
     if (a.tokens == 0) return;
     require(a.slots && a.k && a.v, "kv4 rows: NULL buffer");
-    const int64_t blocks = (a.tokens * a.cache.kv_heads + ROWS_TPB / 64 - 1) / (ROWS_TPB / 64);
+    const int64_t tokens = ROWS_TPB / (a.cache.head_dim / 8);  // of a block
+    const int64_t blocks = (a.tokens + tokens - 1) / tokens * a.cache.kv_heads;
     require(blocks <= INT32_MAX, "kv4 rows: too many rows");
+    auto packs = [&](const void *p, int64_t ts, int64_t hs) {
+        return aligned(p, (size_t)(8 * dtype_size(a.dtype))) && ts % 8 == 0 && hs % 8 == 0;
+    };
+    const bool packed = packs(a.k, a.k_token_stride, a.k_head_stride) && packs(a.v, a.v_token_stride, a.v_head_stride);
+    const dim3 grid((unsigned)blocks);
     with_dtype(a.dtype, [&](auto z) {
-        launch(k_kv4_rows<decltype(z), WRITE>, dim3((unsigned)blocks), dim3(ROWS_TPB), 0, st, a);
+        using T = decltype(z);
+        switch (a.cache.head_dim) {
+            case 64: launch(k_kv4_rows<T, 64, WRITE>, grid, dim3(ROWS_TPB), 0, st, a, packed); break;
+            case 128: launch(k_kv4_rows<T, 128, WRITE>, grid, dim3(ROWS_TPB), 0, st, a, packed); break;
+            default: launch(k_kv4_rows<T, 256, WRITE>, grid, dim3(ROWS_TPB), 0, st, a, packed); break;
+        }
     });
     SILI_HIP(hipGetLastError());
 }

@@ -16,83 +16,115 @@ namespace {
 
 constexpr unsigned TPB = 256;
 
-// V pairs (or, past the rotated channels, V copied channels) of one head.
+// Heads in flight: a thread asks for this many before it stores the first.
+constexpr int HB = 4;
+
+// A run of elements as one register value (a struct of them ends up in memory).
+template <int BYTES> struct RawOf;
+template <> struct RawOf<2> { typedef uint16_t type; };
+template <> struct RawOf<4> { typedef uint32_t type; };
+template <> struct RawOf<8> { typedef uint2 type; };
+template <> struct RawOf<16> { typedef uint4 type; };
+template <typename T, int N>
+using Raw = typename RawOf<N * (int)sizeof(T)>::type;
+
+template <typename T, int N>
+__device__ __forceinline__ Raw<T, N> get(const T *p) { return *reinterpret_cast<const Raw<T, N> *>(p); }
+template <typename T, int N>
+__device__ __forceinline__ void put(T *p, const Raw<T, N> &r) { *reinterpret_cast<Raw<T, N> *>(p) = r; }
+
+// V pairs of one head turned: x1 and x2 in a run each (half), or in turn in one
+// run of 2 V (interleaved; x2 unused).
 template <typename T, int V, bool HALF>
-__device__ __forceinline__ void turn(const T *x, T *y, int rot, int i, const float (&c)[V], const float (&s)[V]) {
-    if (HALF) {
-        float a[V], b[V], u[V], w[V];
-        load_pack<T, V>(x + i, a);
-        load_pack<T, V>(x + rot / 2 + i, b);
+__device__ __forceinline__ void turn(T *y, int rot, int i, Raw<T, HALF ? V : 2 * V> r1, Raw<T, HALF ? V : 2 * V> r2, const float (&c)[V],
+                                     const float (&s)[V]) {
+    constexpr int R = HALF ? V : 2 * V;
+    using RawR = Raw<T, R>;
+    const Pack<T, R> p = __builtin_bit_cast(Pack<T, R>, r1), q = __builtin_bit_cast(Pack<T, R>, r2);
+    Pack<T, R> u, w;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            u[j] = a[j] * c[j] - b[j] * s[j];
-            w[j] = b[j] * c[j] + a[j] * s[j];
+    for (int j = 0; j < V; ++j) {
+        const float x1 = (float)(HALF ? p.v[j] : p.v[2 * j % R]), x2 = (float)(HALF ? q.v[j] : p.v[(2 * j + 1) % R]);
+        // which product is fused is fixed, so that every variant gives the same bits
+        const T y1 = (T)__builtin_fmaf(x1, c[j], -(x2 * s[j])), y2 = (T)__builtin_fmaf(x2, c[j], x1 * s[j]);
+        if (HALF) {
+            u.v[j] = y1;
+            w.v[j] = y2;
+        } else {
+            u.v[2 * j % R] = y1;
+            u.v[(2 * j + 1) % R] = y2;
         }
-        store_pack<T, V>(y + i, u);
-        store_pack<T, V>(y + rot / 2 + i, w);
-    } else {
-        float a[2 * V], u[2 * V];
-        load_pack<T, 2 * V>(x + 2 * i, a);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            u[2 * j] = a[2 * j] * c[j] - a[2 * j + 1] * s[j];
-            u[2 * j + 1] = a[2 * j + 1] * c[j] + a[2 * j] * s[j];
-        }
-        store_pack<T, 2 * V>(y + 2 * i, u);
     }
+    put<T, R>(y + (HALF ? i : 2 * i), __builtin_bit_cast(RawR, u));
+    if (HALF) put<T, R>(y + rot / 2 + i, __builtin_bit_cast(RawR, w));
 }
 
-// Thread: (token, unit); units [0, rot / 2 / V) turn V pairs, the rest copy V
+// Thread: (token, unit); units [0, rot / 2 / V) turn V pairs, the rest copy W
 // channels.  blockIdx.y cuts the heads (q's, then k's) into shares.
-template <typename T, int V, bool HALF>
-__global__ __launch_bounds__(TPB) void k_rotary(sili_rotary_args a, int units, int share) {
-    const int64_t id = (int64_t)blockIdx.x * TPB + threadIdx.x;
-    const int64_t t = id / units;
-    const int unit = (int)(id - t * units);
-    if (t >= a.tokens) return;
+template <typename T, int V, int W, bool HALF>
+__global__ __launch_bounds__(TPB) void k_rotary(sili_rotary_args a, uint32_t units, int share) {
+    const uint32_t id = blockIdx.x * TPB + threadIdx.x, t = id / units, unit = id - t * units;
+    if (t >= (uint64_t)a.tokens) return;
     const int rot = (int)a.rot_dim, turning = rot / 2 / V;
-    float c[V], s[V];
-    const int i = unit * V;
-    if (unit < turning) {
-        const int64_t p = a.positions[t];
+    const bool turns = (int)unit < turning;
+    const int i = turns ? (int)unit * V : rot + ((int)unit - turning) * W;
+    const int nq = (int)a.q_heads, heads = nq + (int)a.k_heads;
+    auto in = [&](int h) {
+        return h < nq ? (const T *)a.q + t * a.q_token_stride + h * a.q_head_stride
+                      : (const T *)a.k + t * a.k_token_stride + (h - nq) * a.k_head_stride;
+    };
+    auto out = [&](int h) {
+        return h < nq ? (T *)a.q_out + t * a.q_out_token_stride + h * a.q_out_head_stride
+                      : (T *)a.k_out + t * a.k_out_token_stride + (h - nq) * a.k_out_head_stride;
+    };
+    const int h1 = min((int)(blockIdx.y + 1) * share, heads);
+    if (!turns) {
+        for (int h = blockIdx.y * share; h < h1; h += HB) {
+            Raw<T, W> p[HB];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const uint64_t phase = (uint64_t)p * a.phase_steps[i + j];
-            const float half_turns = (float)(int32_t)(phase >> 32) * 0x1p-31f;
-            sincospif(half_turns, &s[j], &c[j]);
-            c[j] *= a.scale;
-            s[j] *= a.inverse ? -a.scale : a.scale;
+            for (int k = 0; k < HB; ++k) p[k] = get<T, W>(in(min(h + k, h1 - 1)) + i);
+#pragma unroll
+            for (int k = 0; k < HB; ++k)
+                if (h + k < h1) put<T, W>(out(h + k) + i, p[k]);
         }
+        return;
     }
-    const int heads = (int)(a.q_heads + a.k_heads);
-    const int h0 = blockIdx.y * share, h1 = min(h0 + share, heads);
-    for (int h = h0; h < h1; ++h) {
-        const bool isq = h < a.q_heads;
-        const int64_t g = isq ? h : h - a.q_heads;
-        const T *x = isq ? (const T *)a.q + t * a.q_token_stride + g * a.q_head_stride
-                         : (const T *)a.k + t * a.k_token_stride + g * a.k_head_stride;
-        T *y = isq ? (T *)a.q_out + t * a.q_out_token_stride + g * a.q_out_head_stride
-                   : (T *)a.k_out + t * a.k_out_token_stride + g * a.k_out_head_stride;
-        if (unit < turning) turn<T, V, HALF>(x, y, rot, i, c, s);
-        else {
-            const int at = rot + (unit - turning) * V;
-            *reinterpret_cast<Pack<T, V> *>(y + at) = *reinterpret_cast<const Pack<T, V> *>(x + at);
+    float c[V], s[V];
+    const int64_t pos = a.positions[t];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const uint64_t phase = (uint64_t)pos * a.phase_steps[i + j];
+        sincospif((float)(int32_t)(phase >> 32) * 0x1p-31f, &s[j], &c[j]);
+        c[j] *= a.scale;
+        s[j] *= a.inverse ? -a.scale : a.scale;
+    }
+    for (int h = blockIdx.y * share; h < h1; h += HB) {
+        constexpr int R = HALF ? V : 2 * V;
+        Raw<T, R> x1[HB], x2[HB];
+#pragma unroll
+        for (int k = 0; k < HB; ++k) {
+            const T *x = in(min(h + k, h1 - 1));
+            x1[k] = get<T, R>(x + (HALF ? i : 2 * i));
+            x2[k] = HALF ? get<T, R>(x + rot / 2 + i) : x1[k];
         }
+#pragma unroll
+        for (int k = 0; k < HB; ++k)
+            if (h + k < h1) turn<T, V, HALF>(out(h + k), rot, i, x1[k], x2[k], c, s);
     }
 }
 
-template <typename T, int V>
+template <typename T, int V, int W, bool HALF>
 void run(const sili_rotary_args &a, hipStream_t st) {
-    const int64_t units = a.rot_dim / 2 / V + (a.head_dim - a.rot_dim) / V;
+    const int64_t units = a.rot_dim / 2 / V + (a.head_dim - a.rot_dim) / W;
     const int64_t blocks = (a.tokens * units + TPB - 1) / TPB, heads = a.q_heads + a.k_heads;
-    require(blocks <= INT32_MAX, "rotary: too many tokens");
-    // heads a thread walks: as few as fill the GPU (2048 blocks), since the
-    // sines are worth about one head's traffic
+    require(a.tokens * units < (int64_t(1) << 32) - TPB, "rotary: too many tokens");
+    // heads a thread walks: as few as fill the GPU (2048 blocks), but the HB that
+    // it has in flight, since the sines are worth about one head's traffic
     const int64_t shares = std::clamp<int64_t>(2048 / std::max<int64_t>(blocks, 1), 1, heads);
-    const int share = (int)((heads + shares - 1) / shares);
-    const dim3 grid((unsigned)blocks, (unsigned)((heads + share - 1) / share));
-    if (a.layout == SILI_ROTARY_HALF) launch(k_rotary<T, V, true>, grid, dim3(TPB), 0, st, a, (int)units, share);
-    else launch(k_rotary<T, V, false>, grid, dim3(TPB), 0, st, a, (int)units, share);
+    int64_t share = (heads + shares - 1) / shares;
+    if (share > 1) share = (share + HB - 1) / HB * HB;
+    launch(k_rotary<T, V, W, HALF>, dim3((unsigned)blocks, (unsigned)((heads + share - 1) / share)), dim3(TPB), 0, st, a,
+           (uint32_t)units, (int)share);
 }
 
 }  // namespace
@@ -108,23 +140,21 @@ void rotary(const sili_rotary_args &a, hipStream_t st) {
     require((a.positions && a.phase_steps) || a.rot_dim == 0, "rotary: NULL positions or phase_steps");
     require(a.q_heads == 0 || (a.q && a.q_out), "rotary: NULL q");
     require(a.k_heads == 0 || (a.k && a.k_out), "rotary: NULL k");
-    // vectors need every address and size to divide: 16 bytes of an
-    // interleaved head hold half as many pairs as a run of a half layout
-    const int64_t es = dtype_size(a.dtype);
-    auto fits = [&](int64_t v) {
-        const int64_t run = a.layout == SILI_ROTARY_HALF ? v : 2 * v;
-        auto ok = [&](int64_t heads, const void *x, int64_t ts, int64_t hs) {
-            return heads == 0 || (aligned(x, (size_t)(run * es)) && ts % run == 0 && hs % run == 0);
-        };
-        return a.rot_dim / 2 % v == 0 && a.rot_dim % run == 0 && (a.head_dim - a.rot_dim) % v == 0 &&
-               ok(a.q_heads, a.q, a.q_token_stride, a.q_head_stride) && ok(a.k_heads, a.k, a.k_token_stride, a.k_head_stride) &&
-               ok(a.q_heads, a.q_out, a.q_out_token_stride, a.q_out_head_stride) &&
-               ok(a.k_heads, a.k_out, a.k_out_token_stride, a.k_out_head_stride);
+    // 16-byte runs need every address, stride and size to divide them
+    const int64_t es = dtype_size(a.dtype), run_len = 16 / es;
+    const bool half = a.layout == SILI_ROTARY_HALF;
+    auto ok = [&](int64_t heads, const void *x, int64_t ts, int64_t hs) {
+        return heads == 0 || (aligned(x, 16) && ts % run_len == 0 && hs % run_len == 0);
     };
+    const bool fits = (half ? a.rot_dim / 2 : a.rot_dim) % run_len == 0 && (a.head_dim - a.rot_dim) % run_len == 0 &&
+                      ok(a.q_heads, a.q, a.q_token_stride, a.q_head_stride) && ok(a.k_heads, a.k, a.k_token_stride, a.k_head_stride) &&
+                      ok(a.q_heads, a.q_out, a.q_out_token_stride, a.q_out_head_stride) &&
+                      ok(a.k_heads, a.k_out, a.k_out_token_stride, a.k_out_head_stride);
     with_dtype(a.dtype, [&](auto z) {
         using T = decltype(z);
-        if (fits(4)) run<T, 4>(a, st);
-        else run<T, 1>(a, st);
+        constexpr int N = 16 / (int)sizeof(T);
+        if (half) fits ? run<T, N, N, true>(a, st) : run<T, 1, 1, true>(a, st);
+        else fits ? run<T, N / 2, N, false>(a, st) : run<T, 1, 1, false>(a, st);
     });
     SILI_HIP(hipGetLastError());
 }
