@@ -18,15 +18,23 @@ constexpr int FEW = 4096;       // requests whose sums a block holds in LDS
 constexpr unsigned FEW_TPB = 512;
 constexpr unsigned MANY_TPB = 1024;
 
+// The call's arguments and the division by page_size.
+struct Step {
+    sili_request_slots_args a;
+    int32_t shift;  // page_size = 2^shift, or -1
+};
+__device__ __forceinline__ uint32_t page_of(const Step &s, uint32_t pos) {
+    return s.shift >= 0 ? pos >> s.shift : pos / (uint32_t)s.a.page_size;
+}
+
 struct Req {
     int32_t cached, fresh;  // tokens held, tokens new
     int32_t have, take;     // pages held, pages taken
     uint32_t flags;
 };
 
-__device__ __forceinline__ Req request(const sili_request_slots_args &a, int64_t r) {
+__device__ __forceinline__ Req request(const Step &s, int32_t c, int32_t n) {
     Req q;
-    const int32_t c = a.cached_lens[r], n = a.new_lens[r];
     q.flags = (c < 0 || n < 0) ? SILI_SLOTS_BAD_LENGTH : 0u;
     q.cached = max(c, 0);
     q.fresh = max(n, 0);
@@ -34,11 +42,11 @@ __device__ __forceinline__ Req request(const sili_request_slots_args &a, int64_t
         q.fresh = INT32_MAX - q.cached;
         q.flags |= SILI_SLOTS_BAD_LENGTH;
     }
-    const uint32_t p = (uint32_t)a.page_size;
-    q.have = (int32_t)(((uint32_t)q.cached + p - 1u) / p);
-    const int32_t all = (int32_t)(((uint32_t)q.cached + (uint32_t)q.fresh + p - 1u) / p);
+    const uint32_t p = (uint32_t)s.a.page_size - 1u;
+    q.have = (int32_t)page_of(s, (uint32_t)q.cached + p);
+    const int32_t all = (int32_t)page_of(s, (uint32_t)q.cached + (uint32_t)q.fresh + p);
     q.take = all - q.have;
-    if (q.fresh > 0 && all > a.table_width) q.flags |= SILI_SLOTS_TABLE_FULL;
+    if (q.fresh > 0 && all > s.a.table_width) q.flags |= SILI_SLOTS_TABLE_FULL;
     return q;
 }
 
@@ -50,12 +58,21 @@ __device__ __forceinline__ int32_t slot_of(const sili_request_slots_args &a, int
     return good_page(a, page) ? page * (int32_t)a.page_size + (int32_t)offset : -1;
 }
 
-// The page that request r's first new token shares with its cached ones, when
-// it is no page.
-__device__ __forceinline__ uint32_t held_flags(const sili_request_slots_args &a, const Req &q, int64_t r) {
-    const uint32_t p = (uint32_t)a.page_size, at = (uint32_t)q.cached / p;
-    if (q.fresh == 0 || (uint32_t)q.cached % p == 0u || at >= a.table_width) return 0u;
-    return good_page(a, a.block_table[r * a.table_width + at]) ? 0u : (uint32_t)SILI_SLOTS_BAD_PAGE;
+// The page that request r's first new token shares with its cached ones: whether
+// there is one, and the table's entry (any other where there is none).
+__device__ __forceinline__ bool shares_page(const Step &s, const Req &q) {
+    const uint32_t at = page_of(s, (uint32_t)q.cached);
+    return q.fresh > 0 && (int32_t)at < q.have && at < s.a.table_width;
+}
+__device__ __forceinline__ int32_t shared_page(const Step &s, const Req &q, int64_t r) {
+    return s.a.block_table[r * s.a.table_width + min((int64_t)page_of(s, (uint32_t)q.cached), s.a.table_width - 1)];
+}
+
+// Inclusive sum over the wave of values up to 2^34: 16 low bits and the rest
+// scanned by themselves, in 32 bits.
+__device__ __forceinline__ int64_t wave_scan64(int64_t x) {
+    const uint32_t lo = wave_incl_scan((uint32_t)x & 0xFFFFu), hi = wave_incl_scan((uint32_t)(x >> 16));
+    return ((int64_t)hi << 16) + lo;
 }
 
 // Exclusive sums of (x, y) over the block; the block's totals in tx, ty.
@@ -63,13 +80,8 @@ template <unsigned TPB>
 __device__ __forceinline__ void block_scan(int64_t &x, int64_t &y, int64_t &tx, int64_t &ty, int64_t (&part)[2][TPB / 64]) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const int64_t x0 = x, y0 = y;
-    for (int d = 1; d < 64; d <<= 1) {
-        const int64_t ux = __shfl_up(x, d, 64), uy = __shfl_up(y, d, 64);
-        if ((int)lane >= d) {
-            x += ux;
-            y += uy;
-        }
-    }
+    x = wave_scan64(x);
+    y = wave_scan64(y);
     if (lane == 63u) {
         part[0][wave] = x;
         part[1][wave] = y;
@@ -77,6 +89,7 @@ __device__ __forceinline__ void block_scan(int64_t &x, int64_t &y, int64_t &tx, 
     __syncthreads();
     tx = ty = 0;
     int64_t bx = 0, by = 0;
+#pragma unroll
     for (uint32_t w = 0; w < TPB / 64; ++w) {
         if (w == wave) {
             bx = tx;
@@ -104,85 +117,113 @@ __device__ __forceinline__ int64_t owner(const int32_t *start, I n, int64_t t) {
 
 // Up to FEW requests: every block sums all the lengths itself (they are a few
 // KB, from L2), so that one launch does the whole step; then the blocks share
-// the requests, the pages and the tokens.
-__global__ __launch_bounds__(FEW_TPB) void k_slots_few(sili_request_slots_args a) {
-    extern __shared__ int32_t s_start[];  // tokens [R], pages [R]
+// the requests, the pages and the tokens, all but the last, which checks (alone it
+// does both; a sharing block that checks too took 15.5 us at 4096 requests).  Latency bounds it: the lengths, the
+// sums, a search in LDS and a page are one chain.
+template <int PER>
+__global__ __launch_bounds__(FEW_TPB) void k_slots_few(Step s) {
+    extern __shared__ int32_t s_req[];  // first token, first page taken, cached [R each]
     __shared__ int64_t s_part[2][FEW_TPB / 64];
     __shared__ uint32_t s_flags;
+    const sili_request_slots_args &a = s.a;
     const int R = (int)a.requests;
-    int32_t *tok = s_start, *pag = s_start + R;
-    const int per = (R + (int)FEW_TPB - 1) / (int)FEW_TPB;
-    const int r0 = min((int)threadIdx.x * per, R), r1 = min(r0 + per, R);
+    int32_t *tok = s_req, *pag = s_req + R, *old = s_req + 2 * R;
+    const int r0 = (int)threadIdx.x * PER;
+    const bool checks = blockIdx.x + 1 == gridDim.x;
+    const uint32_t sharing = gridDim.x == 1 ? 1u : gridDim.x - 1u;
+    const int mine0 = (int)((uint32_t)R * blockIdx.x / sharing), mine1 = (int)((uint32_t)R * (blockIdx.x + 1) / sharing);
     if (threadIdx.x == 0) s_flags = 0;
     int64_t nt = 0, np = 0, T, P;
     uint32_t flags = 0;
-    for (int r = r0; r < r1; ++r) {
-        const Req q = request(a, r);
-        nt += q.fresh;
-        np += q.take;
+    int32_t c[PER], n[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const bool in = r0 + k < R;
+        c[k] = in ? a.cached_lens[r0 + k] : 0;
+        n[k] = in ? a.new_lens[r0 + k] : 0;
+    }
+    int32_t fresh[PER], take[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const Req q = request(s, c[k], n[k]);
+        nt += fresh[k] = q.fresh;
+        np += take[k] = q.take;
         flags |= q.flags;
-        if (blockIdx.x == 0) flags |= held_flags(a, q, r);
+        if (r0 + k < R) {
+            old[r0 + k] = q.cached;
+        }
+    }
+    if (checks && a.table_width > 0 && R > 0) {
+        int32_t page[PER];  // all asked for before the first is looked at
+#pragma unroll
+        for (int k = 0; k < PER; ++k) page[k] = shared_page(s, request(s, c[k], n[k]), min(r0 + k, R - 1));
+#pragma unroll
+        for (int k = 0; k < PER; ++k)
+            if (r0 + k < R && shares_page(s, request(s, c[k], n[k])) && !good_page(a, page[k])) flags |= SILI_SLOTS_BAD_PAGE;
     }
     block_scan<FEW_TPB>(nt, np, T, P, s_part);
-    for (int r = r0; r < r1; ++r) {
-        const Req q = request(a, r);
-        tok[r] = (int32_t)min(nt, (int64_t)INT32_MAX);
-        pag[r] = (int32_t)min(np, (int64_t)INT32_MAX);
-        nt += q.fresh;
-        np += q.take;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        if (r0 + k < R) {
+            tok[r0 + k] = (int32_t)min(nt, (int64_t)INT32_MAX);
+            pag[r0 + k] = (int32_t)min(np, (int64_t)INT32_MAX);
+            if (r0 + k >= mine0 && r0 + k < mine1) {
+                a.q_start[r0 + k] = tok[r0 + k];
+                a.kv_lens[r0 + k] = old[r0 + k] + fresh[k];
+            }
+        }
+        nt += fresh[k];
+        np += take[k];
     }
     __syncthreads();
-    const int64_t first = (int64_t)blockIdx.x * FEW_TPB + threadIdx.x, step = (int64_t)gridDim.x * FEW_TPB;
-    for (int64_t r = first; r <= R; r += step) {
-        a.q_start[r] = r < R ? tok[r] : (int32_t)min(T, (int64_t)INT32_MAX);
-        if (r < R) {
-            const Req q = request(a, r);
-            a.kv_lens[r] = q.cached + q.fresh;
-        }
-    }
-    for (int64_t i = first; i < P && i < INT32_MAX; i += step) {
-        const int64_t r = owner(pag, R, i);
-        const int64_t at = request(a, r).have + (i - pag[r]);
-        if (at < a.table_width) a.block_table[r * a.table_width + at] = i < a.n_free ? a.free_pages[i] : -1;
-    }
-    for (int64_t t = first; t < a.max_tokens; t += step) {
-        int32_t pos = 0, slot = -1;
-        if (t < T) {
-            const int64_t r = owner(tok, R, t);
-            const Req q = request(a, r);
-            pos = q.cached + (int32_t)(t - tok[r]);
-            const uint32_t at = (uint32_t)pos / (uint32_t)a.page_size;
-            int32_t page = -1;
-            if ((int64_t)at >= a.table_width) page = -1;
-            else if ((int32_t)at < q.have) page = a.block_table[r * a.table_width + at];
-            else {
-                const int64_t i = (int64_t)pag[r] + ((int32_t)at - q.have);
-                page = i < a.n_free ? a.free_pages[i] : -1;
-            }
-            slot = slot_of(a, page, (uint32_t)pos - at * (uint32_t)a.page_size);
-        }
-        a.positions[t] = pos;
-        a.slots[t] = slot;
-    }
-    if (blockIdx.x == 0) {
-        const int64_t n = min(P, a.n_free);
-        for (int64_t i = threadIdx.x; i < n; i += FEW_TPB)
+    if (checks) {
+        const int64_t n_taken = min(P, a.n_free);
+#pragma unroll 8
+        for (int64_t i = threadIdx.x; i < n_taken; i += FEW_TPB)
             if (!good_page(a, a.free_pages[i])) flags |= SILI_SLOTS_BAD_PAGE;
         if (P > a.n_free) flags |= SILI_SLOTS_NO_PAGE;
         if (T > a.max_tokens) flags |= SILI_SLOTS_TOKENS_FULL;
         if (flags) atomicOr(&s_flags, flags);
         __syncthreads();
         if (threadIdx.x == 0) {
-            a.status[0] = (int32_t)min(n, (int64_t)INT32_MAX);
+            a.status[0] = (int32_t)min(n_taken, (int64_t)INT32_MAX);
             a.status[1] = (int32_t)s_flags;
         }
+        if (gridDim.x > 1) return;
+    }
+    const int64_t first = (int64_t)blockIdx.x * FEW_TPB + threadIdx.x, step = (int64_t)sharing * FEW_TPB;
+    if (first == 0) a.q_start[R] = (int32_t)min(T, (int64_t)INT32_MAX);
+    const uint32_t mask = (uint32_t)a.page_size - 1u;
+    for (int64_t t = first; t < a.max_tokens; t += step) {
+        int32_t pos = 0, slot = -1;
+        if (t < T) {
+            const int32_t r = (int32_t)owner(tok, R, t), held = old[r];
+            pos = held + (int32_t)(t - tok[r]);
+            const uint32_t at = page_of(s, (uint32_t)pos);
+            const int32_t have = (int32_t)page_of(s, (uint32_t)held + mask);
+            int32_t page = -1;
+            if ((int64_t)at < a.table_width) {
+                const int64_t i = (int64_t)pag[r] + ((int32_t)at - have);
+                if ((int32_t)at < have) page = a.block_table[r * a.table_width + at];
+                else if (i < a.n_free) page = a.free_pages[i];
+            }
+            slot = slot_of(a, page, (uint32_t)pos - at * (uint32_t)a.page_size);
+        }
+        a.positions[t] = pos;
+        a.slots[t] = slot;
+    }
+    for (int64_t i = first; i < P && i < INT32_MAX; i += step) {
+        const int64_t r = owner(pag, R, i);
+        const int64_t at = (int64_t)page_of(s, (uint32_t)old[r] + mask) + (i - pag[r]);
+        if (at < a.table_width) a.block_table[r * a.table_width + at] = i < a.n_free ? a.free_pages[i] : -1;
     }
 }
 
 // More requests: one block walks them in order and writes their rows, then a
 // second launch takes the tokens, which find their request in q_start and
 // their page in the table.
-__global__ __launch_bounds__(MANY_TPB) void k_slots_rows(sili_request_slots_args a) {
+__global__ __launch_bounds__(MANY_TPB) void k_slots_rows(Step s) {
+    const sili_request_slots_args &a = s.a;
     __shared__ int64_t s_part[2][MANY_TPB / 64];
     __shared__ uint32_t s_flags;
     if (threadIdx.x == 0) s_flags = 0;
@@ -191,11 +232,12 @@ __global__ __launch_bounds__(MANY_TPB) void k_slots_rows(sili_request_slots_args
     for (int64_t c = 0; c < a.requests; c += MANY_TPB) {
         const int64_t r = c + threadIdx.x;
         Req q{};
-        if (r < a.requests) q = request(a, r);
+        if (r < a.requests) q = request(s, a.cached_lens[r], a.new_lens[r]);
         int64_t nt = q.fresh, np = q.take, T, P;
         block_scan<MANY_TPB>(nt, np, T, P, s_part);
         if (r < a.requests) {
-            flags |= q.flags | held_flags(a, q, r);
+            flags |= q.flags;
+            if (shares_page(s, q) && !good_page(a, shared_page(s, q, r))) flags |= SILI_SLOTS_BAD_PAGE;
             a.q_start[r] = (int32_t)min(baseT + nt, (int64_t)INT32_MAX);
             a.kv_lens[r] = q.cached + q.fresh;
             for (int32_t j = 0; j < q.take && (int64_t)q.have + j < a.table_width; ++j) {
@@ -220,14 +262,15 @@ __global__ __launch_bounds__(MANY_TPB) void k_slots_rows(sili_request_slots_args
     }
 }
 
-__global__ __launch_bounds__(256) void k_slots_tokens(sili_request_slots_args a) {
+__global__ __launch_bounds__(256) void k_slots_tokens(Step s) {
+    const sili_request_slots_args &a = s.a;
     const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (t >= a.max_tokens) return;
     int32_t pos = 0, slot = -1;
     if (t < (int64_t)a.q_start[a.requests]) {
         const int64_t r = owner(a.q_start, a.requests, t);
         pos = max(a.cached_lens[r], 0) + (int32_t)(t - a.q_start[r]);
-        const uint32_t at = (uint32_t)pos / (uint32_t)a.page_size;
+        const uint32_t at = page_of(s, (uint32_t)pos);
         if ((int64_t)at < a.table_width)
             slot = slot_of(a, a.block_table[r * a.table_width + at], (uint32_t)pos - at * (uint32_t)a.page_size);
     }
@@ -248,13 +291,18 @@ void request_slots(const sili_request_slots_args &a, hipStream_t st) {
     require(a.n_free == 0 || a.free_pages, "request_slots: NULL free_pages");
     require(a.max_tokens == 0 || (a.positions && a.slots), "request_slots: NULL buffer");
     require(a.q_start && a.status, "request_slots: NULL buffer");
+    Step s{a, -1};
+    if ((a.page_size & (a.page_size - 1)) == 0) s.shift = __builtin_ctzll((unsigned long long)a.page_size);
     if (a.requests <= FEW) {
-        // four tokens a thread, and no more blocks than the GPU runs at once
-        const int64_t blocks = std::clamp<int64_t>((a.max_tokens + 4 * FEW_TPB - 1) / (4 * FEW_TPB), 1, 512);
-        launch(k_slots_few, dim3((unsigned)blocks), dim3(FEW_TPB), (uint32_t)(8 * std::max<int64_t>(a.requests, 1)), st, a);
+        // a token a thread until every CU has a block, and one to check
+        int64_t blocks = std::clamp<int64_t>((a.max_tokens + FEW_TPB - 1) / FEW_TPB, 1, 255);
+        if (blocks > 1) ++blocks;
+        const uint32_t lds = (uint32_t)(12 * std::max<int64_t>(a.requests, 1));
+        if (a.requests <= (int)FEW_TPB) launch(k_slots_few<1>, dim3((unsigned)blocks), dim3(FEW_TPB), lds, st, s);
+        else launch(k_slots_few<FEW / (int)FEW_TPB>, dim3((unsigned)blocks), dim3(FEW_TPB), lds, st, s);
     } else {
-        launch(k_slots_rows, dim3(1), dim3(MANY_TPB), 0, st, a);
-        if (a.max_tokens > 0) launch(k_slots_tokens, dim3((unsigned)((a.max_tokens + 255) / 256)), dim3(256), 0, st, a);
+        launch(k_slots_rows, dim3(1), dim3(MANY_TPB), 0, st, s);
+        if (a.max_tokens > 0) launch(k_slots_tokens, dim3((unsigned)((a.max_tokens + 255) / 256)), dim3(256), 0, st, s);
     }
     SILI_HIP(hipGetLastError());
 }
