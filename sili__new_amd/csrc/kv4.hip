@@ -125,23 +125,20 @@ __global__ __launch_bounds__(ROWS_TPB) void k_kv4_rows(sili_kv4_rows_args a, boo
 // ---- attention -----------------------------------------------------------------
 //
 // Rows of a (request, kv head) are its query tokens times the group of query
-// heads that share the kv head: row = token * group + head in group.  A wave
-// takes 16 NT of them against 64 keys a step, on the bf16 matrix cores:
+// heads that share the kv head: row = token * group + head in group.  Both
+// kernels take 64 keys a step on the bf16 matrix cores:
 //
-//   S^T = K q^T    16 keys x 16 rows a tile, codes x q, four tiles a step
+//   S^T = K q^T               codes x q
 //   p   = exp2(c (k_scale S - m)),   l += p
-//   O^T += V^T (v_scale p)^T         16 channels x 16 rows a tile
+//   O^T += V^T (v_scale p)^T  codes x weights
 //
 // E2M1 codes are exact in bf16, and the two scales of a key multiply its score
 // and its weight in fp32, so the cache's values lose nothing; q and p enter in
-// one bf16 part or two (the second the rest of the first), 8 or 16 significant
-// bits.  In both products the row is the lane's column (lane % 16), and with
-//     tile x row of K  ->  key 16 (row / 4) + 4 x + row % 4
-// the lane's four results of the four score tiles are the keys 16 g .. 16 g +
-// 15, g = lane / 16: the very k indices its share of the second product's right
-// operand holds, so no score moves between lanes.  The left operands come from
-// memory as the lane needs them: 32 channels of a K row are 16 bytes, and 16
-// keys of a V channel pair are 16 bytes.
+// bf16 parts, each the nearest to what the parts before leave.  With the scores
+// transposed a row is a lane's column in both products, so its statistics and
+// its scaling need no exchange, and the key order is chosen so that the scores
+// a lane holds are the k indices its share of the second product's right operand
+// takes: no weight moves between lanes.
 //
 // The running maximum m is raised only when a score passes it by 2^8 (in exp2's
 // argument 8): until then weights stay below 2^8 and nothing has to be rescaled.
@@ -153,8 +150,13 @@ typedef __attribute__((ext_vector_type(2))) float f32x2;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+
 __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 __device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){x, y}, bf16x2));
@@ -195,11 +197,11 @@ __device__ __forceinline__ float lanes_sum(float v) {
 // bf16 parts of q: 24 bits of fp32, all 11 of f16, all 8 of bf16.
 template <typename T>
 constexpr int q_parts() { return sizeof(T) == 4 ? 3 : __is_same(T, __bf16) ? 1 : 2; }
-// ... of p: 24 bits for fp32, 16 for f16.  bf16 takes one where the matrix
-// cores' time counts (its rounding is as large as the output's own, together
-// 1.4 times that), two where memory bounds the kernel.
-template <typename T, bool BY_KEYS>
-constexpr int p_parts() { return sizeof(T) == 4 ? 3 : __is_same(T, __bf16) && !BY_KEYS ? 1 : 2; }
+// ... of p: 24 bits for fp32, 16 for f16.  bf16 takes two where memory bounds the
+// kernel (FEW rows), one where the matrix cores' time counts: its rounding is as
+// large as the output's own, together 1.4 times that.
+template <typename T, bool FEW>
+constexpr int p_parts() { return sizeof(T) == 4 ? 3 : __is_same(T, __bf16) && !FEW ? 1 : 2; }
 // x, y in N parts: part k the bf16 nearest to what the parts before leave.
 template <int N>
 __device__ __forceinline__ void split_bf16(float x, float y, uint32_t (&part)[N]) {
@@ -271,30 +273,38 @@ struct KeyRange {
 };
 
 // Registers allow this many waves on a SIMD without spilling.
-template <typename T, int D, bool BY_KEYS, int CP>
+template <typename T, int D, int CP>
 constexpr int waves_per_simd() {
-    if (!BY_KEYS) return 1;
     constexpr bool lean = __is_same(T, __bf16) || (CP > 1 && D < 256);  // no more than two parts in registers
     return (D == 64 ? 4 : D == 128 ? 3 : 2) - (lean ? 0 : 1);
 }
 
-// BY_KEYS: the block's waves share 16 NT rows and take every fourth step of
-// keys each; their results are joined in LDS.  Otherwise each wave has rows of
-// its own.
+// ... of the many-rows kernel.
+template <typename T, int D>
+constexpr int many_waves() { return __is_same(T, __bf16) && D <= 128 ? 2 : 1; }
+
+// Few rows: a tile of 16 a block, whose waves take a step of keys each in turn and
+// are joined in LDS; every byte of the cache goes from memory to one wave's
+// registers, a step ahead.  Memory bounds it (8 kv heads of 5.1 K keys a request,
+// 128 requests: 153 us, 4.6 TB/s of the 5.65 that the loads alone reach).  With
+//     16x16 tile x, row of K  ->  key 16 (row / 4) + 4 x + row % 4
+// a lane's results of the four score tiles are the keys 16 g .. 16 g + 15, g =
+// lane / 16.  The left operands come from memory as the lane needs them: a
+// quarter of a K row, and 16 keys of a V channel pair, are 16 bytes each.
 //
 // CP > 1: with 16 / CP rows at most, the parts of q and p go to the columns that
 // would be empty instead of to products of their own: column r + (16 / CP) k
 // holds part k of row r.  Scores are summed over a row's columns (rotations
 // within 16 lanes), so every one of them holds the row's weights and takes its
 // own part of them; the outputs are summed once, at the end.
-template <typename T, int D, int NT, bool BY_KEYS, int WAVES, int CP = 1>
-__global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, BY_KEYS, CP>())) void k_attend(sili_kv4_attend_args a, AttendPlan pl) {
-    constexpr int QP = q_parts<T>(), PP = p_parts<T, BY_KEYS>();
+template <typename T, int D, int WAVES, int CP>
+__global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_attend_few(sili_kv4_attend_args a, AttendPlan pl) {
+    constexpr int QP = q_parts<T>(), PP = p_parts<T, true>();
     constexpr int KS = D / 32;   // steps of 32 channels
     constexpr int CT = D / 32;   // blocks of 32 output channels
     constexpr int RT = 16 / CP;  // rows of a tile
     constexpr int QM = CP > 1 ? 1 : QP, PM = CP > 1 ? 1 : PP;  // products each
-    static_assert(CP == 1 || (BY_KEYS && NT == 1 && CP >= QP && CP >= PP), "parts fit the columns");
+    static_assert(CP == 1 || (CP >= QP && CP >= PP), "parts fit the columns");
     extern __shared__ float s_join[];
     const sili_kv4_cache &cache = a.cache;
     const int wave = (int)uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, r16 = lane & 15;
@@ -302,10 +312,10 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, BY_KEYS, CP>())) 
     const int H = pl.kv_heads, group = pl.group;
     const int h = blockIdx.x % H, tile = blockIdx.x / H, split = blockIdx.y, req = blockIdx.z;
     const int32_t *table = a.block_table + (int64_t)req * a.table_width;
-    const int32_t stride = BY_KEYS ? 64 * WAVES : 64;
+    constexpr int32_t stride = 64 * WAVES;
     // the page of the first step, asked for before the lengths are here (the
     // table has the entry whatever they say)
-    int32_t key = split * pl.chunk + (BY_KEYS ? 64 * wave : 0);
+    int32_t key = split * pl.chunk + 64 * wave;
     auto entry = [&](int32_t k) {
         const int32_t mine = (k >> 4) + g;
         return table[pl.page_shift >= 0 ? mine >> pl.page_shift : mine / pl.groups_per_page];
@@ -317,15 +327,15 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, BY_KEYS, CP>())) 
     const int32_t n_all = a.q_start[req + 1] - q0, n = min(n_all, (int32_t)a.max_new);
     const int32_t kv = a.kv_lens[req];
     const int32_t n_rows = n * group;
-    const int32_t first = (BY_KEYS ? tile : tile * WAVES + wave) * (RT * NT);
+    const int32_t first = tile * RT;
     if (q0 < 0 || n_rows <= pl.few || n_rows > pl.many) return;
-    if (first >= n_rows) return;  // BY_KEYS: the whole block
+    if (first >= n_rows) return;
     KeyRange kr;
     kr.base = kv - n_all;
     kr.window = (int32_t)a.window;
     kr.causal = a.causal != 0;
     kr.cap = min(kv, pl.most);
-    const int32_t i_first = token_of(pl, first), i_last = token_of(pl, min(first + RT * NT - 1, n_rows - 1));
+    const int32_t i_first = token_of(pl, first), i_last = token_of(pl, min(first + RT - 1, n_rows - 1));
     const int32_t lo = kr.begin(i_first) & ~63, hi = kr.end(i_last);
     const int32_t all_end = kr.end(i_first), all_begin = kr.begin(i_last);  // what every row sees
     const int32_t c0 = lo + split * pl.chunk, c1 = min(hi, c0 + pl.chunk);
@@ -337,13 +347,11 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, BY_KEYS, CP>())) 
     for (int k = 0; k < PP; ++k) take_p[k] = my_part == k ? ~0u : 0u;
 
     // this lane's rows
-    int32_t end[NT], begin[NT];
-    u32x4 q[NT][KS][QM];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int32_t row = min(first + 16 * t + my_row, n_rows - 1), i = token_of(pl, row);
-        end[t] = kr.end(i);
-        begin[t] = kr.begin(i);
+    const int32_t my_i = token_of(pl, min(first + my_row, n_rows - 1));
+    const int32_t end = kr.end(my_i), begin = kr.begin(my_i);
+    u32x4 q[KS][QM];
+    {
+        const int32_t row = min(first + my_row, n_rows - 1), i = my_i;
         const int64_t token = q0 + i;
         const T *src = (const T *)a.q + (token < a.tokens ? token * a.q_token_stride : 0) +
                        (h * group + (row - i * group)) * a.q_head_stride + g * (D / 4);
@@ -367,20 +375,15 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, BY_KEYS, CP>())) 
                 uint32_t part[QP];
                 split_bf16<QP>(x[2 * j], x[2 * j + 1], part);
 #pragma unroll
-                for (int k = 0; k < QM; ++k) q[t][s][k][j] = CP > 1 && QP > 1 ? pick<QP>(part, take_q) : part[k];
+                for (int k = 0; k < QM; ++k) q[s][k][j] = CP > 1 && QP > 1 ? pick<QP>(part, take_q) : part[k];
             }
         }
     }
 
-    float m[NT], l[NT];  // m in units of c; l this lane's keys only
-    f32x4 o[NT][CT][2];
+    float m = -INFINITY, l = 0.0f;  // m in units of c; l of this lane's keys only
+    f32x4 o[CT][2];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        m[t] = -INFINITY;
-        l[t] = 0.0f;
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) o[t][ct][0] = o[t][ct][1] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-    }
+    for (int ct = 0; ct < CT; ++ct) o[ct][0] = o[ct][1] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 
     // The keys of a step as this lane needs them, loaded a step ahead: a part's
     // registers take the next step's as soon as this one's are used.
@@ -436,20 +439,16 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, BY_KEYS, CP>())) 
         page = page_of(key + stride);
     }
     for (; key < c1; key += stride) {
-        f32x4 sc[NT][4];
+        f32x4 sc[4];
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) sc[t][x] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+        for (int x = 0; x < 4; ++x) sc[x] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int x = 0; x < 4; ++x)
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
                 const u32x4 kk = codes8(kw[x][s]);
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int k = 0; k < QM; ++k) sc[t][x] = mma(kk, q[t][s][k], sc[t][x]);
+                for (int k = 0; k < QM; ++k) sc[x] = mma(kk, q[s][k], sc[x]);
             }
         // wave-uniform: every row sees every key of the step
         const bool here = held, whole = key >= all_begin && key + 64 <= all_end && __all(here);
@@ -459,61 +458,58 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, BY_KEYS, CP>())) 
             load_k();
             page = page_of(key + 2 * stride);
         }
-        u32x4 p[NT][2][PM];
+        u32x4 p[2][PM];
+        float v[16], w[16];  // scores, then weights, of keys 16 g + 0 .. 15
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            float v[16], w[16];  // scores, then weights, of keys 16 g + 0 .. 15
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                v[j] = sc[t][j >> 2][j & 3];
-                if (QP > 1) v[j] = columns_sum<CP>(v[j]);
-            }
-            times_scales(v, ks);
-            if (!whole) {
-                const int32_t from = here ? begin[t] - (key + 16 * g) : 16, to = end[t] - (key + 16 * g);
-#pragma unroll
-                for (int j = 0; j < 16; ++j) v[j] = j >= from && j < to ? v[j] : -INFINITY;
-            }
-            float top = v[0];
-#pragma unroll
-            for (int j = 1; j < 16; ++j) top = fmaxf(top, v[j]);
-            top *= pl.c;
-            if (__any(top > m[t] + SLACK)) {
-                const float up = fmaxf(m[t], lanes_max(top));
-                // a row without a key so far keeps m = -inf, and factor 1 on its zeros
-                const float keep = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[t] - up);
-                m[t] = up;
-                l[t] *= keep;
-#pragma unroll
-                for (int ct = 0; ct < CT; ++ct) {
-                    o[t][ct][0] *= keep;
-                    o[t][ct][1] *= keep;
-                }
-            }
-            const float ref = m[t] == -INFINITY ? 0.0f : m[t];
-            float sum = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(v[j], pl.c, -ref));
-                sum += w[j];
-            }
-            l[t] += sum;
-            times_scales(w, vs);
-            if (!whole) {
-                // a key that this row does not see may hold anything
-#pragma unroll
-                for (int j = 0; j < 16; ++j) w[j] = v[j] == -INFINITY ? 0.0f : w[j];
-            }
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint32_t part[PP];
-                    split_bf16<PP>(w[8 * e + 2 * j], w[8 * e + 2 * j + 1], part);
-#pragma unroll
-                    for (int k = 0; k < PM; ++k) p[t][e][k][j] = CP > 1 ? pick<PP>(part, take_p) : part[k];
-                }
+        for (int j = 0; j < 16; ++j) {
+            v[j] = sc[j >> 2][j & 3];
+            if (QP > 1) v[j] = columns_sum<CP>(v[j]);
         }
+        times_scales(v, ks);
+        if (!whole) {
+            const int32_t from = here ? begin - (key + 16 * g) : 16, to = end - (key + 16 * g);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = j >= from && j < to ? v[j] : -INFINITY;
+        }
+        float top = v[0];
+#pragma unroll
+        for (int j = 1; j < 16; ++j) top = fmaxf(top, v[j]);
+        top *= pl.c;
+        if (__any(top > m + SLACK)) {
+            const float up = fmaxf(m, lanes_max(top));
+            // a row without a key so far keeps m = -inf, and factor 1 on its zeros
+            const float keep = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - up);
+            m = up;
+            l *= keep;
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+                o[ct][0] *= keep;
+                o[ct][1] *= keep;
+            }
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(v[j], pl.c, -ref));
+            sum += w[j];
+        }
+        l += sum;
+        times_scales(w, vs);
+        if (!whole) {
+            // a key that this row does not see may hold anything
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j] = v[j] == -INFINITY ? 0.0f : w[j];
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint32_t part[PP];
+                split_bf16<PP>(w[8 * e + 2 * j], w[8 * e + 2 * j + 1], part);
+#pragma unroll
+                for (int k = 0; k < PM; ++k) p[e][k][j] = CP > 1 ? pick<PP>(part, take_p) : part[k];
+            }
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
@@ -523,119 +519,331 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, BY_KEYS, CP>())) 
                 codes_by_channel(e ? vw[ct].w : vw[ct].y, e1, o1);
                 const u32x4 even = {e0[0], e0[1], e1[0], e1[1]}, odd = {o0[0], o0[1], o1[0], o1[1]};
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int y = 0; y < PM; ++y) {
-                        o[t][ct][0] = mma(even, p[t][e][y], o[t][ct][0]);
-                        o[t][ct][1] = mma(odd, p[t][e][y], o[t][ct][1]);
-                    }
+                for (int y = 0; y < PM; ++y) {
+                    o[ct][0] = mma(even, p[e][y], o[ct][0]);
+                    o[ct][1] = mma(odd, p[e][y], o[ct][1]);
+                }
             }
         if (more) load_v();
     }
-#pragma unroll
-    for (int t = 0; t < NT; ++t) l[t] = lanes_sum(l[t]);
+    l = lanes_sum(l);
 
     // lane: row r16, channels 32 ct + 8 g + 2 i + (even, odd)
-    if (BY_KEYS) {
-        const int ROWS = pl.join_rows;
-        float *s_o = s_join, *s_m = s_join + WAVES * ROWS * D, *s_l = s_m + WAVES * ROWS;
+    const int ROWS = pl.join_rows;
+    float *s_o = s_join, *s_m = s_join + WAVES * ROWS * D, *s_l = s_m + WAVES * ROWS;
+    f32x4 sum[CT][2];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            f32x4 sum[CT][2];
+    for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-            for (int ct = 0; ct < CT; ++ct)
+        for (int i = 0; i < 4; ++i) {
+            sum[ct][0][i] = columns_sum<CP>(o[ct][0][i]);
+            sum[ct][1][i] = columns_sum<CP>(o[ct][1][i]);
+        }
+    if (first + r16 < n_rows && r16 < RT) {
+        float *dst = s_o + (wave * ROWS + r16) * D + 8 * g;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    sum[ct][0][i] = columns_sum<CP>(o[t][ct][0][i]);
-                    sum[ct][1][i] = columns_sum<CP>(o[t][ct][1][i]);
-                }
-            if (first + 16 * t + r16 >= n_rows || r16 >= RT) continue;
-            float *dst = s_o + (wave * ROWS + 16 * t + r16) * D + 8 * g;
+        for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-            for (int ct = 0; ct < CT; ++ct)
+            for (int i = 0; i < 4; ++i) {
+                dst[32 * ct + 2 * i] = sum[ct][0][i];
+                dst[32 * ct + 2 * i + 1] = sum[ct][1][i];
+            }
+        if (g == 0) {
+            s_m[wave * ROWS + r16] = m;
+            s_l[wave * ROWS + r16] = l;
+        }
+    }
+    __syncthreads();
+    const int rows = min(RT, n_rows - first);
+    for (int at = threadIdx.x; at < rows * (D / 4); at += 64 * WAVES) {
+        const int row = at / (D / 4), ch = 4 * (at - row * (D / 4));
+        float f[WAVES], mm = -INFINITY, ll = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    dst[32 * ct + 2 * i] = sum[ct][0][i];
-                    dst[32 * ct + 2 * i + 1] = sum[ct][1][i];
-                }
-            if (g == 0) {
-                s_m[wave * ROWS + 16 * t + r16] = m[t];
-                s_l[wave * ROWS + 16 * t + r16] = l[t];
+        for (int w = 0; w < WAVES; ++w) {
+            f[w] = s_m[w * ROWS + row];
+            mm = fmaxf(mm, f[w]);
+        }
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            // a wave without keys has m = -inf and zeros
+            f[w] = f[w] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(f[w] - mm);
+            ll += f[w] * s_l[w * ROWS + row];
+            const float4 x = *reinterpret_cast<const float4 *>(s_o + (w * ROWS + row) * D + ch);
+            acc[0] += f[w] * x.x;
+            acc[1] += f[w] * x.y;
+            acc[2] += f[w] * x.z;
+            acc[3] += f[w] * x.w;
+        }
+        const int32_t i = token_of(pl, first + row);
+        const int64_t token = q0 + i, qh = h * group + (first + row - i * group);
+        if (token >= a.tokens) continue;
+        if (pl.splits > 1) {
+            const int64_t slot = (token * a.q_heads + qh) * pl.splits + split;
+            if (ll != 0.0f) *reinterpret_cast<float4 *>(pl.part_o + slot * D + ch) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            if (ch == 0) pl.part_ml[slot] = make_float2(mm, ll);
+        } else {
+            const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j] *= inv;
+            store4<T>((T *)a.out + token * a.out_token_stride + qh * a.out_head_stride + ch, acc, pl.out_packed);
+            if (a.lse && ch == 0)
+                a.lse[token * a.q_heads + qh] = ll != 0.0f ? (mm + __builtin_amdgcn_logf(ll)) * 0.69314718f : -INFINITY;
+        }
+    }
+}
+
+// Many rows: 128 a block, 32 a wave.  The block turns a step's codes into bf16 once,
+// in LDS (two buffers: the next step's codes are asked for before this one's
+// products and written after them), and each wave takes its 32x32 tiles from
+// there.  With tile x of K's keys in order, a lane's 16 results are the keys
+// 32 x + 8 a + 4 hf + b (a, b < 4; hf = lane / 32), so V's keys lie in LDS in the
+// order 0-3, 8-11, 4-7, 12-15 of every 16: eight at 16 s + 8 hf are the lane's
+// own.  Rows of LDS are padded by 16 bytes, which spreads eight lanes' 16 bytes
+// over all banks.
+constexpr int MANY_WAVES = 4, MANY_ROWS = 32 * MANY_WAVES;
+
+template <int D>
+struct ManyLds {
+    static constexpr int K_ROW = 2 * D + 16, V_ROW = 2 * 64 + 16;  // bytes
+    uint8_t k[64 * K_ROW];  // [key][channel]
+    uint8_t v[D * V_ROW];   // [channel][key]
+    float ks[64], vs[64];
+    int32_t held[4];        // the group of 16 keys is in the cache
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(64 * MANY_WAVES, (many_waves<T, D>())) void k_attend_many(sili_kv4_attend_args a, AttendPlan pl) {
+    constexpr int QP = q_parts<T>(), PP = p_parts<T, false>();
+    constexpr int KS = D / 16, CT = D / 32;
+    constexpr int UN = D <= 128 ? 1 : D / 128;  // 16-byte units of K, and of V, a thread turns
+    using Lds = ManyLds<D>;
+    extern __shared__ __align__(16) uint8_t s_many[];
+    Lds *lds = reinterpret_cast<Lds *>(s_many);
+    const sili_kv4_cache &cache = a.cache;
+    const int tid = threadIdx.x, wave = (int)uniform(tid >> 6), lane = tid & 63, hf = lane >> 5, r32 = lane & 31;
+    const int H = pl.kv_heads, group = pl.group;
+    const int h = blockIdx.x % H, tile = blockIdx.x / H, split = blockIdx.y, req = blockIdx.z;
+    const int32_t *table = a.block_table + (int64_t)req * a.table_width;
+    const int32_t q0 = a.q_start[req];
+    const int32_t n_all = a.q_start[req + 1] - q0, n = min(n_all, (int32_t)a.max_new);
+    const int32_t kv = a.kv_lens[req];
+    const int32_t n_rows = n * group;
+    const int32_t block_first = tile * MANY_ROWS;
+    if (q0 < 0 || n_rows <= pl.few || n_rows > pl.many || block_first >= n_rows) return;
+    KeyRange kr;
+    kr.base = kv - n_all;
+    kr.window = (int32_t)a.window;
+    kr.causal = a.causal != 0;
+    kr.cap = min(kv, pl.most);
+    const int32_t lo = kr.begin(token_of(pl, block_first)) & ~63, hi = kr.end(token_of(pl, min(block_first + MANY_ROWS, n_rows) - 1));
+    const int32_t c0 = lo + split * pl.chunk, c1 = min(hi, c0 + pl.chunk);
+
+    // this wave's rows (past the last: the last again), and this lane's
+    const int32_t first = block_first + 32 * wave, row = min(first + r32, n_rows - 1), my_i = token_of(pl, row);
+    const int32_t i_first = token_of(pl, min(first, n_rows - 1)), i_last = token_of(pl, min(first + 31, n_rows - 1));
+    const int32_t end = kr.end(my_i), begin = kr.begin(my_i);
+    const int32_t w_begin = kr.begin(i_first), w_end = first < n_rows ? kr.end(i_last) : 0;  // what any row sees
+    const int32_t all_end = kr.end(i_first), all_begin = kr.begin(i_last);                   // what every row sees
+
+    u32x4 q[KS][QP];  // channels 16 s + 8 hf + 0 .. 7
+    {
+        const int64_t token = q0 + my_i;
+        const T *src = (const T *)a.q + (token < a.tokens ? token * a.q_token_stride : 0) +
+                       (h * group + (row - my_i * group)) * a.q_head_stride + 8 * hf;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            float x[8];
+            load8<T>(src + 16 * s, pl.q_packed, x);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint32_t part[QP];
+                split_bf16<QP>(pl.negative ? -x[2 * j] : x[2 * j], pl.negative ? -x[2 * j + 1] : x[2 * j + 1], part);
+#pragma unroll
+                for (int k = 0; k < QP; ++k) q[s][k][j] = part[k];
             }
         }
+    }
+
+    float m = -INFINITY, l = 0.0f;  // m in units of c; l of this lane's keys only
+    f32x16 o[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[ct][i] = 0.0f;
+
+    // A step's codes: unit u = (key, 32 channels) of K and (16 keys, channel pair)
+    // of V, both of the step's group of 16 keys u / (D / 2).
+    uint4 kw[UN], vw[UN];
+    float scale = 0.0f;
+    int32_t held = 0;
+    auto place = [&](int32_t key, int sub, bool &in) -> int64_t {  // group `sub` of the step at `key`, in groups of 16 keys
+        const int32_t mine = (key >> 4) + sub;
+        const int32_t pi = pl.page_shift >= 0 ? mine >> pl.page_shift : mine / pl.groups_per_page;
+        const int32_t page = 16 * mine < kr.cap ? table[pi] : -1;
+        in = page >= 0 && page < pl.n_pages;
+        return in ? (int64_t)(page * H + h) * pl.groups_per_page + (mine - pi * pl.groups_per_page) : (int64_t)h * pl.groups_per_page;
+    };
+    auto fetch = [&](int32_t key) {
+#pragma unroll
+        for (int j = 0; j < UN; ++j) {
+            const int u = tid + 256 * j;
+            if (D < 128 && u >= 2 * D) break;
+            bool in;
+            const int64_t at = place(key, u / (D / 2), in) * (8 * D) + (u % (D / 2)) * 16;
+            kw[j] = *reinterpret_cast<const uint4 *>(cache.k + at);
+            vw[j] = *reinterpret_cast<const uint4 *>(cache.v + at);
+        }
+        if (tid < 128) {
+            bool in;
+            const int64_t at = place(key, (tid & 63) >> 4, in) * 16 + (tid & 15);
+            scale = (tid < 64 ? cache.k_scale : cache.v_scale)[at];
+            held = in;
+        }
+    };
+    auto unpack = [&](Lds &b) {
+#pragma unroll
+        for (int j = 0; j < UN; ++j) {
+            const int u = tid + 256 * j;
+            if (D < 128 && u >= 2 * D) break;
+            u32x4 *kd = reinterpret_cast<u32x4 *>(b.k + (u / (D / 32)) * Lds::K_ROW + (u % (D / 32)) * 64);
+            kd[0] = codes8(kw[j].x);
+            kd[1] = codes8(kw[j].y);
+            kd[2] = codes8(kw[j].z);
+            kd[3] = codes8(kw[j].w);
+            uint32_t e[4][2], d[4][2];
+            codes_by_channel(vw[j].x, e[0], d[0]);
+            codes_by_channel(vw[j].y, e[1], d[1]);
+            codes_by_channel(vw[j].z, e[2], d[2]);
+            codes_by_channel(vw[j].w, e[3], d[3]);
+            uint8_t *vd = b.v + 2 * (u % (D / 2)) * Lds::V_ROW + (u / (D / 2)) * 32;
+            *reinterpret_cast<u32x4 *>(vd) = (u32x4){e[0][0], e[0][1], e[2][0], e[2][1]};
+            *reinterpret_cast<u32x4 *>(vd + 16) = (u32x4){e[1][0], e[1][1], e[3][0], e[3][1]};
+            *reinterpret_cast<u32x4 *>(vd + Lds::V_ROW) = (u32x4){d[0][0], d[0][1], d[2][0], d[2][1]};
+            *reinterpret_cast<u32x4 *>(vd + Lds::V_ROW + 16) = (u32x4){d[1][0], d[1][1], d[3][0], d[3][1]};
+        }
+        if (tid < 128) (tid < 64 ? b.ks : b.vs)[tid & 63] = scale;
+        if (tid < 64 && (tid & 15) == 0) b.held[tid >> 4] = held;
+    };
+
+    if (c0 < c1) {
+        fetch(c0);
+        unpack(lds[0]);
+    }
+    int buf = 0;
+    for (int32_t key = c0; key < c1; key += 64, buf ^= 1) {
         __syncthreads();
-        const int rows = min(RT * NT, n_rows - first);
-        for (int at = threadIdx.x; at < rows * (D / 4); at += 64 * WAVES) {
-            const int row = at / (D / 4), ch = 4 * (at - row * (D / 4));
-            float f[WAVES], mm = -INFINITY, ll = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const Lds &b = lds[buf];
+        const bool more = key + 64 < c1;
+        if (more) fetch(key + 64);
+        if (key < w_end && key + 64 > w_begin) {
+            f32x16 sc[2];
 #pragma unroll
-            for (int w = 0; w < WAVES; ++w) {
-                f[w] = s_m[w * ROWS + row];
-                mm = fmaxf(mm, f[w]);
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sc[x][i] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const u32x4 kk = *reinterpret_cast<const u32x4 *>(b.k + (32 * x + r32) * Lds::K_ROW + 32 * s + 16 * hf);
+#pragma unroll
+                    for (int k = 0; k < QP; ++k) sc[x] = mma(kk, q[s][k], sc[x]);
+                }
+            // wave-uniform: every row sees every key of the step
+            const int4 in = *reinterpret_cast<const int4 *>(b.held);
+            const bool whole = key >= all_begin && key + 64 <= all_end && uniform(in.x & in.y & in.z & in.w) != 0;
+            float v[32];  // scores, then weights: 16 x + 4 a + b
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+                const float4 f = *reinterpret_cast<const float4 *>(b.ks + 8 * y + 4 * hf);
+                v[4 * y] = sc[y >> 2][4 * (y & 3)] * f.x;
+                v[4 * y + 1] = sc[y >> 2][4 * (y & 3) + 1] * f.y;
+                v[4 * y + 2] = sc[y >> 2][4 * (y & 3) + 2] * f.z;
+                v[4 * y + 3] = sc[y >> 2][4 * (y & 3) + 3] * f.w;
             }
+            if (!whole) {
+                const int32_t from = begin - key - 4 * hf, to = end - key - 4 * hf;
+                const int32_t there[4] = {in.x, in.y, in.z, in.w};
 #pragma unroll
-            for (int w = 0; w < WAVES; ++w) {
-                // a wave without keys has m = -inf and zeros
-                f[w] = f[w] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(f[w] - mm);
-                ll += f[w] * s_l[w * ROWS + row];
-                const float4 x = *reinterpret_cast<const float4 *>(s_o + (w * ROWS + row) * D + ch);
-                acc[0] += f[w] * x.x;
-                acc[1] += f[w] * x.y;
-                acc[2] += f[w] * x.z;
-                acc[3] += f[w] * x.w;
-            }
-            const int32_t i = token_of(pl, first + row);
-            const int64_t token = q0 + i, qh = h * group + (first + row - i * group);
-            if (token >= a.tokens) continue;
-            if (pl.splits > 1) {
-                const int64_t slot = (token * a.q_heads + qh) * pl.splits + split;
-                if (ll != 0.0f) *reinterpret_cast<float4 *>(pl.part_o + slot * D + ch) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-                if (ch == 0) pl.part_ml[slot] = make_float2(mm, ll);
-            } else {
-                const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[j] *= inv;
-                store4<T>((T *)a.out + token * a.out_token_stride + qh * a.out_head_stride + ch, acc, pl.out_packed);
-                if (a.lse && ch == 0)
-                    a.lse[token * a.q_heads + qh] = ll != 0.0f ? (mm + __builtin_amdgcn_logf(ll)) * 0.69314718f : -INFINITY;
-            }
-        }
-    } else {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const int32_t row = first + 16 * t + r16;
-            const int32_t qi = token_of(pl, row);
-            const int64_t token = q0 + qi, qh = h * group + (row - qi * group);
-            if (row >= n_rows || token >= a.tokens) continue;
-            if (pl.splits > 1) {
-                const int64_t slot = (token * a.q_heads + qh) * pl.splits + split;
-                float *dst = pl.part_o + slot * D + 8 * g;
-                if (l[t] != 0.0f)
-#pragma unroll
-                    for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            dst[32 * ct + 2 * i] = o[t][ct][0][i];
-                            dst[32 * ct + 2 * i + 1] = o[t][ct][1][i];
-                        }
-                if (g == 0) pl.part_ml[slot] = make_float2(m[t], l[t]);
-            } else {
-                const float inv = l[t] != 0.0f ? 1.0f / l[t] : 0.0f;
-                T *out = (T *)a.out + token * a.out_token_stride + qh * a.out_head_stride + 8 * g;
-#pragma unroll
-                for (int ct = 0; ct < CT; ++ct) {
-                    float x[4];
+                for (int y = 0; y < 8; ++y)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        x[2 * (i & 1)] = o[t][ct][0][i] * inv;
-                        x[2 * (i & 1) + 1] = o[t][ct][1][i] * inv;
-                        if (i & 1) store4<T>(out + 32 * ct + 2 * (i - 1), x, pl.out_packed);
+                        const int32_t j = 8 * y + i;
+                        v[4 * y + i] = j >= from && j < to && there[y >> 1] ? v[4 * y + i] : -INFINITY;
                     }
+            }
+            float top = v[0];
+#pragma unroll
+            for (int j = 1; j < 32; ++j) top = fmaxf(top, v[j]);
+            top *= pl.c;
+            if (__any(top > m + SLACK)) {
+                const float up = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
+                // a row without a key so far keeps m = -inf, and factor 1 on its zeros
+                const float keep = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - up);
+                m = up;
+                l *= keep;
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct) o[ct] *= keep;
+            }
+            const float ref = m == -INFINITY ? 0.0f : m;
+            float sum = 0.0f;
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+                const float4 f = *reinterpret_cast<const float4 *>(b.vs + 8 * y + 4 * hf);
+                const float fs[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(v[4 * y + i], pl.c, -ref));
+                    sum += e;
+                    // a key that this row does not see may hold anything
+                    v[4 * y + i] = !whole && v[4 * y + i] == -INFINITY ? 0.0f : e * fs[i];
                 }
-                if (a.lse && g == 0)
-                    a.lse[token * a.q_heads + qh] = l[t] != 0.0f ? (m[t] + __builtin_amdgcn_logf(l[t])) * 0.69314718f : -INFINITY;
+            }
+            l += sum;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {  // 16 keys
+                u32x4 p[PP];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t part[PP];
+                    split_bf16<PP>(v[8 * s + 2 * j], v[8 * s + 2 * j + 1], part);
+#pragma unroll
+                    for (int k = 0; k < PP; ++k) p[k][j] = part[k];
+                }
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct) {
+                    const u32x4 vv = *reinterpret_cast<const u32x4 *>(b.v + (32 * ct + r32) * Lds::V_ROW + 32 * s + 16 * hf);
+#pragma unroll
+                    for (int k = 0; k < PP; ++k) o[ct] = mma(vv, p[k], o[ct]);
+                }
             }
         }
+        if (more) unpack(lds[buf ^ 1]);
+    }
+    l += __shfl_xor(l, 32, 64);
+
+    // lane: row r32, channels 32 ct + 8 a + 4 hf + 0 .. 3
+    const int64_t token = q0 + my_i, qh = h * group + (row - my_i * group);
+    if (first + r32 >= n_rows || token >= a.tokens) return;
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    const int64_t slot = (token * a.q_heads + qh) * pl.splits + split;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+            const int ch = 32 * ct + 8 * y + 4 * hf;
+            if (pl.splits > 1) {
+                if (l != 0.0f)
+                    *reinterpret_cast<float4 *>(pl.part_o + slot * D + ch) =
+                        make_float4(o[ct][4 * y], o[ct][4 * y + 1], o[ct][4 * y + 2], o[ct][4 * y + 3]);
+            } else {
+                const float x[4] = {o[ct][4 * y] * inv, o[ct][4 * y + 1] * inv, o[ct][4 * y + 2] * inv, o[ct][4 * y + 3] * inv};
+                store4<T>((T *)a.out + token * a.out_token_stride + qh * a.out_head_stride + ch, x, pl.out_packed);
+            }
+        }
+    if (hf == 0) {
+        if (pl.splits > 1) pl.part_ml[slot] = make_float2(m, l);
+        else if (a.lse) a.lse[token * a.q_heads + qh] = l != 0.0f ? (m + __builtin_amdgcn_logf(l)) * 0.69314718f : -INFINITY;
     }
 }
 
@@ -762,7 +970,6 @@ namespace {
 // Requests of up to FEW_ROWS rows have their keys shared by a block's waves, a
 // row tile of 16 each; larger ones give each wave rows of its own.
 constexpr int32_t FEW_ROWS = 64;
-constexpr int NT_MANY = 2, WAVES_MANY = 4;
 
 struct Launch {
     bool on = false;
@@ -777,7 +984,7 @@ int waves_of(int dtype, int64_t head_dim, int columns) {
         using T = decltype(z);
         auto of = [&](auto d) {
             constexpr int D = decltype(d)::value;
-            return 4 * (columns > 1 ? waves_per_simd<T, D, true, 2>() : waves_per_simd<T, D, true, 1>());
+            return 4 * (columns > 1 ? waves_per_simd<T, D, 2>() : waves_per_simd<T, D, 1>());
         };
         n = head_dim == 64 ? of(std::integral_constant<int, 64>{}) : head_dim == 128 ? of(std::integral_constant<int, 128>{})
                                                                                      : of(std::integral_constant<int, 256>{});
@@ -796,7 +1003,7 @@ void plan_attend(const sili_kv4_attend_args &a, Launch (&out)[2]) {
         p.group = (int32_t)group;
         p.group_inv = group == 1 ? ~0u : (uint32_t)((uint64_t(1) << 32) / (uint64_t)group);
         p.n_pages = (int32_t)a.cache.n_pages;
-        p.most = p.n_pages == 0 ? 0 : (int32_t)std::min(a.max_len, a.table_width * a.cache.page_size);
+        p.most = p.n_pages == 0 ? 0 : (int32_t)std::min({a.max_len, a.table_width * a.cache.page_size, int64_t(INT32_MAX) - (1 << 20)});
         const int64_t es = dtype_size(a.dtype);
         p.q_packed = aligned(a.q, (size_t)(8 * es)) && a.q_token_stride % 8 == 0 && a.q_head_stride % 8 == 0;
         p.out_packed = aligned(a.out, (size_t)(4 * es)) && a.out_token_stride % 4 == 0 && a.out_head_stride % 4 == 0;
@@ -810,7 +1017,7 @@ void plan_attend(const sili_kv4_attend_args &a, Launch (&out)[2]) {
         L.on = k == 0 || rows > FEW_ROWS;
         const int parts = a.dtype == SILI_F32 ? 4 : 2;
         p.columns = k == 0 && rows <= 16 / parts ? parts : 1;
-        const int64_t tile_rows = k == 0 ? 16 / p.columns : 16 * NT_MANY * WAVES_MANY;
+        const int64_t tile_rows = k == 0 ? 16 / p.columns : MANY_ROWS;
         L.tiles = (std::min<int64_t>(rows, p.many) + tile_rows - 1) / tile_rows;
         p.join_rows = (int32_t)std::min<int64_t>(16, rows);
         // keys a row tile can reach: its rows' windows, aligned to 64
@@ -827,7 +1034,7 @@ void plan_attend(const sili_kv4_attend_args &a, Launch (&out)[2]) {
         // splits until every CU has a wave on each SIMD as often as registers
         // allow; fp32, which the vector units bound, twice at most (320 blocks
         // of 2048 keys: 22.7 us, with a second split 21.4 + 4.7 to join)
-        const int64_t fill = k == 0 ? 256 * std::max(1, std::min(wide, a.dtype == SILI_F32 ? 8 : wide) / p.waves) : 2048;
+        const int64_t fill = k == 0 ? 256 * std::max(1, std::min(wide, a.dtype == SILI_F32 ? 8 : wide) / p.waves) : 512;
         const int64_t want = std::clamp<int64_t>(fill / blocks, 1, std::max<int64_t>(1, (reach + 255) / 256));
         p.chunk = (int32_t)std::max<int64_t>(step, ((reach + want - 1) / want + step - 1) / step * step);
         p.splits = (int32_t)std::max<int64_t>(1, (reach + p.chunk - 1) / p.chunk);
@@ -857,18 +1064,18 @@ void run_attend(const sili_kv4_attend_args &a, Launch (&L)[2], hipStream_t st) {
         const dim3 grid((unsigned)x, (unsigned)p.splits, (unsigned)a.requests);
         if (k == 0) {
             constexpr int PARTS = sizeof(T) == 4 ? 4 : 2;
-            constexpr int WIDE = 4 * waves_per_simd<T, D, true, 1>(), WIDE_P = 4 * waves_per_simd<T, D, true, PARTS>();
+            constexpr int WIDE = 4 * waves_per_simd<T, D, 1>(), WIDE_P = 4 * waves_per_simd<T, D, PARTS>();
             const uint32_t lds = p.waves * p.join_rows * (D + 2) * sizeof(float);
             const dim3 block(64 * p.waves);
             if (p.columns > 1) {
-                if (p.waves == WIDE_P) launch(k_attend<T, D, 1, true, WIDE_P, PARTS>, grid, block, lds, st, a, p);
-                else launch(k_attend<T, D, 1, true, 4, PARTS>, grid, block, lds, st, a, p);
+                if (p.waves == WIDE_P) launch(k_attend_few<T, D, WIDE_P, PARTS>, grid, block, lds, st, a, p);
+                else launch(k_attend_few<T, D, 4, PARTS>, grid, block, lds, st, a, p);
             } else {
-                if (p.waves == WIDE) launch(k_attend<T, D, 1, true, WIDE>, grid, block, lds, st, a, p);
-                else launch(k_attend<T, D, 1, true, 4>, grid, block, lds, st, a, p);
+                if (p.waves == WIDE) launch(k_attend_few<T, D, WIDE, 1>, grid, block, lds, st, a, p);
+                else launch(k_attend_few<T, D, 4, 1>, grid, block, lds, st, a, p);
             }
         } else {
-            launch(k_attend<T, D, NT_MANY, false, WAVES_MANY>, grid, dim3(64 * WAVES_MANY), 0, st, a, p);
+            launch(k_attend_many<T, D>, grid, dim3(64 * MANY_WAVES), (uint32_t)(2 * sizeof(ManyLds<D>)), st, a, p);
         }
         const int64_t rows = std::min<int64_t>(a.max_new * (a.q_heads / a.cache.kv_heads), p.many);
         if (p.splits > 1)
