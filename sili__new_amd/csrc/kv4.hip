@@ -253,6 +253,9 @@ __device__ __forceinline__ int32_t token_of(const AttendPlan &pl, int32_t row) {
     const int32_t q = (int32_t)__umulhi((uint32_t)row, pl.group_inv);
     return q + (row - q * pl.group >= pl.group ? 1 : 0);
 }
+// Keeps a wave-uniform branch that is seldom taken a branch: the compiler would
+// else turn it into selects that every step pays for, or keep its conditions.
+__device__ __forceinline__ void stay_branch(int32_t &x, int32_t &y) { __asm__ volatile("" : "+v"(x), "+v"(y)); }
 // Four channels of an output row.
 template <typename T>
 __device__ __forceinline__ void store4(T *out, const float (&x)[4], bool packed) {
@@ -467,7 +470,8 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_at
         }
         times_scales(v, ks);
         if (!whole) {
-            const int32_t from = here ? begin - (key + 16 * g) : 16, to = end - (key + 16 * g);
+            int32_t from = here ? begin - (key + 16 * g) : 16, to = end - (key + 16 * g);
+            stay_branch(from, to);
 #pragma unroll
             for (int j = 0; j < 16; ++j) v[j] = j >= from && j < to ? v[j] : -INFINITY;
         }
@@ -498,8 +502,10 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_at
         times_scales(w, vs);
         if (!whole) {
             // a key that this row does not see may hold anything
+            int32_t from = here ? begin - (key + 16 * g) : 16, to = end - (key + 16 * g);
+            stay_branch(from, to);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) w[j] = v[j] == -INFINITY ? 0.0f : w[j];
+            for (int j = 0; j < 16; ++j) w[j] = j >= from && j < to ? w[j] : 0.0f;
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e)
@@ -606,7 +612,7 @@ template <int D>
 struct ManyLds {
     static constexpr int K_ROW = 2 * D + 16, V_ROW = 2 * 64 + 16;  // bytes
     uint8_t k[64 * K_ROW];  // [key][channel]
-    uint8_t v[D * V_ROW];   // [channel][key]
+    uint8_t v[D * V_ROW];   // [channel][key], the even channels before the odd ones
     float ks[64], vs[64];
     int32_t held[4];        // the group of 16 keys is in the cache
 };
@@ -671,8 +677,9 @@ __global__ __launch_bounds__(64 * MANY_WAVES, (many_waves<T, D>())) void k_atten
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[ct][i] = 0.0f;
 
-    // A step's codes: unit u = (key, 32 channels) of K and (16 keys, channel pair)
-    // of V, both of the step's group of 16 keys u / (D / 2).
+    // A step's codes: unit u = (32 channels, key) of K and (16 keys, channel pair)
+    // of V, both of the step's group of 16 keys u / (D / 2); consecutive threads
+    // write consecutive rows of LDS, whose padding spreads them over the banks.
     uint4 kw[UN], vw[UN];
     float scale = 0.0f;
     int32_t held = 0;
@@ -689,9 +696,9 @@ __global__ __launch_bounds__(64 * MANY_WAVES, (many_waves<T, D>())) void k_atten
             const int u = tid + 256 * j;
             if (D < 128 && u >= 2 * D) break;
             bool in;
-            const int64_t at = place(key, u / (D / 2), in) * (8 * D) + (u % (D / 2)) * 16;
-            kw[j] = *reinterpret_cast<const uint4 *>(cache.k + at);
-            vw[j] = *reinterpret_cast<const uint4 *>(cache.v + at);
+            const int64_t at = place(key, u / (D / 2), in) * (8 * D);
+            kw[j] = *reinterpret_cast<const uint4 *>(cache.k + at + (u % 16) * (D / 2) + (u % (D / 2)) / 16 * 16);
+            vw[j] = *reinterpret_cast<const uint4 *>(cache.v + at + (u % (D / 2)) * 16);
         }
         if (tid < 128) {
             bool in;
@@ -705,7 +712,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, (many_waves<T, D>())) void k_atten
         for (int j = 0; j < UN; ++j) {
             const int u = tid + 256 * j;
             if (D < 128 && u >= 2 * D) break;
-            u32x4 *kd = reinterpret_cast<u32x4 *>(b.k + (u / (D / 32)) * Lds::K_ROW + (u % (D / 32)) * 64);
+            u32x4 *kd = reinterpret_cast<u32x4 *>(b.k + (u / (D / 2) * 16 + u % 16) * Lds::K_ROW + (u % (D / 2)) / 16 * 64);
             kd[0] = codes8(kw[j].x);
             kd[1] = codes8(kw[j].y);
             kd[2] = codes8(kw[j].z);
@@ -715,11 +722,11 @@ __global__ __launch_bounds__(64 * MANY_WAVES, (many_waves<T, D>())) void k_atten
             codes_by_channel(vw[j].y, e[1], d[1]);
             codes_by_channel(vw[j].z, e[2], d[2]);
             codes_by_channel(vw[j].w, e[3], d[3]);
-            uint8_t *vd = b.v + 2 * (u % (D / 2)) * Lds::V_ROW + (u / (D / 2)) * 32;
+            uint8_t *vd = b.v + (u % (D / 2)) * Lds::V_ROW + (u / (D / 2)) * 32;
             *reinterpret_cast<u32x4 *>(vd) = (u32x4){e[0][0], e[0][1], e[2][0], e[2][1]};
             *reinterpret_cast<u32x4 *>(vd + 16) = (u32x4){e[1][0], e[1][1], e[3][0], e[3][1]};
-            *reinterpret_cast<u32x4 *>(vd + Lds::V_ROW) = (u32x4){d[0][0], d[0][1], d[2][0], d[2][1]};
-            *reinterpret_cast<u32x4 *>(vd + Lds::V_ROW + 16) = (u32x4){d[1][0], d[1][1], d[3][0], d[3][1]};
+            *reinterpret_cast<u32x4 *>(vd + D / 2 * Lds::V_ROW) = (u32x4){d[0][0], d[0][1], d[2][0], d[2][1]};
+            *reinterpret_cast<u32x4 *>(vd + D / 2 * Lds::V_ROW + 16) = (u32x4){d[1][0], d[1][1], d[3][0], d[3][1]};
         }
         if (tid < 128) (tid < 64 ? b.ks : b.vs)[tid & 63] = scale;
         if (tid < 64 && (tid & 15) == 0) b.held[tid >> 4] = held;
@@ -761,17 +768,18 @@ __global__ __launch_bounds__(64 * MANY_WAVES, (many_waves<T, D>())) void k_atten
                 v[4 * y + 2] = sc[y >> 2][4 * (y & 3) + 2] * f.z;
                 v[4 * y + 3] = sc[y >> 2][4 * (y & 3) + 3] * f.w;
             }
-            if (!whole) {
-                const int32_t from = begin - key - 4 * hf, to = end - key - 4 * hf;
-                const int32_t there[4] = {in.x, in.y, in.z, in.w};
+            const int32_t there[4] = {in.x, in.y, in.z, in.w};
+            // v[j] (j: 16 x + 4 a + b) where this row sees the key, else `other`
+            auto hide = [&](float other) {
+                int32_t from = begin - key - 4 * hf, to = end - key - 4 * hf;
+                stay_branch(from, to);
 #pragma unroll
-                for (int y = 0; y < 8; ++y)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int32_t j = 8 * y + i;
-                        v[4 * y + i] = j >= from && j < to && there[y >> 1] ? v[4 * y + i] : -INFINITY;
-                    }
-            }
+                for (int j = 0; j < 32; ++j) {
+                    const int32_t k = 8 * (j >> 2) + (j & 3);
+                    v[j] = k >= from && k < to && there[j >> 3] != 0 ? v[j] : other;
+                }
+            };
+            if (!whole) hide(-INFINITY);
             float top = v[0];
 #pragma unroll
             for (int j = 1; j < 32; ++j) top = fmaxf(top, v[j]);
@@ -795,11 +803,11 @@ __global__ __launch_bounds__(64 * MANY_WAVES, (many_waves<T, D>())) void k_atten
                 for (int i = 0; i < 4; ++i) {
                     const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(v[4 * y + i], pl.c, -ref));
                     sum += e;
-                    // a key that this row does not see may hold anything
-                    v[4 * y + i] = !whole && v[4 * y + i] == -INFINITY ? 0.0f : e * fs[i];
+                    v[4 * y + i] = e * fs[i];
                 }
             }
             l += sum;
+            if (!whole) hide(0.0f);  // a key that this row does not see may hold anything
 #pragma unroll
             for (int s = 0; s < 4; ++s) {  // 16 keys
                 u32x4 p[PP];
@@ -822,22 +830,21 @@ __global__ __launch_bounds__(64 * MANY_WAVES, (many_waves<T, D>())) void k_atten
     }
     l += __shfl_xor(l, 32, 64);
 
-    // lane: row r32, channels 32 ct + 8 a + 4 hf + 0 .. 3
+    // lane: row r32; result 4 a + b of tile ct is row 32 ct + 8 a + 4 hf + b of V's
+    // channels in LDS, even ones in the first half of the tiles
     const int64_t token = q0 + my_i, qh = h * group + (row - my_i * group);
     if (first + r32 >= n_rows || token >= a.tokens) return;
-    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    const float inv = pl.splits > 1 ? 1.0f : l != 0.0f ? 1.0f / l : 0.0f;
     const int64_t slot = (token * a.q_heads + qh) * pl.splits + split;
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct)
+    for (int ct = 0; ct < CT / 2; ++ct)
 #pragma unroll
-        for (int y = 0; y < 4; ++y) {
-            const int ch = 32 * ct + 8 * y + 4 * hf;
+        for (int y = 0; y < 8; ++y) {
+            const int i = 4 * (y >> 1) + 2 * (y & 1), ch = 2 * (32 * ct + 8 * (y >> 1) + 4 * hf) + 4 * (y & 1);
+            const float x[4] = {o[ct][i] * inv, o[ct + CT / 2][i] * inv, o[ct][i + 1] * inv, o[ct + CT / 2][i + 1] * inv};
             if (pl.splits > 1) {
-                if (l != 0.0f)
-                    *reinterpret_cast<float4 *>(pl.part_o + slot * D + ch) =
-                        make_float4(o[ct][4 * y], o[ct][4 * y + 1], o[ct][4 * y + 2], o[ct][4 * y + 3]);
+                if (l != 0.0f) *reinterpret_cast<float4 *>(pl.part_o + slot * D + ch) = make_float4(x[0], x[1], x[2], x[3]);
             } else {
-                const float x[4] = {o[ct][4 * y] * inv, o[ct][4 * y + 1] * inv, o[ct][4 * y + 2] * inv, o[ct][4 * y + 3] * inv};
                 store4<T>((T *)a.out + token * a.out_token_stride + qh * a.out_head_stride + ch, x, pl.out_packed);
             }
         }
