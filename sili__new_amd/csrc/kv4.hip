@@ -680,31 +680,38 @@ __global__ __launch_bounds__(64 * MANY_WAVES, (many_waves<T, D>())) void k_atten
     // A step's codes: unit u = (32 channels, key) of K and (16 keys, channel pair)
     // of V, both of the step's group of 16 keys u / (D / 2); consecutive threads
     // write consecutive rows of LDS, whose padding spreads them over the banks.
+    // Their pages are asked for a step before them.
     uint4 kw[UN], vw[UN];
     float scale = 0.0f;
-    int32_t held = 0;
-    auto place = [&](int32_t key, int sub, bool &in) -> int64_t {  // group `sub` of the step at `key`, in groups of 16 keys
+    int32_t held = 0, page[UN], scale_page = -1;
+    const int scale_group = (tid & 63) >> 4;
+    auto entry = [&](int32_t key, int sub) {  // of group `sub` of 16 keys
         const int32_t mine = (key >> 4) + sub;
-        const int32_t pi = pl.page_shift >= 0 ? mine >> pl.page_shift : mine / pl.groups_per_page;
-        const int32_t page = 16 * mine < kr.cap ? table[pi] : -1;
-        in = page >= 0 && page < pl.n_pages;
-        return in ? (int64_t)(page * H + h) * pl.groups_per_page + (mine - pi * pl.groups_per_page) : (int64_t)h * pl.groups_per_page;
+        return 16 * mine < kr.cap ? table[pl.page_shift >= 0 ? mine >> pl.page_shift : mine / pl.groups_per_page] : -1;
+    };
+    auto find = [&](int32_t key) {
+#pragma unroll
+        for (int j = 0; j < UN; ++j) page[j] = entry(key, min((tid + 256 * j) / (D / 2), 3));
+        scale_page = entry(key, scale_group);
+    };
+    // where the group lies, in groups of 16 keys; of a page outside the cache: some place in it
+    auto place = [&](int32_t pg, int32_t key, int sub) -> int64_t {
+        const int32_t mine = (key >> 4) + sub;
+        const int32_t in_page = pl.page_shift >= 0 ? mine & (pl.groups_per_page - 1) : mine % pl.groups_per_page;
+        return (int64_t)((pg >= 0 && pg < pl.n_pages ? pg : 0) * H + h) * pl.groups_per_page + in_page;
     };
     auto fetch = [&](int32_t key) {
 #pragma unroll
         for (int j = 0; j < UN; ++j) {
             const int u = tid + 256 * j;
             if (D < 128 && u >= 2 * D) break;
-            bool in;
-            const int64_t at = place(key, u / (D / 2), in) * (8 * D);
+            const int64_t at = place(page[j], key, u / (D / 2)) * (8 * D);
             kw[j] = *reinterpret_cast<const uint4 *>(cache.k + at + (u % 16) * (D / 2) + (u % (D / 2)) / 16 * 16);
             vw[j] = *reinterpret_cast<const uint4 *>(cache.v + at + (u % (D / 2)) * 16);
         }
         if (tid < 128) {
-            bool in;
-            const int64_t at = place(key, (tid & 63) >> 4, in) * 16 + (tid & 15);
-            scale = (tid < 64 ? cache.k_scale : cache.v_scale)[at];
-            held = in;
+            scale = (tid < 64 ? cache.k_scale : cache.v_scale)[place(scale_page, key, scale_group) * 16 + (tid & 15)];
+            held = scale_page >= 0 && scale_page < pl.n_pages;
         }
     };
     auto unpack = [&](Lds &b) {
@@ -733,7 +740,9 @@ __global__ __launch_bounds__(64 * MANY_WAVES, (many_waves<T, D>())) void k_atten
     };
 
     if (c0 < c1) {
+        find(c0);
         fetch(c0);
+        find(c0 + 64);
         unpack(lds[0]);
     }
     int buf = 0;
@@ -741,21 +750,35 @@ __global__ __launch_bounds__(64 * MANY_WAVES, (many_waves<T, D>())) void k_atten
         __syncthreads();
         const Lds &b = lds[buf];
         const bool more = key + 64 < c1;
-        if (more) fetch(key + 64);
+        if (more) {
+            fetch(key + 64);
+            find(key + 128);
+        }
         if (key < w_end && key + 64 > w_begin) {
             f32x16 sc[2];
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sc[x][i] = 0.0f;
+            // K's operands, AHEAD steps of 16 channels before their products: the
+            // compiler left to itself waits for each read of LDS
+            constexpr int AHEAD = 2;
+            u32x4 kk[KS][2];
 #pragma unroll
-            for (int s = 0; s < KS; ++s)
+            for (int s = 0; s < KS + AHEAD; ++s) {
+                if (s < KS) {
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const u32x4 kk = *reinterpret_cast<const u32x4 *>(b.k + (32 * x + r32) * Lds::K_ROW + 32 * s + 16 * hf);
-#pragma unroll
-                    for (int k = 0; k < QP; ++k) sc[x] = mma(kk, q[s][k], sc[x]);
+                    for (int x = 0; x < 2; ++x)
+                        kk[s][x] = *reinterpret_cast<const u32x4 *>(b.k + (32 * x + r32) * Lds::K_ROW + 32 * s + 16 * hf);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
+                if (s >= AHEAD) {
+#pragma unroll
+                    for (int k = 0; k < QP; ++k)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) sc[x] = mma(kk[s - AHEAD][x], q[s - AHEAD][k], sc[x]);
+                }
+            }
             // wave-uniform: every row sees every key of the step
             const int4 in = *reinterpret_cast<const int4 *>(b.held);
             const bool whole = key >= all_begin && key + 64 <= all_end && uniform(in.x & in.y & in.z & in.w) != 0;
