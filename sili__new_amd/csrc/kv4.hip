@@ -197,11 +197,9 @@ __device__ __forceinline__ float lanes_sum(float v) {
 // bf16 parts of q: 24 bits of fp32, all 11 of f16, all 8 of bf16.
 template <typename T>
 constexpr int q_parts() { return sizeof(T) == 4 ? 3 : __is_same(T, __bf16) ? 1 : 2; }
-// ... of p: 24 bits for fp32, 16 for f16.  bf16 takes two where memory bounds the
-// kernel (FEW rows), one where the matrix cores' time counts: its rounding is as
-// large as the output's own, together 1.4 times that.
-template <typename T, bool FEW>
-constexpr int p_parts() { return sizeof(T) == 4 ? 3 : __is_same(T, __bf16) && !FEW ? 1 : 2; }
+// ... of p: 24 bits for fp32, 16 for f16 and bf16.
+template <typename T>
+constexpr int p_parts() { return sizeof(T) == 4 ? 3 : 2; }
 // x, y in N parts: part k the bf16 nearest to what the parts before leave.
 template <int N>
 __device__ __forceinline__ void split_bf16(float x, float y, uint32_t (&part)[N]) {
@@ -241,7 +239,7 @@ struct AttendPlan {
     int32_t waves;            // of a block whose waves share rows
     int32_t join_rows;        // rows such a block joins at most
     int32_t columns;          // columns a row takes
-    int32_t few, many;        // takes requests of more than `few` rows, up to `many`
+    int32_t many;             // the most rows of a request for the few-rows kernel; more: the other
     float c;                  // |scale| log2(e)
     bool negative;            // scale < 0: the sign goes to q
     float *part_o;            // [tokens * q_heads][splits][D], unnormalised
@@ -282,10 +280,6 @@ constexpr int waves_per_simd() {
     return (D == 64 ? 4 : D == 128 ? 3 : 2) - (lean ? 0 : 1);
 }
 
-// ... of the many-rows kernel.
-template <typename T, int D>
-constexpr int many_waves() { return __is_same(T, __bf16) && D <= 128 ? 2 : 1; }
-
 // Few rows: a tile of 16 a block, whose waves take a step of keys each in turn and
 // are joined in LDS; every byte of the cache goes from memory to one wave's
 // registers, a step ahead.  Memory bounds it (8 kv heads of 5.1 K keys a request,
@@ -302,7 +296,7 @@ constexpr int many_waves() { return __is_same(T, __bf16) && D <= 128 ? 2 : 1; }
 // own part of them; the outputs are summed once, at the end.
 template <typename T, int D, int WAVES, int CP>
 __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_attend_few(sili_kv4_attend_args a, AttendPlan pl) {
-    constexpr int QP = q_parts<T>(), PP = p_parts<T, true>();
+    constexpr int QP = q_parts<T>(), PP = p_parts<T>();
     constexpr int KS = D / 32;   // steps of 32 channels
     constexpr int CT = D / 32;   // blocks of 32 output channels
     constexpr int RT = 16 / CP;  // rows of a tile
@@ -331,8 +325,7 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_at
     const int32_t kv = a.kv_lens[req];
     const int32_t n_rows = n * group;
     const int32_t first = tile * RT;
-    if (q0 < 0 || n_rows <= pl.few || n_rows > pl.many) return;
-    if (first >= n_rows) return;
+    if (q0 < 0 || n_rows > pl.many || first >= n_rows) return;
     KeyRange kr;
     kr.base = kv - n_all;
     kr.window = (int32_t)a.window;
@@ -605,11 +598,17 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_at
 // 32 x + 8 a + 4 hf + b (a, b < 4; hf = lane / 32), so V's keys lie in LDS in the
 // order 0-3, 8-11, 4-7, 12-15 of every 16: eight at 16 s + 8 hf are the lane's
 // own.  Rows of LDS are padded by 16 bytes, which spreads eight lanes' 16 bytes
-// over all banks.
+// over all banks.  A weight enters in one bf16 part: its rounding is as large as
+// the output's own, together 1.4 times that, and a second part would be half as
+// many products again.  Issue bounds it (2 x 2047 tokens of 40 heads under a window
+// of 4096: 520 us, the vector units busy 45 % of the time, the matrix cores 31 %,
+// with a last round of blocks that fills a quarter of the GPU).
 constexpr int MANY_WAVES = 4, MANY_ROWS = 32 * MANY_WAVES;
 
-template <int D>
+constexpr int MANY_D = 128;
+
 struct ManyLds {
+    static constexpr int D = MANY_D;
     static constexpr int K_ROW = 2 * D + 16, V_ROW = 2 * 64 + 16;  // bytes
     uint8_t k[64 * K_ROW];  // [key][channel]
     uint8_t v[D * V_ROW];   // [channel][key], the even channels before the odd ones
@@ -617,32 +616,29 @@ struct ManyLds {
     int32_t held[4];        // the group of 16 keys is in the cache
 };
 
-template <typename T, int D>
-__global__ __launch_bounds__(64 * MANY_WAVES, (many_waves<T, D>())) void k_attend_many(sili_kv4_attend_args a, AttendPlan pl) {
-    constexpr int QP = q_parts<T>(), PP = p_parts<T, false>();
-    constexpr int KS = D / 16, CT = D / 32;
-    constexpr int UN = D <= 128 ? 1 : D / 128;  // 16-byte units of K, and of V, a thread turns
-    using Lds = ManyLds<D>;
+__global__ __launch_bounds__(64 * MANY_WAVES, 2) void k_attend_many(sili_kv4_attend_args a, AttendPlan pl) {
+    using T = __bf16;
+    constexpr int D = MANY_D, KS = D / 16, CT = D / 32;
+    using Lds = ManyLds;
     extern __shared__ __align__(16) uint8_t s_many[];
     Lds *lds = reinterpret_cast<Lds *>(s_many);
     const sili_kv4_cache &cache = a.cache;
     const int tid = threadIdx.x, wave = (int)uniform(tid >> 6), lane = tid & 63, hf = lane >> 5, r32 = lane & 31;
     const int H = pl.kv_heads, group = pl.group;
-    const int h = blockIdx.x % H, tile = blockIdx.x / H, split = blockIdx.y, req = blockIdx.z;
+    const int h = blockIdx.x % H, tile = blockIdx.x / H, req = blockIdx.z;
     const int32_t *table = a.block_table + (int64_t)req * a.table_width;
     const int32_t q0 = a.q_start[req];
     const int32_t n_all = a.q_start[req + 1] - q0, n = min(n_all, (int32_t)a.max_new);
     const int32_t kv = a.kv_lens[req];
     const int32_t n_rows = n * group;
     const int32_t block_first = tile * MANY_ROWS;
-    if (q0 < 0 || n_rows <= pl.few || n_rows > pl.many || block_first >= n_rows) return;
+    if (q0 < 0 || n_rows <= pl.many || block_first >= n_rows) return;
     KeyRange kr;
     kr.base = kv - n_all;
     kr.window = (int32_t)a.window;
     kr.causal = a.causal != 0;
     kr.cap = min(kv, pl.most);
-    const int32_t lo = kr.begin(token_of(pl, block_first)) & ~63, hi = kr.end(token_of(pl, min(block_first + MANY_ROWS, n_rows) - 1));
-    const int32_t c0 = lo + split * pl.chunk, c1 = min(hi, c0 + pl.chunk);
+    const int32_t c0 = kr.begin(token_of(pl, block_first)) & ~63, c1 = kr.end(token_of(pl, min(block_first + MANY_ROWS, n_rows) - 1));
 
     // this wave's rows (past the last: the last again), and this lane's
     const int32_t first = block_first + 32 * wave, row = min(first + r32, n_rows - 1), my_i = token_of(pl, row);
@@ -651,7 +647,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, (many_waves<T, D>())) void k_atten
     const int32_t w_begin = kr.begin(i_first), w_end = first < n_rows ? kr.end(i_last) : 0;  // what any row sees
     const int32_t all_end = kr.end(i_first), all_begin = kr.begin(i_last);                   // what every row sees
 
-    u32x4 q[KS][QP];  // channels 16 s + 8 hf + 0 .. 7
+    u32x4 q[KS];  // channels 16 s + 8 hf + 0 .. 7
     {
         const int64_t token = q0 + my_i;
         const T *src = (const T *)a.q + (token < a.tokens ? token * a.q_token_stride : 0) +
@@ -661,12 +657,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, (many_waves<T, D>())) void k_atten
             float x[8];
             load8<T>(src + 16 * s, pl.q_packed, x);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t part[QP];
-                split_bf16<QP>(pl.negative ? -x[2 * j] : x[2 * j], pl.negative ? -x[2 * j + 1] : x[2 * j + 1], part);
-#pragma unroll
-                for (int k = 0; k < QP; ++k) q[s][k][j] = part[k];
-            }
+            for (int j = 0; j < 4; ++j) q[s][j] = pl.negative ? pack_bf16(-x[2 * j], -x[2 * j + 1]) : pack_bf16(x[2 * j], x[2 * j + 1]);
         }
     }
 
@@ -677,21 +668,19 @@ __global__ __launch_bounds__(64 * MANY_WAVES, (many_waves<T, D>())) void k_atten
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[ct][i] = 0.0f;
 
-    // A step's codes: unit u = (32 channels, key) of K and (16 keys, channel pair)
-    // of V, both of the step's group of 16 keys u / (D / 2); consecutive threads
-    // write consecutive rows of LDS, whose padding spreads them over the banks.
-    // Their pages are asked for a step before them.
-    uint4 kw[UN], vw[UN];
+    // A step's codes: a thread turns 32 channels of a key, and 16 keys of a channel
+    // pair, of the step's group of 16 keys tid / 64; consecutive threads write
+    // consecutive rows of LDS.  Their pages are asked for a step before them.
+    uint4 kw, vw;
     float scale = 0.0f;
-    int32_t held = 0, page[UN], scale_page = -1;
+    int32_t held = 0, page = -1, scale_page = -1;
     const int scale_group = (tid & 63) >> 4;
     auto entry = [&](int32_t key, int sub) {  // of group `sub` of 16 keys
         const int32_t mine = (key >> 4) + sub;
         return 16 * mine < kr.cap ? table[pl.page_shift >= 0 ? mine >> pl.page_shift : mine / pl.groups_per_page] : -1;
     };
     auto find = [&](int32_t key) {
-#pragma unroll
-        for (int j = 0; j < UN; ++j) page[j] = entry(key, min((tid + 256 * j) / (D / 2), 3));
+        page = entry(key, wave);
         scale_page = entry(key, scale_group);
     };
     // where the group lies, in groups of 16 keys; of a page outside the cache: some place in it
@@ -701,40 +690,30 @@ __global__ __launch_bounds__(64 * MANY_WAVES, (many_waves<T, D>())) void k_atten
         return (int64_t)((pg >= 0 && pg < pl.n_pages ? pg : 0) * H + h) * pl.groups_per_page + in_page;
     };
     auto fetch = [&](int32_t key) {
-#pragma unroll
-        for (int j = 0; j < UN; ++j) {
-            const int u = tid + 256 * j;
-            if (D < 128 && u >= 2 * D) break;
-            const int64_t at = place(page[j], key, u / (D / 2)) * (8 * D);
-            kw[j] = *reinterpret_cast<const uint4 *>(cache.k + at + (u % 16) * (D / 2) + (u % (D / 2)) / 16 * 16);
-            vw[j] = *reinterpret_cast<const uint4 *>(cache.v + at + (u % (D / 2)) * 16);
-        }
+        const int64_t at = place(page, key, wave) * (8 * D);
+        kw = *reinterpret_cast<const uint4 *>(cache.k + at + (lane % 16) * (D / 2) + lane / 16 * 16);
+        vw = *reinterpret_cast<const uint4 *>(cache.v + at + lane * 16);
         if (tid < 128) {
             scale = (tid < 64 ? cache.k_scale : cache.v_scale)[place(scale_page, key, scale_group) * 16 + (tid & 15)];
             held = scale_page >= 0 && scale_page < pl.n_pages;
         }
     };
     auto unpack = [&](Lds &b) {
-#pragma unroll
-        for (int j = 0; j < UN; ++j) {
-            const int u = tid + 256 * j;
-            if (D < 128 && u >= 2 * D) break;
-            u32x4 *kd = reinterpret_cast<u32x4 *>(b.k + (u / (D / 2) * 16 + u % 16) * Lds::K_ROW + (u % (D / 2)) / 16 * 64);
-            kd[0] = codes8(kw[j].x);
-            kd[1] = codes8(kw[j].y);
-            kd[2] = codes8(kw[j].z);
-            kd[3] = codes8(kw[j].w);
-            uint32_t e[4][2], d[4][2];
-            codes_by_channel(vw[j].x, e[0], d[0]);
-            codes_by_channel(vw[j].y, e[1], d[1]);
-            codes_by_channel(vw[j].z, e[2], d[2]);
-            codes_by_channel(vw[j].w, e[3], d[3]);
-            uint8_t *vd = b.v + (u % (D / 2)) * Lds::V_ROW + (u / (D / 2)) * 32;
-            *reinterpret_cast<u32x4 *>(vd) = (u32x4){e[0][0], e[0][1], e[2][0], e[2][1]};
-            *reinterpret_cast<u32x4 *>(vd + 16) = (u32x4){e[1][0], e[1][1], e[3][0], e[3][1]};
-            *reinterpret_cast<u32x4 *>(vd + D / 2 * Lds::V_ROW) = (u32x4){d[0][0], d[0][1], d[2][0], d[2][1]};
-            *reinterpret_cast<u32x4 *>(vd + D / 2 * Lds::V_ROW + 16) = (u32x4){d[1][0], d[1][1], d[3][0], d[3][1]};
-        }
+        u32x4 *kd = reinterpret_cast<u32x4 *>(b.k + (16 * wave + lane % 16) * Lds::K_ROW + lane / 16 * 64);
+        kd[0] = codes8(kw.x);
+        kd[1] = codes8(kw.y);
+        kd[2] = codes8(kw.z);
+        kd[3] = codes8(kw.w);
+        uint32_t e[4][2], d[4][2];
+        codes_by_channel(vw.x, e[0], d[0]);
+        codes_by_channel(vw.y, e[1], d[1]);
+        codes_by_channel(vw.z, e[2], d[2]);
+        codes_by_channel(vw.w, e[3], d[3]);
+        uint8_t *vd = b.v + lane * Lds::V_ROW + wave * 32;
+        *reinterpret_cast<u32x4 *>(vd) = (u32x4){e[0][0], e[0][1], e[2][0], e[2][1]};
+        *reinterpret_cast<u32x4 *>(vd + 16) = (u32x4){e[1][0], e[1][1], e[3][0], e[3][1]};
+        *reinterpret_cast<u32x4 *>(vd + D / 2 * Lds::V_ROW) = (u32x4){d[0][0], d[0][1], d[2][0], d[2][1]};
+        *reinterpret_cast<u32x4 *>(vd + D / 2 * Lds::V_ROW + 16) = (u32x4){d[1][0], d[1][1], d[3][0], d[3][1]};
         if (tid < 128) (tid < 64 ? b.ks : b.vs)[tid & 63] = scale;
         if (tid < 64 && (tid & 15) == 0) b.held[tid >> 4] = held;
     };
@@ -774,9 +753,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, (many_waves<T, D>())) void k_atten
                 }
                 if (s >= AHEAD) {
 #pragma unroll
-                    for (int k = 0; k < QP; ++k)
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) sc[x] = mma(kk[s - AHEAD][x], q[s - AHEAD][k], sc[x]);
+                    for (int x = 0; x < 2; ++x) sc[x] = mma(kk[s - AHEAD][x], q[s - AHEAD], sc[x]);
                 }
             }
             // wave-uniform: every row sees every key of the step
@@ -833,19 +810,13 @@ __global__ __launch_bounds__(64 * MANY_WAVES, (many_waves<T, D>())) void k_atten
             if (!whole) hide(0.0f);  // a key that this row does not see may hold anything
 #pragma unroll
             for (int s = 0; s < 4; ++s) {  // 16 keys
-                u32x4 p[PP];
+                u32x4 p;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint32_t part[PP];
-                    split_bf16<PP>(v[8 * s + 2 * j], v[8 * s + 2 * j + 1], part);
-#pragma unroll
-                    for (int k = 0; k < PP; ++k) p[k][j] = part[k];
-                }
+                for (int j = 0; j < 4; ++j) p[j] = pack_bf16(v[8 * s + 2 * j], v[8 * s + 2 * j + 1]);
 #pragma unroll
                 for (int ct = 0; ct < CT; ++ct) {
                     const u32x4 vv = *reinterpret_cast<const u32x4 *>(b.v + (32 * ct + r32) * Lds::V_ROW + 32 * s + 16 * hf);
-#pragma unroll
-                    for (int k = 0; k < PP; ++k) o[ct] = mma(vv, p[k], o[ct]);
+                    o[ct] = mma(vv, p, o[ct]);
                 }
             }
         }
@@ -857,24 +828,17 @@ __global__ __launch_bounds__(64 * MANY_WAVES, (many_waves<T, D>())) void k_atten
     // channels in LDS, even ones in the first half of the tiles
     const int64_t token = q0 + my_i, qh = h * group + (row - my_i * group);
     if (first + r32 >= n_rows || token >= a.tokens) return;
-    const float inv = pl.splits > 1 ? 1.0f : l != 0.0f ? 1.0f / l : 0.0f;
-    const int64_t slot = (token * a.q_heads + qh) * pl.splits + split;
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    T *out = (T *)a.out + token * a.out_token_stride + qh * a.out_head_stride;
 #pragma unroll
     for (int ct = 0; ct < CT / 2; ++ct)
 #pragma unroll
         for (int y = 0; y < 8; ++y) {
             const int i = 4 * (y >> 1) + 2 * (y & 1), ch = 2 * (32 * ct + 8 * (y >> 1) + 4 * hf) + 4 * (y & 1);
             const float x[4] = {o[ct][i] * inv, o[ct + CT / 2][i] * inv, o[ct][i + 1] * inv, o[ct + CT / 2][i + 1] * inv};
-            if (pl.splits > 1) {
-                if (l != 0.0f) *reinterpret_cast<float4 *>(pl.part_o + slot * D + ch) = make_float4(x[0], x[1], x[2], x[3]);
-            } else {
-                store4<T>((T *)a.out + token * a.out_token_stride + qh * a.out_head_stride + ch, x, pl.out_packed);
-            }
+            store4<T>(out + ch, x, pl.out_packed);
         }
-    if (hf == 0) {
-        if (pl.splits > 1) pl.part_ml[slot] = make_float2(m, l);
-        else if (a.lse) a.lse[token * a.q_heads + qh] = l != 0.0f ? (m + __builtin_amdgcn_logf(l)) * 0.69314718f : -INFINITY;
-    }
+    if (a.lse && hf == 0) a.lse[token * a.q_heads + qh] = l != 0.0f ? (m + __builtin_amdgcn_logf(l)) * 0.69314718f : -INFINITY;
 }
 
 // Joins the splits of a row: a block a (row, kv head, request); D / 4 threads
@@ -888,7 +852,7 @@ __global__ __launch_bounds__(256) void k_attend_join(sili_kv4_attend_args a, Att
     const int32_t row = blockIdx.x, h = blockIdx.y, req = blockIdx.z;
     const int32_t group = pl.group;
     const int32_t q0 = a.q_start[req], n_rows = min(a.q_start[req + 1] - q0, (int32_t)a.max_new) * group;
-    if (q0 < 0 || n_rows <= pl.few || n_rows > pl.many || row >= n_rows) return;
+    if (q0 < 0 || n_rows > pl.many || row >= n_rows) return;
     const int32_t i = token_of(pl, row);
     const int64_t token = q0 + i, qh = h * group + (row - i * group);
     if (token >= a.tokens) return;
@@ -997,16 +961,6 @@ void kv4_read(const sili_kv4_rows_args &a, hipStream_t st) { rows<false>(a, st, 
 
 namespace {
 
-// Requests of up to FEW_ROWS rows have their keys shared by a block's waves, a
-// row tile of 16 each; larger ones give each wave rows of its own.
-constexpr int32_t FEW_ROWS = 64;
-
-struct Launch {
-    bool on = false;
-    int64_t tiles = 0;  // row tiles of a (request, kv head)
-    AttendPlan plan{};
-};
-
 // Waves of a CU that run the few-rows kernel at once.
 int waves_of(int dtype, int64_t head_dim, int columns) {
     int n = 0;
@@ -1022,104 +976,98 @@ int waves_of(int dtype, int64_t head_dim, int columns) {
     return n;
 }
 
-// The two launches of a call (few rows, many rows).
-void plan_attend(const sili_kv4_attend_args &a, Launch (&out)[2]) {
-    const int64_t group = a.q_heads / a.cache.kv_heads, rows = a.max_new * group;
-    const int64_t gpp = a.cache.page_size / 16;
-    for (int k = 0; k < 2; ++k) {
-        Launch &L = out[k];
-        AttendPlan &p = L.plan;
-        p.kv_heads = (int32_t)a.cache.kv_heads;
-        p.group = (int32_t)group;
-        p.group_inv = group == 1 ? ~0u : (uint32_t)((uint64_t(1) << 32) / (uint64_t)group);
-        p.n_pages = (int32_t)a.cache.n_pages;
-        p.most = p.n_pages == 0 ? 0 : (int32_t)std::min({a.max_len, a.table_width * a.cache.page_size, int64_t(INT32_MAX) - (1 << 20)});
-        const int64_t es = dtype_size(a.dtype);
-        p.q_packed = aligned(a.q, (size_t)(8 * es)) && a.q_token_stride % 8 == 0 && a.q_head_stride % 8 == 0;
-        p.out_packed = aligned(a.out, (size_t)(4 * es)) && a.out_token_stride % 4 == 0 && a.out_head_stride % 4 == 0;
-        p.groups_per_page = (int32_t)gpp;
-        p.page_shift = (gpp & (gpp - 1)) == 0 ? (int32_t)__builtin_ctzll((unsigned long long)gpp) : -1;
-        // a scale of zero leaves all scores equal; c > 0 keeps hidden ones at -inf
-        p.c = std::max(std::fabs(a.scale) * 1.44269504f, 0x1p-100f);
-        p.negative = a.scale < 0.0f;
-        p.few = k == 0 ? 0 : FEW_ROWS;
-        p.many = k == 0 ? FEW_ROWS : INT32_MAX;
-        L.on = k == 0 || rows > FEW_ROWS;
-        const int parts = a.dtype == SILI_F32 ? 4 : 2;
-        p.columns = k == 0 && rows <= 16 / parts ? parts : 1;
-        const int64_t tile_rows = k == 0 ? 16 / p.columns : MANY_ROWS;
-        L.tiles = (std::min<int64_t>(rows, p.many) + tile_rows - 1) / tile_rows;
-        p.join_rows = (int32_t)std::min<int64_t>(16, rows);
-        // keys a row tile can reach: its rows' windows, aligned to 64
-        int64_t reach = a.max_len;
-        if (a.window > 0) reach = std::min(reach, a.window + (tile_rows - 1) / group + 1 + 63);
-        const int64_t blocks = std::max<int64_t>(1, a.requests * a.cache.kv_heads * L.tiles);
-        // few blocks: as many waves in one as a CU holds, so that fewer splits
-        // are left to join (40 heads of 131071 keys, 8 blocks a split: 31 + 5
-        // us against 31 + 7 with 4 waves; 320 blocks of 2048 keys: 24 us
-        // against 22.6, a second round of blocks)
-        const int wide = waves_of(a.dtype, a.cache.head_dim, p.columns);
-        p.waves = blocks <= 128 ? wide : 4;
-        const int64_t step = k == 0 ? 64 * p.waves : 64;
-        // splits until every CU has a wave on each SIMD as often as registers
-        // allow; fp32, which the vector units bound, twice at most (320 blocks
-        // of 2048 keys: 22.7 us, with a second split 21.4 + 4.7 to join)
-        const int64_t fill = k == 0 ? 256 * std::max(1, std::min(wide, a.dtype == SILI_F32 ? 8 : wide) / p.waves) : 512;
-        const int64_t want = std::clamp<int64_t>(fill / blocks, 1, std::max<int64_t>(1, (reach + 255) / 256));
-        p.chunk = (int32_t)std::max<int64_t>(step, ((reach + want - 1) / want + step - 1) / step * step);
-        p.splits = (int32_t)std::max<int64_t>(1, (reach + p.chunk - 1) / p.chunk);
-        if (!L.on) p.splits = 1;
-    }
+// How a call is launched: requests of up to plan.many rows go to the few-rows
+// kernel, `tiles` row tiles a (request, kv head), those of more to the other.
+struct Launch {
+    int64_t tiles = 0, many_tiles = 0;
+    AttendPlan plan{};
+};
+
+Launch plan_attend(const sili_kv4_attend_args &a) {
+    Launch L;
+    AttendPlan &p = L.plan;
+    const int64_t group = a.q_heads / a.cache.kv_heads, rows = a.max_new * group, heads = a.requests * a.cache.kv_heads;
+    const int64_t gpp = a.cache.page_size / 16, es = dtype_size(a.dtype);
+    p.kv_heads = (int32_t)a.cache.kv_heads;
+    p.group = (int32_t)group;
+    p.group_inv = group == 1 ? ~0u : (uint32_t)((uint64_t(1) << 32) / (uint64_t)group);
+    p.n_pages = (int32_t)a.cache.n_pages;
+    p.most = p.n_pages == 0 ? 0 : (int32_t)std::min({a.max_len, a.table_width * a.cache.page_size, int64_t(INT32_MAX) - (1 << 20)});
+    p.q_packed = aligned(a.q, (size_t)(8 * es)) && a.q_token_stride % 8 == 0 && a.q_head_stride % 8 == 0;
+    p.out_packed = aligned(a.out, (size_t)(4 * es)) && a.out_token_stride % 4 == 0 && a.out_head_stride % 4 == 0;
+    p.groups_per_page = (int32_t)gpp;
+    p.page_shift = (gpp & (gpp - 1)) == 0 ? (int32_t)__builtin_ctzll((unsigned long long)gpp) : -1;
+    // a scale of zero leaves all scores equal; c > 0 keeps hidden ones at -inf
+    p.c = std::max(std::fabs(a.scale) * 1.44269504f, 0x1p-100f);
+    p.negative = a.scale < 0.0f;
+
+    // The many-rows kernel pays where its blocks fill the GPU, two a CU (bf16, 8 kv
+    // heads of 5 query heads each, us of it and of the other: 2 x 2047 tokens 676 and
+    // 877, 1 x 1024 169 and 149), in bf16 and at its head_dim; of fp32 and f16 (2 x
+    // 2047: 1200 and 1013, 873 and 743) and of head_dim 64 and 256 (1 x 1024: 133 and
+    // 98, 394 and 276) a like kernel was slower everywhere.  192 rows of 2048 keys
+    // took 33 us in the few-rows kernel, 51 in the other.
+    constexpr int64_t FEW_ROWS = 256;
+    const int64_t many_tiles = (rows + MANY_ROWS - 1) / MANY_ROWS;
+    if (a.dtype == SILI_BF16 && a.cache.head_dim == MANY_D && rows > FEW_ROWS && heads * many_tiles >= 512) L.many_tiles = many_tiles;
+    p.many = L.many_tiles ? (int32_t)FEW_ROWS : INT32_MAX;
+
+    const int parts = a.dtype == SILI_F32 ? 4 : 2;
+    p.columns = rows <= 16 / parts ? parts : 1;
+    const int64_t tile_rows = 16 / p.columns;
+    L.tiles = (std::min<int64_t>(rows, p.many) + tile_rows - 1) / tile_rows;
+    p.join_rows = (int32_t)std::min(tile_rows, rows);
+    // keys a row tile can reach: its rows' windows, aligned to 64
+    int64_t reach = a.max_len;
+    if (a.window > 0) reach = std::min(reach, a.window + (tile_rows - 1) / group + 1 + 63);
+    const int64_t blocks = std::max<int64_t>(1, heads * L.tiles);
+    // few blocks: as many waves in one as a CU holds, so that fewer splits are left
+    // to join (40 heads of 131071 keys, 8 blocks a split: 31 + 5 us against 31 + 7
+    // with 4 waves; 320 blocks of 2048 keys: 24 us against 22.6, a second round)
+    const int wide = waves_of(a.dtype, a.cache.head_dim, p.columns);
+    p.waves = blocks <= 128 ? wide : 4;
+    const int64_t step = 64 * p.waves;
+    // splits until every SIMD has as many waves as registers allow; fp32, which the
+    // vector units bound, two at most (320 blocks of 2048 keys: 22.7 us, with a
+    // second split 21.4 + 4.7 to join)
+    const int64_t fill = 256 * std::max(1, std::min(wide, a.dtype == SILI_F32 ? 8 : wide) / p.waves);
+    const int64_t want = std::clamp<int64_t>(fill / blocks, 1, std::max<int64_t>(1, (reach + 255) / 256));
+    p.chunk = (int32_t)std::max(step, ((reach + want - 1) / want + step - 1) / step * step);
+    p.splits = (int32_t)std::max<int64_t>(1, (reach + p.chunk - 1) / p.chunk);
+    return L;
 }
 
-size_t part_bytes(const sili_kv4_attend_args &a, const Launch &L) {
-    if (!L.on || L.plan.splits == 1) return 0;
-    return (size_t)a.tokens * (size_t)a.q_heads * (size_t)L.plan.splits * ((size_t)a.cache.head_dim * sizeof(float) + sizeof(float2));
+size_t part_bytes(const sili_kv4_attend_args &a, const AttendPlan &p) {
+    if (p.splits == 1) return 0;
+    return (size_t)a.tokens * (size_t)a.q_heads * (size_t)p.splits * ((size_t)a.cache.head_dim * sizeof(float) + sizeof(float2));
 }
 
 template <typename T, int D>
-void run_attend(const sili_kv4_attend_args &a, Launch (&L)[2], hipStream_t st) {
-    char *work = static_cast<char *>(a.workspace);
-    for (int k = 0; k < 2; ++k) {
-        if (!L[k].on) continue;
-        AttendPlan &p = L[k].plan;
-        const int64_t parts = a.tokens * a.q_heads * p.splits;
-        if (p.splits > 1) {
-            p.part_o = reinterpret_cast<float *>(work);
-            p.part_ml = reinterpret_cast<float2 *>(work + parts * D * sizeof(float));
-            work += part_bytes(a, L[k]);
-        }
-        const int64_t x = L[k].tiles * a.cache.kv_heads;
-        require(x <= INT32_MAX && p.splits <= 65535, "kv4_attend: too many rows or keys");
-        const dim3 grid((unsigned)x, (unsigned)p.splits, (unsigned)a.requests);
-        if (k == 0) {
-            constexpr int PARTS = sizeof(T) == 4 ? 4 : 2;
-            constexpr int WIDE = 4 * waves_per_simd<T, D, 1>(), WIDE_P = 4 * waves_per_simd<T, D, PARTS>();
-            const uint32_t lds = p.waves * p.join_rows * (D + 2) * sizeof(float);
-            const dim3 block(64 * p.waves);
-            if (p.columns > 1) {
-                if (p.waves == WIDE_P) launch(k_attend_few<T, D, WIDE_P, PARTS>, grid, block, lds, st, a, p);
-                else launch(k_attend_few<T, D, 4, PARTS>, grid, block, lds, st, a, p);
-            } else {
-                if (p.waves == WIDE) launch(k_attend_few<T, D, WIDE, 1>, grid, block, lds, st, a, p);
-                else launch(k_attend_few<T, D, 4, 1>, grid, block, lds, st, a, p);
-            }
-        } else {
-            launch(k_attend_many<T, D>, grid, dim3(64 * MANY_WAVES), (uint32_t)(2 * sizeof(ManyLds<D>)), st, a, p);
-        }
-        const int64_t rows = std::min<int64_t>(a.max_new * (a.q_heads / a.cache.kv_heads), p.many);
-        if (p.splits > 1)
-            launch(k_attend_join<T, D>, dim3((unsigned)rows, (unsigned)a.cache.kv_heads, (unsigned)a.requests), dim3(256), 0, st, a, p);
+void run_few(const sili_kv4_attend_args &a, const Launch &L, hipStream_t st) {
+    AttendPlan p = L.plan;
+    constexpr int PARTS = sizeof(T) == 4 ? 4 : 2;
+    constexpr int WIDE = 4 * waves_per_simd<T, D, 1>(), WIDE_P = 4 * waves_per_simd<T, D, PARTS>();
+    p.part_o = static_cast<float *>(a.workspace);
+    p.part_ml = reinterpret_cast<float2 *>(p.part_o + a.tokens * a.q_heads * p.splits * D);
+    const dim3 grid((unsigned)(L.tiles * a.cache.kv_heads), (unsigned)p.splits, (unsigned)a.requests), block(64 * p.waves);
+    const uint32_t lds = p.waves * p.join_rows * (D + 2) * sizeof(float);
+    if (p.columns > 1) {
+        if (p.waves == WIDE_P) launch(k_attend_few<T, D, WIDE_P, PARTS>, grid, block, lds, st, a, p);
+        else launch(k_attend_few<T, D, 4, PARTS>, grid, block, lds, st, a, p);
+    } else {
+        if (p.waves == WIDE) launch(k_attend_few<T, D, WIDE, 1>, grid, block, lds, st, a, p);
+        else launch(k_attend_few<T, D, 4, 1>, grid, block, lds, st, a, p);
     }
+    const int64_t rows = std::min<int64_t>(a.max_new * p.group, p.many);
+    if (p.splits > 1)
+        launch(k_attend_join<T, D>, dim3((unsigned)rows, (unsigned)a.cache.kv_heads, (unsigned)a.requests), dim3(256), 0, st, a, p);
 }
 
 }  // namespace
 
 size_t kv4_attend_workspace(const sili_kv4_attend_args &a) {
     check_attend(a);
-    Launch L[2];
-    plan_attend(a, L);
-    return part_bytes(a, L[0]) + part_bytes(a, L[1]);
+    return part_bytes(a, plan_attend(a).plan);
 }
 
 void kv4_attend(const sili_kv4_attend_args &a, hipStream_t st) {
@@ -1127,19 +1075,23 @@ void kv4_attend(const sili_kv4_attend_args &a, hipStream_t st) {
     if (a.tokens == 0 || a.requests == 0 || a.max_new == 0) return;
     require(a.q && a.out && a.q_start && a.kv_lens, "kv4_attend: NULL buffer");
     require(a.block_table || a.table_width == 0, "kv4_attend: NULL block_table");
-    Launch L[2];
-    plan_attend(a, L);
-    const size_t need = part_bytes(a, L[0]) + part_bytes(a, L[1]);
+    const Launch L = plan_attend(a);
+    const size_t need = part_bytes(a, L.plan);
     require(need == 0 || (a.workspace && aligned(a.workspace, 16) && a.workspace_bytes >= need),
             "kv4_attend: workspace too small or not 16-byte aligned");
+    require(L.tiles * a.cache.kv_heads <= INT32_MAX && L.plan.splits <= 65535, "kv4_attend: too many rows or keys");
     with_dtype(a.dtype, [&](auto z) {
         using T = decltype(z);
         switch (a.cache.head_dim) {
-            case 64: run_attend<T, 64>(a, L, st); break;
-            case 128: run_attend<T, 128>(a, L, st); break;
-            default: run_attend<T, 256>(a, L, st); break;
+            case 64: run_few<T, 64>(a, L, st); break;
+            case 128: run_few<T, 128>(a, L, st); break;
+            default: run_few<T, 256>(a, L, st); break;
         }
     });
+    if (L.many_tiles) {
+        launch(k_attend_many, dim3((unsigned)(L.many_tiles * a.cache.kv_heads), 1, (unsigned)a.requests), dim3(64 * MANY_WAVES),
+               (uint32_t)(2 * sizeof(ManyLds)), st, a, L.plan);
+    }
     SILI_HIP(hipGetLastError());
 }
 

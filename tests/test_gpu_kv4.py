@@ -229,6 +229,35 @@ def test_chunks(hip, d, heads, group, page, dtype, causal, window):
     check(host, attend(gpu, q, starts(new), lens, table, causal, window), starts(new), lens, table, causal, window)
 
 
+@pytest.mark.parametrize("causal,window,page", [(1, 0, 16), (0, 0, 48), (1, 70, 32)])
+def test_a_batch_of_long_chunks(hip, causal, window, page):
+    """Enough rows for blocks of 128 of them: chunks beside single tokens and
+    requests without any, lengths about the edges of steps, hidden pages."""
+    new = np.array([257, 300, 1, 0, 259, 320, 257, 2, 258, 299, 511, 257])
+    lens = np.array([257, 411, 700, 64, 320, 250, 513, 40, 385, 300, 600, 1000])
+    heads = 16
+    host, gpu, table = filled(lens, heads, page, 128, page)
+    table = table.copy()
+    table[5, 1], table[8, 0] = -1, len(host["k"]) + 3
+    q = queries(int(new.sum()), heads, 128, torch.bfloat16, 3)
+    s = attend(gpu, q, starts(new), lens, table, causal, window)
+    check(host, s, starts(new), lens, table, causal, window)
+    # strides, and a NaN scale that only the rows that see it meet
+    wide = torch.zeros(q.shape[0], heads + 1, 131, dtype=torch.bfloat16, device="cuda")
+    wide[:, :heads, 1:129] = q
+    out = torch.full((q.shape[0], heads, 132), 3.0, dtype=torch.bfloat16, device="cuda")
+    t = attend(gpu, wide[:, :heads, 1:129], starts(new), lens, table, causal, window, out=out[..., :128])
+    assert torch.equal(t["out"], s["out"]) and torch.equal(t["lse"], s["lse"]) and float((out[..., 128:].float() - 3).abs().max()) == 0
+    bad, r = 280, 1
+    gpu["v_scale"][table[r, bad // page], :, bad % page] = float("nan")
+    got = np.isnan(np64(attend(gpu, q, starts(new), lens, table, causal, window)["out"])).all(-1)
+    pos = lens[r] - new[r] + np.arange(new[r])
+    sees = (pos >= bad) & ((pos - window < bad) | (window == 0)) if causal else np.ones(new[r], bool)
+    want = np.zeros(q.shape[0], bool)
+    want[starts(new)[r]:starts(new)[r + 1]] = sees
+    assert np.array_equal(got, np.repeat(want[:, None], heads, 1))
+
+
 def test_rows_without_keys(hip):
     """More new tokens than keys: the first queries see nothing; a request without keys."""
     new, lens = np.array([5, 2, 4]), np.array([2, 0, 4])
