@@ -690,8 +690,8 @@ int sili_block_norm_backward(const sili_block_norm_args *args, const sili_block_
 int sili_block_norm_workspace(const sili_block_norm_args *args, size_t *bytes);
 
 /* A paged cache of keys and values in 4 bits.  Per token and kv head one fp32
- * scale amax / 6 and head_dim E2M1 codes, fp4_encode(x * (6 / amax)), the
- * layers' own codec (nearest, ties away from zero).  A head whose amax is below
+ * scale amax / 6 and head_dim E2M1 codes, fp4_encode(x * (6 * (1 / amax))) in
+ * fp32, the layers' own codec (nearest, ties away from zero).  A head whose amax is below
  * 2^-120 is stored as zeros; one with a NaN or an infinity gets a NaN scale and
  * reads as NaN.  Bytes hold channel 2b in the low and 2b + 1 in the high
  * nibble:

@@ -25,7 +25,7 @@ __device__ __forceinline__ float wave_max(float v) {
 // k codes, four bytes of v codes.  The bytes of 16 tokens share their 16-byte runs
 // of v codes, so a block takes one head of as many tokens as its threads cover:
 // their bytes meet in one L2 (a block of one token's heads, whose neighbours run on
-// other XCDs, wrote 2048 tokens of 40 heads in 42 us).
+// other XCDs, wrote 2048 tokens of 40 fp32 heads in 42 us; so, 30, and 27 read).
 constexpr int ROWS_TPB = 256;
 
 // Maximum over the aligned group of N lanes.
@@ -58,7 +58,7 @@ __device__ __forceinline__ uint32_t encode8(const float (&x)[8], float &scale) {
     const float bad = sum != 0.0f || sum != sum ? INFINITY : 0.0f;
     top = group_max<N>(fmaxf(top, bad));
     const bool finite = top < INFINITY, zero = !finite || top < 0x1p-120f;
-    const float inv = zero ? 0.0f : 6.0f / top;
+    const float inv = zero ? 0.0f : 6.0f * (1.0f / top);
     uint32_t w = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) w |= fp4_encode(x[j] * inv) << (4 * j);

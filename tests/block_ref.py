@@ -111,7 +111,7 @@ def kv4_codes(x):
     bad = ~np.isfinite(x).all(-1, keepdims=True)
     zero = bad | (top < np.float32(2.0 ** -120))
     with np.errstate(all="ignore"):
-        y = np.where(zero, np.float32(0), x * np.where(zero, np.float32(0), np.float32(6) / top))
+        y = np.where(zero, np.float32(0), x * np.where(zero, np.float32(0), np.float32(6) * (np.float32(1) / top)))
     mag = np.searchsorted(np.float32([.25, .75, 1.25, 1.75, 2.5, 3.5, 5]), np.abs(y), side="right")
     scale = np.where(bad, np.float32(np.nan), np.where(zero, np.float32(0), top / np.float32(6)))
     return (mag + 8 * ((y < 0) & (mag > 0))).astype(np.uint8), scale[..., 0].astype(np.float32)
