@@ -334,7 +334,7 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_at
     const int32_t i_first = token_of(pl, first), i_last = token_of(pl, min(first + RT - 1, n_rows - 1));
     const int32_t lo = kr.begin(i_first) & ~63, hi = kr.end(i_last);
     const int32_t all_end = kr.end(i_first), all_begin = kr.begin(i_last);  // what every row sees
-    const int32_t c0 = lo + split * pl.chunk, c1 = min(hi, c0 + pl.chunk);
+    const int32_t c0 = lo + split * pl.chunk, c1 = c0 + min(hi - c0, pl.chunk);
 
     uint32_t take_q[QP], take_p[PP];  // CP > 1: the part this lane's column holds
 #pragma unroll
@@ -908,7 +908,7 @@ void check_cache(const sili_kv4_cache &c, const char *what) {
     need(c.head_dim == 64 || c.head_dim == 128 || c.head_dim == 256, "head_dim is none of 64, 128, 256");
     need(c.page_size >= 16 && c.page_size % 16 == 0 && c.page_size <= 65536, "page_size is not a multiple of 16 up to 65536");
     need(c.kv_heads >= 1 && c.kv_heads <= 65535, "kv_heads out of range");
-    need(c.n_pages >= 0 && c.n_pages * c.page_size <= (int64_t(1) << 31), "more than 2^31 slots");
+    need(c.n_pages >= 0 && c.n_pages <= (int64_t(1) << 31) / c.page_size, "more than 2^31 slots");
     need(c.n_pages == 0 || (c.k && c.v && c.k_scale && c.v_scale), "NULL cache");
     need(aligned(c.k, 16) && aligned(c.v, 16) && aligned(c.k_scale, 16) && aligned(c.v_scale, 16), "cache is not 16-byte aligned");
 }
@@ -922,7 +922,7 @@ void rows(const sili_kv4_rows_args &a, hipStream_t st, const char *what) {
     require(a.slots && a.k && a.v, "kv4 rows: NULL buffer");
     const int64_t tokens = ROWS_TPB / (a.cache.head_dim / 8);  // of a block
     const int64_t blocks = (a.tokens + tokens - 1) / tokens * a.cache.kv_heads;
-    require(blocks <= INT32_MAX, "kv4 rows: too many rows");
+    require(blocks < (int64_t(1) << 32) / ROWS_TPB, "kv4 rows: too many rows");
     auto packs = [&](const void *p, int64_t ts, int64_t hs) {
         return aligned(p, (size_t)(8 * dtype_size(a.dtype))) && ts % 8 == 0 && hs % 8 == 0;
     };
@@ -947,9 +947,9 @@ void check_attend(const sili_kv4_attend_args &a) {
     require(a.q_heads >= 1 && a.q_heads % a.cache.kv_heads == 0, "kv4_attend: q_heads is no multiple of kv_heads");
     require(a.q_heads <= 65535 && a.tokens * a.q_heads <= INT32_MAX, "kv4_attend: too many query heads");
     require(a.cache.n_pages * (a.cache.page_size / 16) * a.cache.kv_heads <= INT32_MAX, "kv4_attend: cache too large");
-    require(a.max_new * (a.q_heads / a.cache.kv_heads) <= INT32_MAX, "kv4_attend: too many rows");
     require(a.table_width >= 0 && a.max_new >= 0 && a.max_len >= 0, "kv4_attend: negative size");
-    require(a.max_len < (int64_t(1) << 31) && a.max_new < (int64_t(1) << 31), "kv4_attend: bound out of range");
+    require(a.max_len <= INT32_MAX && a.max_new <= INT32_MAX && a.table_width <= INT32_MAX, "kv4_attend: bound out of range");
+    require(a.max_new * (a.q_heads / a.cache.kv_heads) <= INT32_MAX, "kv4_attend: too many rows");
     require(a.window >= 0 && (a.window == 0 || a.causal), "kv4_attend: a window needs the causal mask");
 }
 
@@ -957,7 +957,6 @@ void check_attend(const sili_kv4_attend_args &a) {
 
 void kv4_append(const sili_kv4_rows_args &a, hipStream_t st) { rows<true>(a, st, "kv4_append"); }
 void kv4_read(const sili_kv4_rows_args &a, hipStream_t st) { rows<false>(a, st, "kv4_read"); }
-
 
 namespace {
 
@@ -979,14 +978,15 @@ int waves_of(int dtype, int64_t head_dim, int columns) {
 // How a call is launched: requests of up to plan.many rows go to the few-rows
 // kernel, `tiles` row tiles a (request, kv head), those of more to the other.
 struct Launch {
-    int64_t tiles = 0, many_tiles = 0;
+    int64_t rows = 0, tiles = 0, many_tiles = 0;
     AttendPlan plan{};
 };
 
 Launch plan_attend(const sili_kv4_attend_args &a) {
     Launch L;
     AttendPlan &p = L.plan;
-    const int64_t group = a.q_heads / a.cache.kv_heads, rows = a.max_new * group, heads = a.requests * a.cache.kv_heads;
+    const int64_t group = a.q_heads / a.cache.kv_heads, heads = a.requests * a.cache.kv_heads;
+    const int64_t rows = std::min(a.max_new, a.tokens) * group;  // of the longest request at most
     const int64_t gpp = a.cache.page_size / 16, es = dtype_size(a.dtype);
     p.kv_heads = (int32_t)a.cache.kv_heads;
     p.group = (int32_t)group;
@@ -1015,10 +1015,11 @@ Launch plan_attend(const sili_kv4_attend_args &a) {
     const int parts = a.dtype == SILI_F32 ? 4 : 2;
     p.columns = rows <= 16 / parts ? parts : 1;
     const int64_t tile_rows = 16 / p.columns;
-    L.tiles = (std::min<int64_t>(rows, p.many) + tile_rows - 1) / tile_rows;
+    L.rows = std::min<int64_t>(rows, p.many);
+    L.tiles = (L.rows + tile_rows - 1) / tile_rows;
     p.join_rows = (int32_t)std::min(tile_rows, rows);
     // keys a row tile can reach: its rows' windows, aligned to 64
-    int64_t reach = a.max_len;
+    int64_t reach = p.most;
     if (a.window > 0) reach = std::min(reach, a.window + (tile_rows - 1) / group + 1 + 63);
     const int64_t blocks = std::max<int64_t>(1, heads * L.tiles);
     // few blocks: as many waves in one as a CU holds, so that fewer splits are left
@@ -1058,9 +1059,8 @@ void run_few(const sili_kv4_attend_args &a, const Launch &L, hipStream_t st) {
         if (p.waves == WIDE) launch(k_attend_few<T, D, WIDE, 1>, grid, block, lds, st, a, p);
         else launch(k_attend_few<T, D, 4, 1>, grid, block, lds, st, a, p);
     }
-    const int64_t rows = std::min<int64_t>(a.max_new * p.group, p.many);
     if (p.splits > 1)
-        launch(k_attend_join<T, D>, dim3((unsigned)rows, (unsigned)a.cache.kv_heads, (unsigned)a.requests), dim3(256), 0, st, a, p);
+        launch(k_attend_join<T, D>, dim3((unsigned)L.rows, (unsigned)a.cache.kv_heads, (unsigned)a.requests), dim3(256), 0, st, a, p);
 }
 
 }  // namespace
@@ -1079,7 +1079,10 @@ void kv4_attend(const sili_kv4_attend_args &a, hipStream_t st) {
     const size_t need = part_bytes(a, L.plan);
     require(need == 0 || (a.workspace && aligned(a.workspace, 16) && a.workspace_bytes >= need),
             "kv4_attend: workspace too small or not 16-byte aligned");
-    require(L.tiles * a.cache.kv_heads <= INT32_MAX && L.plan.splits <= 65535, "kv4_attend: too many rows or keys");
+    const int64_t most = (int64_t(1) << 32) - 1;  // threads of a grid's x
+    require(L.tiles * a.cache.kv_heads * 64 * L.plan.waves <= most && L.many_tiles * a.cache.kv_heads * 64 * MANY_WAVES <= most &&
+                L.rows * (L.plan.splits > 1 ? 256 : 1) <= most && L.plan.splits <= 65535,
+            "kv4_attend: too many rows or keys");
     with_dtype(a.dtype, [&](auto z) {
         using T = decltype(z);
         switch (a.cache.head_dim) {

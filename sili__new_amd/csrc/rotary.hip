@@ -3,8 +3,10 @@
 // Pair i of a head at position p turns by the angle p * step_i, in turns of
 // 2^64: the product wraps modulo one turn, so the fraction keeps its accuracy
 // at any position (32 bits of it are used, 1.5e-9 rad).  Bound by memory: each
-// element is read and written once.  A thread owns one vector of pairs of a
-// token, takes its sines and cosines once and walks heads with them.
+// element is read and written once.  A thread owns one run of pairs of a token,
+// 16 bytes, takes its sines and cosines once and walks heads with them, four in
+// flight (8192 tokens of 48 bf16 heads of 128, half of each turned: 44 us, 4.6 TB/s;
+// a head at a time, 51 us).
 #include "block_ops.hpp"
 
 #include <algorithm>
@@ -131,7 +133,8 @@ void run(const sili_rotary_args &a, hipStream_t st) {
 
 void rotary(const sili_rotary_args &a, hipStream_t st) {
     require(a.tokens >= 0 && a.q_heads >= 0 && a.k_heads >= 0, "rotary: negative size");
-    require(a.q_heads + a.k_heads <= 65535, "rotary: too many heads");
+    require(a.tokens < (int64_t(1) << 31), "rotary: too many tokens");
+    require(a.q_heads <= 65535 && a.k_heads <= 65535 && a.q_heads + a.k_heads <= 65535, "rotary: too many heads");
     require(a.head_dim > 0 && a.head_dim <= 65536, "rotary: head_dim out of range");
     require(a.rot_dim >= 0 && a.rot_dim % 2 == 0 && a.rot_dim <= a.head_dim, "rotary: rot_dim is not an even number up to head_dim");
     require(a.layout == SILI_ROTARY_HALF || a.layout == SILI_ROTARY_INTERLEAVED, "rotary: unknown layout");

@@ -285,6 +285,19 @@ def test_bounds_and_pages_outside_the_cache(hip):
     check(host, attend(gpu, q, starts(new), lens, table[:, :3]), starts(new), lens, table[:, :3])
 
 
+@pytest.mark.parametrize("heads,requests,window", [(1, 3, 0), (8, 40, 0), (4, 3, 50), (8, 40, 130)])
+def test_bounds_that_bound_nothing(hip, heads, requests, window):
+    """The largest max_len and max_new: the table's width and the batch bound the work."""
+    rng = np.random.default_rng(requests + window)
+    new = rng.integers(1, 4, requests)
+    lens = new + rng.integers(0, 900, requests)
+    host, gpu, table = filled(lens, heads, 16, 128, 5)
+    for dtype in (torch.float32, torch.bfloat16):
+        q = queries(int(new.sum()), 2 * heads, 128, dtype, 4)
+        s = attend(gpu, q, starts(new), lens, table, 1, window, max_new=(1 << 30) - 1, max_len=(1 << 31) - 1)
+        check(host, s, starts(new), lens, table, 1, window)
+
+
 def test_tokens_of_no_request_are_left_alone(hip):
     """Padding before the first and past the last request's tokens."""
     lens = np.array([20, 33])
