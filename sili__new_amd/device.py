@@ -11,7 +11,9 @@ argument struct, with the header's field names (pointers as integers, e.g.
 
 The calls are asynchronous on their stream.  Errors raise the exceptions that
 SparseLinearLayer's methods raise: ValueError, MemoryError, IndexError,
-RuntimeError.  An argument struct may be kept and called again.
+RuntimeError.  An argument struct may be kept and called again.  A program that
+also uses torch imports torch before this package (torch brings a HIP runtime
+of its own and finds no device next to another one).
 """
 from __future__ import annotations
 

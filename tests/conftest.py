@@ -10,6 +10,12 @@ if ROOT not in sys.path:
 
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs an MI355X (runs the HIP path)")
+    try:
+        # before any test file loads the library: torch brings a HIP runtime of its own,
+        # and a process that has loaded another one first gives torch no device
+        import torch  # noqa: F401
+    except ImportError:
+        pass
 
 
 def gpu_available() -> bool:
