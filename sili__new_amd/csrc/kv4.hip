@@ -600,9 +600,11 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_at
 // own.  Rows of LDS are padded by 16 bytes, which spreads eight lanes' 16 bytes
 // over all banks.  A weight enters in one bf16 part: its rounding is as large as
 // the output's own, together 1.4 times that, and a second part would be half as
-// many products again.  Issue bounds it (2 x 2047 tokens of 40 heads under a window
-// of 4096: 520 us, the vector units busy 45 % of the time, the matrix cores 31 %,
-// with a last round of blocks that fills a quarter of the GPU).
+// many products again.  Half of a step's scores are scaled under the products of
+// the other half, and the weights of 16 keys are taken under the products of the 16
+// before; without, the wave's vector work and its products take turns (2 x 2047
+// tokens of 40 heads under a window of 4096: 455 us, with it 434, 0.79 PFLOP/s).
+// Issue bounds it, with a last round of blocks that leaves half of their places empty.
 constexpr int MANY_WAVES = 4, MANY_ROWS = 32 * MANY_WAVES;
 
 constexpr int MANY_D = 128;
@@ -612,7 +614,7 @@ struct ManyLds {
     static constexpr int K_ROW = 2 * D + 16, V_ROW = 2 * 64 + 16;  // bytes
     uint8_t k[64 * K_ROW];  // [key][channel]
     uint8_t v[D * V_ROW];   // [channel][key], the even channels before the odd ones
-    float ks[64], vs[64];
+    float ks[64], vs[64];  // ks times c
     int32_t held[4];        // the group of 16 keys is in the cache
 };
 
@@ -714,7 +716,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void k_attend_many(sili_kv4_att
         *reinterpret_cast<u32x4 *>(vd + 16) = (u32x4){e[1][0], e[1][1], e[3][0], e[3][1]};
         *reinterpret_cast<u32x4 *>(vd + D / 2 * Lds::V_ROW) = (u32x4){d[0][0], d[0][1], d[2][0], d[2][1]};
         *reinterpret_cast<u32x4 *>(vd + D / 2 * Lds::V_ROW + 16) = (u32x4){d[1][0], d[1][1], d[3][0], d[3][1]};
-        if (tid < 128) (tid < 64 ? b.ks : b.vs)[tid & 63] = scale;
+        if (tid < 128) (tid < 64 ? b.ks : b.vs)[tid & 63] = tid < 64 ? scale * pl.c : scale;
         if (tid < 64 && (tid & 15) == 0) b.held[tid >> 4] = held;
     };
 
@@ -739,51 +741,54 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void k_attend_many(sili_kv4_att
             for (int x = 0; x < 2; ++x)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sc[x][i] = 0.0f;
-            // K's operands, AHEAD steps of 16 channels before their products: the
-            // compiler left to itself waits for each read of LDS
-            constexpr int AHEAD = 2;
-            u32x4 kk[KS][2];
+            float ref = m == -INFINITY ? 0.0f : m;
+            float v[32];  // scores less ref, then weights: 16 x + 4 a + b
+            // K's operands, AHEAD products before theirs: the compiler left to itself
+            // waits for each read of LDS.  The first half's scores are scaled under the
+            // second half's products.
+            constexpr int AHEAD = 4;
+            u32x4 kk[2 * KS];
+            f32x4 f[8];
 #pragma unroll
-            for (int s = 0; s < KS + AHEAD; ++s) {
-                if (s < KS) {
-#pragma unroll
-                    for (int x = 0; x < 2; ++x)
-                        kk[s][x] = *reinterpret_cast<const u32x4 *>(b.k + (32 * x + r32) * Lds::K_ROW + 32 * s + 16 * hf);
+            for (int s = 0; s < 2 * KS + AHEAD; ++s) {
+                if (s < 2 * KS) {
+                    kk[s] = *reinterpret_cast<const u32x4 *>(b.k + (32 * (s / KS) + r32) * Lds::K_ROW + 32 * (s % KS) + 16 * hf);
+                    if (s % 2 == 1) f[s / 2] = *reinterpret_cast<const f32x4 *>(b.ks + 8 * (s / 2) + 4 * hf);
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                if (s >= AHEAD) {
+                const int t = s - AHEAD;
+                if (t >= 0) sc[t / KS] = mma(kk[t], q[t % KS], sc[t / KS]);
+                if (t >= KS + 2) {  // the first half's last product is two before this one
+                    constexpr int LEFT = KS - 2;
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) sc[x] = mma(kk[s - AHEAD][x], q[s - AHEAD], sc[x]);
+                    for (int j = 16 * (t - KS - 2) / LEFT; j < 16 * (t - KS - 1) / LEFT; ++j) {
+                        v[j] = __builtin_fmaf(sc[0][j], f[j >> 2][j & 3], -ref);
+                        __asm__ volatile("" : "+v"(v[j]));  // here, not past the next branch
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
+#pragma unroll
+            for (int j = 16; j < 32; ++j) v[j] = __builtin_fmaf(sc[1][j - 16], f[j >> 2][j & 3], -ref);
             // wave-uniform: every row sees every key of the step
             const int4 in = *reinterpret_cast<const int4 *>(b.held);
             const bool whole = key >= all_begin && key + 64 <= all_end && uniform(in.x & in.y & in.z & in.w) != 0;
-            float v[32];  // scores, then weights: 16 x + 4 a + b
-#pragma unroll
-            for (int y = 0; y < 8; ++y) {
-                const float4 f = *reinterpret_cast<const float4 *>(b.ks + 8 * y + 4 * hf);
-                v[4 * y] = sc[y >> 2][4 * (y & 3)] * f.x;
-                v[4 * y + 1] = sc[y >> 2][4 * (y & 3) + 1] * f.y;
-                v[4 * y + 2] = sc[y >> 2][4 * (y & 3) + 2] * f.z;
-                v[4 * y + 3] = sc[y >> 2][4 * (y & 3) + 3] * f.w;
-            }
             const int32_t there[4] = {in.x, in.y, in.z, in.w};
-            // v[j] (j: 16 x + 4 a + b) where this row sees the key, else `other`
-            auto hide = [&](float other) {
+            // w[0 .. n) (v[at ..), j: 16 x + 4 a + b) where this row sees the key, else `other`
+            auto hide = [&](float *w, int at, int n, float other) {
                 int32_t from = begin - key - 4 * hf, to = end - key - 4 * hf;
                 stay_branch(from, to);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
+                for (int j = at; j < at + n; ++j) {
                     const int32_t k = 8 * (j >> 2) + (j & 3);
-                    v[j] = k >= from && k < to && there[j >> 3] != 0 ? v[j] : other;
+                    w[j - at] = k >= from && k < to && there[j >> 3] != 0 ? w[j - at] : other;
                 }
             };
-            if (!whole) hide(-INFINITY);
+            if (!whole) hide(v, 0, 32, -INFINITY);
             float top = v[0];
 #pragma unroll
             for (int j = 1; j < 32; ++j) top = fmaxf(top, v[j]);
-            top *= pl.c;
+            top += ref;
             if (__any(top > m + SLACK)) {
                 const float up = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
                 // a row without a key so far keeps m = -inf, and factor 1 on its zeros
@@ -792,33 +797,56 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void k_attend_many(sili_kv4_att
                 l *= keep;
 #pragma unroll
                 for (int ct = 0; ct < CT; ++ct) o[ct] *= keep;
+                const float less = up == -INFINITY ? 0.0f : up - ref;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] -= less;
             }
-            const float ref = m == -INFINITY ? 0.0f : m;
-            float sum = 0.0f;
+            // Weights of 16 keys at a time, under the products of the 16 before.
+            float sum = 0.0f, w[8];
+            auto weigh = [&](int t) {
 #pragma unroll
-            for (int y = 0; y < 8; ++y) {
-                const float4 f = *reinterpret_cast<const float4 *>(b.vs + 8 * y + 4 * hf);
-                const float fs[4] = {f.x, f.y, f.z, f.w};
+                for (int y = 0; y < 2; ++y) {
+                    const float4 f = *reinterpret_cast<const float4 *>(b.vs + 8 * (2 * t + y) + 4 * hf);
+                    const float fs[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(v[4 * y + i], pl.c, -ref));
-                    sum += e;
-                    v[4 * y + i] = e * fs[i];
+                    for (int i = 0; i < 4; ++i) {
+                        const float g = __builtin_amdgcn_exp2f(v[8 * t + 4 * y + i]);
+                        sum += g;
+                        w[4 * y + i] = g * fs[i];
+                    }
+                }
+            };
+            u32x4 vv[2][CT];
+            auto values = [&](int t) {
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct) vv[t & 1][ct] = *reinterpret_cast<const u32x4 *>(b.v + (32 * ct + r32) * Lds::V_ROW + 32 * t + 16 * hf);
+            };
+            weigh(0);
+            values(0);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                if (!whole) hide(w, 8 * t, 8, 0.0f);  // a key that this row does not see may hold anything
+                u32x4 p;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) p[j] = pack_bf16(w[2 * j], w[2 * j + 1]);
+                if (t < 3) {
+                    values(t + 1);
+                    weigh(t + 1);
+                }
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct) o[ct] = mma(vv[t & 1][ct], p, o[ct]);
+                if (t < 3) {  // the order: reads of LDS, the four packs; a product, two exp2, four others; ...
+                    __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+#pragma unroll
+                    for (int ct = 0; ct < CT; ++ct) {
+                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x400, 2, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+                    }
                 }
             }
             l += sum;
-            if (!whole) hide(0.0f);  // a key that this row does not see may hold anything
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {  // 16 keys
-                u32x4 p;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) p[j] = pack_bf16(v[8 * s + 2 * j], v[8 * s + 2 * j + 1]);
-#pragma unroll
-                for (int ct = 0; ct < CT; ++ct) {
-                    const u32x4 vv = *reinterpret_cast<const u32x4 *>(b.v + (32 * ct + r32) * Lds::V_ROW + 32 * s + 16 * hf);
-                    o[ct] = mma(vv, p, o[ct]);
-                }
-            }
         }
         if (more) unpack(lds[buf ^ 1]);
     }
