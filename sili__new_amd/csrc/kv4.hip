@@ -603,7 +603,7 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_at
 // many products again.  Half of a step's scores are scaled under the products of
 // the other half, and the weights of 16 keys are taken under the products of the 16
 // before; without, the wave's vector work and its products take turns (2 x 2047
-// tokens of 40 heads under a window of 4096: 455 us, with it 434, 0.79 PFLOP/s).
+// tokens of 40 heads under a window of 4096: 455 us, with it 434, 0.75 PFLOP/s).
 // Issue bounds it, with a last round of blocks that leaves half of their places empty.
 constexpr int MANY_WAVES = 4, MANY_ROWS = 32 * MANY_WAVES;
 
