@@ -1030,11 +1030,13 @@ Launch plan_attend(const sili_kv4_attend_args &a) {
     p.negative = a.scale < 0.0f;
 
     // The many-rows kernel pays where its blocks fill the GPU, two a CU (bf16, 8 kv
-    // heads of 5 query heads each, us of it and of the other: 2 x 2047 tokens 676 and
-    // 877, 1 x 1024 169 and 149), in bf16 and at its head_dim; of fp32 and f16 (2 x
-    // 2047: 1200 and 1013, 873 and 743) and of head_dim 64 and 256 (1 x 1024: 133 and
-    // 98, 394 and 276) a like kernel was slower everywhere.  192 rows of 2048 keys
-    // took 33 us in the few-rows kernel, 51 in the other.
+    // heads of 5 query heads each, chunks at the end of 4096 keys more, us of it and of
+    // the other: 1280 blocks 452 and 625, 768 276 and 310, 640 214 and 258, 384 146 and
+    // 152, 320 204 and 197 or 151 and 128, 160 142 and 104), in bf16 and at its
+    // head_dim; of fp32 and f16 (2 x 2047 tokens: 1200 and 1013, 873 and 743) and of
+    // head_dim 64 and 256 (1 x 1024: 133 and 98, 394 and 276) a like kernel was slower
+    // everywhere.  192 rows of 2048 keys took 33 us in the few-rows kernel, 51 in the
+    // other.
     constexpr int64_t FEW_ROWS = 256;
     const int64_t many_tiles = (rows + MANY_ROWS - 1) / MANY_ROWS;
     if (a.dtype == SILI_BF16 && a.cache.head_dim == MANY_D && rows > FEW_ROWS && heads * many_tiles >= 512) L.many_tiles = many_tiles;
