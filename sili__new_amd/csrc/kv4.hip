@@ -232,6 +232,7 @@ struct AttendPlan {
     int32_t kv_heads, group;  // query heads a kv head
     uint32_t group_inv;       // floor(2^32 / group), at most 2^32 - 1
     int32_t n_pages, most;    // pages of the cache; keys that max_len and the table allow
+    int32_t window;           // 0: none
     bool q_packed, out_packed;  // rows of q in 16-byte pieces; of out in pieces of 4 elements
     int32_t groups_per_page;  // page_size / 16
     int32_t page_shift;       // its logarithm, or -1
@@ -270,7 +271,10 @@ struct KeyRange {
     int32_t base, cap, window;  // keys before the first query, keys there are
     bool causal;
     __device__ __forceinline__ int32_t end(int32_t i) const { return causal ? min(cap, base + i + 1) : cap; }
-    __device__ __forceinline__ int32_t begin(int32_t i) const { return window > 0 ? max(0, base + i + 1 - window) : 0; }
+    __device__ __forceinline__ int32_t begin(int32_t i) const {
+        const int32_t upto = base + i + 1;  // negative where the query comes before the first key
+        return window > 0 && upto > window ? upto - window : 0;
+    }
 };
 
 // Registers allow this many waves on a SIMD without spilling.
@@ -318,7 +322,7 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_at
         return table[pl.page_shift >= 0 ? mine >> pl.page_shift : mine / pl.groups_per_page];
     };
     int32_t page = -1;
-    if (a.window == 0 && key + 16 * g < pl.most) page = entry(key);
+    if (pl.window == 0 && key + 16 * g < pl.most) page = entry(key);
 
     const int32_t q0 = a.q_start[req];
     const int32_t n_all = a.q_start[req + 1] - q0, n = min(n_all, (int32_t)a.max_new);
@@ -328,7 +332,7 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_at
     if (q0 < 0 || n_rows > pl.many || first >= n_rows) return;
     KeyRange kr;
     kr.base = kv - n_all;
-    kr.window = (int32_t)a.window;
+    kr.window = pl.window;
     kr.causal = a.causal != 0;
     kr.cap = min(kv, pl.most);
     const int32_t i_first = token_of(pl, first), i_last = token_of(pl, min(first + RT - 1, n_rows - 1));
@@ -424,7 +428,7 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_at
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) vw[ct] = *reinterpret_cast<const uint4 *>(vp + ct * 256);
     };
-    if (a.window > 0) {
+    if (pl.window > 0) {
         key += lo;
         page = page_of(key);
     }
@@ -637,7 +641,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void k_attend_many(sili_kv4_att
     if (q0 < 0 || n_rows <= pl.many || block_first >= n_rows) return;
     KeyRange kr;
     kr.base = kv - n_all;
-    kr.window = (int32_t)a.window;
+    kr.window = pl.window;
     kr.causal = a.causal != 0;
     kr.cap = min(kv, pl.most);
     const int32_t c0 = kr.begin(token_of(pl, block_first)) & ~63, c1 = kr.end(token_of(pl, min(block_first + MANY_ROWS, n_rows) - 1));
@@ -1021,6 +1025,9 @@ Launch plan_attend(const sili_kv4_attend_args &a) {
     p.group_inv = group == 1 ? ~0u : (uint32_t)((uint64_t(1) << 32) / (uint64_t)group);
     p.n_pages = (int32_t)a.cache.n_pages;
     p.most = p.n_pages == 0 ? 0 : (int32_t)std::min({a.max_len, a.table_width * a.cache.page_size, int64_t(INT32_MAX) - (1 << 20)});
+    // lengths are int32, so a window of 2^31 - 1 hides nothing (max_len says less: positions
+    // count the keys past it)
+    p.window = a.window < INT32_MAX ? (int32_t)a.window : 0;
     p.q_packed = aligned(a.q, (size_t)(8 * es)) && a.q_token_stride % 8 == 0 && a.q_head_stride % 8 == 0;
     p.out_packed = aligned(a.out, (size_t)(4 * es)) && a.out_token_stride % 4 == 0 && a.out_head_stride % 4 == 0;
     p.groups_per_page = (int32_t)gpp;
@@ -1050,7 +1057,7 @@ Launch plan_attend(const sili_kv4_attend_args &a) {
     p.join_rows = (int32_t)std::min(tile_rows, rows);
     // keys a row tile can reach: its rows' windows, aligned to 64
     int64_t reach = p.most;
-    if (a.window > 0) reach = std::min(reach, a.window + (tile_rows - 1) / group + 1 + 63);
+    if (p.window > 0) reach = std::min(reach, p.window + (tile_rows - 1) / group + 1 + 63);
     const int64_t blocks = std::max<int64_t>(1, heads * L.tiles);
     // few blocks: as many waves in one as a CU holds, so that fewer splits are left
     // to join (40 heads of 131071 keys, 8 blocks a split: 31 + 5 us against 31 + 7
