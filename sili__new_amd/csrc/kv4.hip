@@ -266,6 +266,21 @@ __device__ __forceinline__ void store4(T *out, const float (&x)[4], bool packed)
     }
 }
 
+// A request's query tokens: the first, how many it has, and how many of them are
+// computed: the launch and the join's LDS are sized for max_new and for the
+// batch's tokens, which q_start may pass (it does where a step brought more tokens
+// than its buffers hold).
+struct Queries {
+    int32_t first, all, n;
+};
+__device__ __forceinline__ Queries queries_of(const sili_kv4_attend_args &a, int req) {
+    Queries q;
+    q.first = a.q_start[req];
+    q.all = a.q_start[req + 1] - q.first;
+    q.n = q.first < 0 ? 0 : min(q.all, min((int32_t)a.max_new, (int32_t)a.tokens - q.first));
+    return q;
+}
+
 // Keys that query i of n sees, [begin, end).
 struct KeyRange {
     int32_t base, cap, window;  // keys before the first query, keys there are
@@ -324,14 +339,13 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_at
     int32_t page = -1;
     if (pl.window == 0 && key + 16 * g < pl.most) page = entry(key);
 
-    const int32_t q0 = a.q_start[req];
-    const int32_t n_all = a.q_start[req + 1] - q0, n = min(n_all, (int32_t)a.max_new);
+    const Queries qs = queries_of(a, req);
     const int32_t kv = a.kv_lens[req];
-    const int32_t n_rows = n * group;
+    const int32_t n_rows = qs.n * group;
     const int32_t first = tile * RT;
-    if (q0 < 0 || n_rows > pl.many || first >= n_rows) return;
+    if (n_rows > pl.many || first >= n_rows) return;
     KeyRange kr;
-    kr.base = kv - n_all;
+    kr.base = kv - qs.all;
     kr.window = pl.window;
     kr.causal = a.causal != 0;
     kr.cap = min(kv, pl.most);
@@ -352,9 +366,7 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_at
     u32x4 q[KS][QM];
     {
         const int32_t row = min(first + my_row, n_rows - 1), i = my_i;
-        const int64_t token = q0 + i;
-        const T *src = (const T *)a.q + (token < a.tokens ? token * a.q_token_stride : 0) +
-                       (h * group + (row - i * group)) * a.q_head_stride + g * (D / 4);
+        const T *src = (const T *)a.q + (int64_t)(qs.first + i) * a.q_token_stride + (h * group + (row - i * group)) * a.q_head_stride + g * (D / 4);
         float xs[KS][8];
         if (pl.q_packed) {
 #pragma unroll
@@ -578,8 +590,7 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_at
             acc[3] += f[w] * x.w;
         }
         const int32_t i = token_of(pl, first + row);
-        const int64_t token = q0 + i, qh = h * group + (first + row - i * group);
-        if (token >= a.tokens) continue;
+        const int64_t token = qs.first + i, qh = h * group + (first + row - i * group);
         if (pl.splits > 1) {
             const int64_t slot = (token * a.q_heads + qh) * pl.splits + split;
             if (ll != 0.0f) *reinterpret_cast<float4 *>(pl.part_o + slot * D + ch) = make_float4(acc[0], acc[1], acc[2], acc[3]);
@@ -633,14 +644,13 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void k_attend_many(sili_kv4_att
     const int H = pl.kv_heads, group = pl.group;
     const int h = blockIdx.x % H, tile = blockIdx.x / H, req = blockIdx.z;
     const int32_t *table = a.block_table + (int64_t)req * a.table_width;
-    const int32_t q0 = a.q_start[req];
-    const int32_t n_all = a.q_start[req + 1] - q0, n = min(n_all, (int32_t)a.max_new);
+    const Queries qs = queries_of(a, req);
     const int32_t kv = a.kv_lens[req];
-    const int32_t n_rows = n * group;
+    const int32_t n_rows = qs.n * group;
     const int32_t block_first = tile * MANY_ROWS;
-    if (q0 < 0 || n_rows <= pl.many || block_first >= n_rows) return;
+    if (n_rows <= pl.many || block_first >= n_rows) return;
     KeyRange kr;
-    kr.base = kv - n_all;
+    kr.base = kv - qs.all;
     kr.window = pl.window;
     kr.causal = a.causal != 0;
     kr.cap = min(kv, pl.most);
@@ -655,9 +665,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void k_attend_many(sili_kv4_att
 
     u32x4 q[KS];  // channels 16 s + 8 hf + 0 .. 7
     {
-        const int64_t token = q0 + my_i;
-        const T *src = (const T *)a.q + (token < a.tokens ? token * a.q_token_stride : 0) +
-                       (h * group + (row - my_i * group)) * a.q_head_stride + 8 * hf;
+        const T *src = (const T *)a.q + (int64_t)(qs.first + my_i) * a.q_token_stride + (h * group + (row - my_i * group)) * a.q_head_stride + 8 * hf;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             float x[8];
@@ -858,8 +866,8 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void k_attend_many(sili_kv4_att
 
     // lane: row r32; result 4 a + b of tile ct is row 32 ct + 8 a + 4 hf + b of V's
     // channels in LDS, even ones in the first half of the tiles
-    const int64_t token = q0 + my_i, qh = h * group + (row - my_i * group);
-    if (first + r32 >= n_rows || token >= a.tokens) return;
+    const int64_t token = qs.first + my_i, qh = h * group + (row - my_i * group);
+    if (first + r32 >= n_rows) return;
     const float inv = l != 0.0f ? 1.0f / l : 0.0f;
     T *out = (T *)a.out + token * a.out_token_stride + qh * a.out_head_stride;
 #pragma unroll
@@ -883,11 +891,11 @@ __global__ __launch_bounds__(256) void k_attend_join(sili_kv4_attend_args a, Att
     __shared__ float s_w[4], s_sum[GROUPS];
     const int32_t row = blockIdx.x, h = blockIdx.y, req = blockIdx.z;
     const int32_t group = pl.group;
-    const int32_t q0 = a.q_start[req], n_rows = min(a.q_start[req + 1] - q0, (int32_t)a.max_new) * group;
-    if (q0 < 0 || n_rows > pl.many || row >= n_rows) return;
+    const Queries qs = queries_of(a, req);
+    const int32_t n_rows = qs.n * group;
+    if (n_rows > pl.many || row >= n_rows) return;
     const int32_t i = token_of(pl, row);
-    const int64_t token = q0 + i, qh = h * group + (row - i * group);
-    if (token >= a.tokens) return;
+    const int64_t token = qs.first + i, qh = h * group + (row - i * group);
     const int64_t id = token * a.q_heads + qh;
     const float2 *ml = pl.part_ml + id * pl.splits;
     float m = -INFINITY;
