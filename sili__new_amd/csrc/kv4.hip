@@ -269,26 +269,35 @@ __device__ __forceinline__ void store4(T *out, const float (&x)[4], bool packed)
 // A request's query tokens: the first, how many it has, and how many of them are
 // computed: the launch and the join's LDS are sized for max_new and for the
 // batch's tokens, which q_start may pass (it does where a step brought more tokens
-// than its buffers hold).
+// than its buffers hold).  A negative start, or an end before it: none.
 struct Queries {
     int32_t first, all, n;
 };
 __device__ __forceinline__ Queries queries_of(const sili_kv4_attend_args &a, int req) {
+    const int32_t from = a.q_start[req], upto = a.q_start[req + 1];
     Queries q;
-    q.first = a.q_start[req];
-    q.all = a.q_start[req + 1] - q.first;
-    q.n = q.first < 0 ? 0 : min(q.all, min((int32_t)a.max_new, (int32_t)a.tokens - q.first));
+    q.first = max(from, 0);
+    q.all = from < 0 ? 0 : max(upto, from) - from;
+    q.n = max(0, min(q.all, min((int32_t)a.max_new, (int32_t)a.tokens - q.first)));
     return q;
 }
 
-// Keys that query i of n sees, [begin, end).
+// Keys that query i of n sees, [begin, end), both within the keys there are
+// whatever the length says.
 struct KeyRange {
     int32_t base, cap, window;  // keys before the first query, keys there are
     bool causal;
-    __device__ __forceinline__ int32_t end(int32_t i) const { return causal ? min(cap, base + i + 1) : cap; }
+    __device__ __forceinline__ KeyRange(const sili_kv4_attend_args &a, const AttendPlan &pl, const Queries &q, int req) {
+        const int32_t len = max(a.kv_lens[req], 0);
+        base = len - q.all;
+        cap = min(len, pl.most);
+        window = pl.window;
+        causal = a.causal != 0;
+    }
+    __device__ __forceinline__ int32_t end(int32_t i) const { return causal ? max(0, min(cap, base + i + 1)) : cap; }
     __device__ __forceinline__ int32_t begin(int32_t i) const {
         const int32_t upto = base + i + 1;  // negative where the query comes before the first key
-        return window > 0 && upto > window ? upto - window : 0;
+        return window > 0 && upto > window ? min(cap, upto - window) : 0;
     }
 };
 
@@ -340,19 +349,14 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_at
     if (pl.window == 0 && key + 16 * g < pl.most) page = entry(key);
 
     const Queries qs = queries_of(a, req);
-    const int32_t kv = a.kv_lens[req];
+    const KeyRange kr(a, pl, qs, req);
     const int32_t n_rows = qs.n * group;
     const int32_t first = tile * RT;
     if (n_rows > pl.many || first >= n_rows) return;
-    KeyRange kr;
-    kr.base = kv - qs.all;
-    kr.window = pl.window;
-    kr.causal = a.causal != 0;
-    kr.cap = min(kv, pl.most);
     const int32_t i_first = token_of(pl, first), i_last = token_of(pl, min(first + RT - 1, n_rows - 1));
     const int32_t lo = kr.begin(i_first) & ~63, hi = kr.end(i_last);
     const int32_t all_end = kr.end(i_first), all_begin = kr.begin(i_last);  // what every row sees
-    const int32_t c0 = lo + split * pl.chunk, c1 = c0 + min(hi - c0, pl.chunk);
+    const int32_t c1 = lo + min(hi - lo, (split + 1) * pl.chunk);
 
     uint32_t take_q[QP], take_p[PP];  // CP > 1: the part this lane's column holds
 #pragma unroll
@@ -441,7 +445,7 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_at
         for (int ct = 0; ct < CT; ++ct) vw[ct] = *reinterpret_cast<const uint4 *>(vp + ct * 256);
     };
     if (pl.window > 0) {
-        key += lo;
+        key = key < hi - lo ? lo + key : c1;
         page = page_of(key);
     }
     if (key < c1) {
@@ -645,15 +649,10 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void k_attend_many(sili_kv4_att
     const int h = blockIdx.x % H, tile = blockIdx.x / H, req = blockIdx.z;
     const int32_t *table = a.block_table + (int64_t)req * a.table_width;
     const Queries qs = queries_of(a, req);
-    const int32_t kv = a.kv_lens[req];
+    const KeyRange kr(a, pl, qs, req);
     const int32_t n_rows = qs.n * group;
     const int32_t block_first = tile * MANY_ROWS;
     if (n_rows <= pl.many || block_first >= n_rows) return;
-    KeyRange kr;
-    kr.base = kv - qs.all;
-    kr.window = pl.window;
-    kr.causal = a.causal != 0;
-    kr.cap = min(kv, pl.most);
     const int32_t c0 = kr.begin(token_of(pl, block_first)) & ~63, c1 = kr.end(token_of(pl, min(block_first + MANY_ROWS, n_rows) - 1));
 
     // this wave's rows (past the last: the last again), and this lane's
