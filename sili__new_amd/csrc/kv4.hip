@@ -988,7 +988,6 @@ void check_attend(const sili_kv4_attend_args &a) {
     require(a.cache.n_pages * (a.cache.page_size / 16) * a.cache.kv_heads <= INT32_MAX, "kv4_attend: cache too large");
     require(a.table_width >= 0 && a.max_new >= 0 && a.max_len >= 0, "kv4_attend: negative size");
     require(a.max_len <= INT32_MAX && a.max_new <= INT32_MAX && a.table_width <= INT32_MAX, "kv4_attend: bound out of range");
-    require(a.max_new * (a.q_heads / a.cache.kv_heads) <= INT32_MAX, "kv4_attend: too many rows");
     require(a.window >= 0 && (a.window == 0 || a.causal), "kv4_attend: a window needs the causal mask");
 }
 
@@ -1025,7 +1024,7 @@ Launch plan_attend(const sili_kv4_attend_args &a) {
     Launch L;
     AttendPlan &p = L.plan;
     const int64_t group = a.q_heads / a.cache.kv_heads, heads = a.requests * a.cache.kv_heads;
-    const int64_t rows = std::min(a.max_new, a.tokens) * group;  // of the longest request at most
+    const int64_t rows = std::min(a.max_new, a.tokens) * group;  // of the longest request at most; below 2^31 as tokens * q_heads is
     const int64_t gpp = a.cache.page_size / 16, es = dtype_size(a.dtype);
     p.kv_heads = (int32_t)a.cache.kv_heads;
     p.group = (int32_t)group;

@@ -46,3 +46,12 @@ def test_slots_that_leave_tokens_out_then_attention(hip):
     assert step["q_start"].cpu().tolist() == [0, 3, 9, 14]
     q = queries(14, 5, 128, torch.bfloat16, 4)
     short_batch(host, gpu, q, step["q_start"].cpu().numpy(), old + new, table, 7)
+
+
+@pytest.mark.parametrize("group", [2, 5])
+def test_the_largest_max_new(hip, group):
+    new, lens = np.array([2, 1, 3]), np.array([70, 900, 3])
+    host, gpu, table = filled(lens, 2, 16, 64, 3)
+    q = queries(6, 2 * group, 64, torch.float32, 5)
+    s = attend(gpu, q, starts(new), lens, table, max_new=(1 << 31) - 1)
+    check(host, s, starts(new), lens, table)
