@@ -568,7 +568,8 @@ int sili_memcpy_d2h_ordered(sili_layer *layer, void *dst, const void *src, size_
  * says host; strides count elements.  The calls run on `stream` (NULL: HIP's
  * default stream) of the calling thread's current device, allocate nothing,
  * wait for nothing, keep nothing between calls, and may be recorded into a
- * graph.  Sums, softmax statistics and norms are held in fp32; results are
+ * graph.  Outputs overlap neither inputs nor each other but where an entry
+ * allows it.  Sums, softmax statistics and norms are held in fp32; results are
  * rounded once, to `dtype`. */
 enum { SILI_F32 = 0, SILI_BF16 = 1, SILI_F16 = 2 };
 
@@ -584,7 +585,9 @@ enum { SILI_F32 = 0, SILI_BF16 = 1, SILI_F16 = 2 };
  * get slot -1 (which sili_kv4_append skips) and position 0.
  * status[0]: pages taken; status[1]: 0, or the sum of SILI_SLOTS_* for what
  * did not fit: a table entry without a page becomes -1 and its tokens get slot
- * -1; tokens past max_tokens are left out.  Negative lengths count as 0. */
+ * -1; tokens past max_tokens are left out (q_start and kv_lens count them all
+ * the same).  Negative lengths count as 0.  Overlapping buffers are refused:
+ * kv_lens is the next step's cached_lens, so a program keeps two and swaps them. */
 enum {
     SILI_SLOTS_NO_PAGE = 1,    /* free_pages is too short */
     SILI_SLOTS_TABLE_FULL = 2, /* a request needs more than table_width pages */

@@ -279,6 +279,27 @@ __global__ __launch_bounds__(256) void k_slots_tokens(Step s) {
     a.slots[t] = slot;
 }
 
+// Blocks read lengths, tables and pages while others write their results, so no
+// output may lie on an input or on another output.
+void check_apart(const sili_request_slots_args &a) {
+    struct Range {
+        uintptr_t begin, end;
+    };
+    auto range = [](const int32_t *p, int64_t rows, int64_t width = 1) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+        const auto bytes = (unsigned __int128)rows * (unsigned __int128)width * sizeof(int32_t);
+        return Range{at, at + (uintptr_t)std::min<unsigned __int128>(bytes, UINTPTR_MAX - at)};
+    };
+    auto meet = [](const Range &x, const Range &y) { return std::max(x.begin, y.begin) < std::min(x.end, y.end); };
+    const Range written[] = {range(a.q_start, a.requests + 1), range(a.kv_lens, a.requests), range(a.positions, a.max_tokens),
+                             range(a.slots, a.max_tokens), range(a.status, 2), range(a.block_table, a.requests, a.table_width)};
+    const Range read[] = {range(a.cached_lens, a.requests), range(a.new_lens, a.requests), range(a.free_pages, a.n_free)};
+    for (const Range &w : written) {
+        for (const Range &r : read) require(!meet(w, r), "request_slots: an output overlaps an input");
+        for (const Range &o : written) require(&o == &w || !meet(w, o), "request_slots: outputs overlap");
+    }
+}
+
 }  // namespace
 
 void request_slots(const sili_request_slots_args &a, hipStream_t st) {
@@ -292,6 +313,7 @@ void request_slots(const sili_request_slots_args &a, hipStream_t st) {
     require(a.n_free == 0 || a.free_pages, "request_slots: NULL free_pages");
     require(a.max_tokens == 0 || (a.positions && a.slots), "request_slots: NULL buffer");
     require(a.q_start && a.status, "request_slots: NULL buffer");
+    check_apart(a);
     Step s{a, -1};
     if ((a.page_size & (a.page_size - 1)) == 0) s.shift = __builtin_ctzll((unsigned long long)a.page_size);
     if (a.requests <= FEW) {
