@@ -216,7 +216,21 @@ __global__ __launch_bounds__(FEW_TPB) void k_slots_few(Step s) {
     for (int64_t i = first; i < P && i < INT32_MAX; i += step) {
         const int64_t r = owner(pag, R, i);
         const int64_t at = (int64_t)page_of(s, (uint32_t)old[r] + mask) + (i - pag[r]);
-        if (at < a.table_width) a.block_table[r * a.table_width + at] = i < a.n_free ? a.free_pages[i] : -1;
+        if (at < a.table_width) {
+            a.block_table[r * a.table_width + at] = i < a.n_free ? a.free_pages[i] : -1;
+        } else {
+            // on to the next request's pages: a length past the table may ask for 2^31
+            const int64_t left = (r + 1 < R ? (int64_t)pag[r + 1] : P) - i;
+            i += (left - 1) / step * step;
+        }
+    }
+    // pages whose number passes 31 bits: there are none
+    if (P > INT32_MAX) {
+        for (int r = mine0 + (int)threadIdx.x; r < mine1; r += FEW_TPB) {
+            const Req q = request(s, a.cached_lens[r], a.new_lens[r]);
+            const int64_t upto = min((int64_t)q.have + q.take, a.table_width);
+            for (int64_t at = (int64_t)q.have + (INT32_MAX - pag[r]); at < upto; ++at) a.block_table[r * a.table_width + at] = -1;
+        }
     }
 }
 
