@@ -106,7 +106,8 @@ class Stack:
         """Pages, slots and positions of a step that brings new[r] tokens to request r."""
         i32 = lambda n: torch.empty(n, dtype=torch.int32, device="cuda")  # noqa: E731
         n, total = len(new), sum(new)
-        old = torch.tensor(self.lens, dtype=torch.int32, device="cuda")
+        lens = self.lens + [0] * (n - len(self.lens))
+        old = torch.tensor(lens, dtype=torch.int32, device="cuda")
         fresh = torch.tensor(new, dtype=torch.int32, device="cuda")
         free = torch.tensor(self.free, dtype=torch.int32, device="cuda")
         p = dict(q_start=i32(n + 1), kv_lens=i32(n), positions=i32(total), slots=i32(total), status=i32(2))
@@ -118,7 +119,7 @@ class Stack:
         if flags:
             raise MemoryError(f"the cache or the block table is full (request_slots status {flags})")
         self.free = self.free[taken:]
-        self.lens = [a + b for a, b in zip(self.lens, new)]
+        self.lens = [a + b for a, b in zip(lens, new)]
         p.update(tokens=total, requests=n, max_new=max(new), max_len=max(self.lens))
         return p
 
@@ -153,8 +154,11 @@ class Stack:
     def step(self, tokens):
         """tokens: a list of new tokens for each request (new requests at the end).
         -> the last hidden state of every token [tokens, hidden]."""
+        if not len(self.lens) <= len(tokens) <= len(self.table):
+            raise ValueError(f"{len(tokens)} lists of tokens: one for each of {len(self.lens)} requests, and {len(self.table)} requests at most")
+        if not any(tokens):
+            raise ValueError("a step without tokens")
         with torch.cuda.stream(self.stream):
-            self.lens += [0] * (len(tokens) - len(self.lens))
             p = self.plan([len(t) for t in tokens])
             x = self.embedding[torch.tensor([i for t in tokens for i in t], device="cuda")]
             h = x * torch.rsqrt(x.square().mean(1, keepdim=True) + EPS) * self.w_first
