@@ -169,10 +169,11 @@ class Stack:
             return h
 
     def next_tokens(self, h, tokens):
-        """The most likely token after the last one of each request."""
+        """The most likely token after the last one of each request; None for one without tokens in this step."""
         with torch.cuda.stream(self.stream):
-            last = torch.tensor(np.cumsum([len(t) for t in tokens]) - 1, device="cuda")
-            return (h[last] @ self.out).argmax(1).tolist()
+            last = torch.tensor(np.cumsum([len(t) for t in tokens]) - 1, device="cuda").clamp(min=0)
+            picked = (h[last] @ self.out).argmax(1).tolist()
+        return [p if t else None for p, t in zip(picked, tokens)]
 
 
 def generate(stack, prompts, steps):

@@ -1,5 +1,7 @@
 """GPU: steps of the folded stack (examples/folded_block.py) that it cannot take
-are refused with nothing changed."""
+are refused with nothing changed, and requests that rest in a step stay out of
+its answers."""
+import numpy as np
 import pytest
 import torch
 
@@ -27,3 +29,17 @@ def test_refused_steps(hip, example):  # noqa: F811
     want = other.step([[4], [5], [6]])
     torch.cuda.synchronize()
     assert near(h.double().cpu().numpy(), want.double().cpu().numpy()) and stack.lens == [3, 2, 1]
+
+
+def test_requests_that_rest(hip, example):  # noqa: F811
+    stack = example.Stack(**SIZES)
+    tokens = [[7, 8], [], [9], []]
+    h = stack.step(tokens)
+    picked = stack.next_tokens(h, tokens)
+    assert [p is None for p in picked] == [False, True, False, True]
+    with torch.cuda.stream(stack.stream):
+        best = (h[torch.tensor([1, 1, 2, 2], device="cuda")] @ stack.out).argmax(1).tolist()
+    assert [picked[0], picked[2]] == [best[0], best[2]]
+    first = [[], [7, 8]]
+    other = example.Stack(**SIZES)
+    assert np.array_equal([p is None for p in other.next_tokens(other.step(first), first)], [True, False])
