@@ -694,7 +694,8 @@ int sili_block_norm_workspace(const sili_block_norm_args *args, size_t *bytes);
 
 /* A paged cache of keys and values in 4 bits.  Per token and kv head one fp32
  * scale amax / 6 and head_dim E2M1 codes, fp4_encode(x * (6 * (1 / amax))) in
- * fp32, the layers' own codec (nearest, ties away from zero).  A head whose amax is below
+ * fp32, each operation rounded (the factor so, and not as 6 / amax), the layers'
+ * own codec (nearest, ties away from zero).  A head whose amax is below
  * 2^-120 is stored as zeros; one with a NaN or an infinity gets a NaN scale and
  * reads as NaN.  Bytes hold channel 2b in the low and 2b + 1 in the high
  * nibble:
@@ -735,11 +736,20 @@ int sili_kv4_read(const sili_kv4_rows_args *args, void *stream);
  * max_new and max_len bound the requests' query tokens and key counts (host
  * values; they size the grid): queries past max_new are not computed, keys past
  * max_len not seen.  A table entry outside the cache hides its page's keys.
- * Products run on the bf16 matrix cores: the codes are exact there, q and the
- * softmax weights enter in as many bf16 parts as their type has bits (fp32 three,
- * f16 two, bf16 one or two), and sums are fp32.  workspace: device memory of
- * sili_kv4_attend_workspace(args) bytes, 16-byte aligned; calls that overlap
- * need one each. */
+ * Whatever q_start, kv_lens and block_table hold, the call stays within its
+ * buffers: queries past `tokens` are not computed, a negative length counts as 0,
+ * a negative start or an end before it as no queries.  A window of 2^31 - 1 or
+ * more is none.
+ * Products run on the bf16 matrix cores and sums are fp32.  The codes are exact
+ * there; q enters in as many bf16 parts as its type has bits (fp32 three, f16
+ * two, bf16 one), a softmax weight in three (fp32) or two (f16, bf16).  bf16
+ * weights enter in one part, rounded to 8 bits as the output is, for requests of
+ * more than 256 rows (query tokens x query heads a kv head) at head_dim 128 in
+ * calls with 512 blocks of 128 such rows or more (requests x kv_heads x
+ * ceil(rows of the longest request / 128)): the error against exact arithmetic
+ * is 1.4 times that of the output's own rounding there.  workspace: device
+ * memory of sili_kv4_attend_workspace(args) bytes, 16-byte aligned; calls that
+ * overlap need one each. */
 typedef struct {
     sili_kv4_cache cache;
     int32_t dtype, causal;

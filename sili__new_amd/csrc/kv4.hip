@@ -20,12 +20,15 @@ __device__ __forceinline__ float wave_max(float v) {
 }
 
 // ---- rows ------------------------------------------------------------------------
-// Bound by memory: 4.25 bits stored a channel beside the row's own. A thread takes
+// 4.25 bits stored a channel beside the row's own. A thread takes
 // 8 channels of a (token, kv head), k's and v's: 16 or 32 bytes a load, a dword of
 // k codes, four bytes of v codes.  The bytes of 16 tokens share their 16-byte runs
 // of v codes, so a block takes one head of as many tokens as its threads cover:
 // their bytes meet in one L2 (a block of one token's heads, whose neighbours run on
-// other XCDs, wrote 2048 tokens of 40 fp32 heads in 42 us; so, 30, and 27 read).
+// other XCDs, wrote 2048 tokens of 40 fp32 heads in 42 us; so, 29, and 30 read).
+// Writing is bound by the codec's arithmetic (vector units 88 % busy, 526
+// instructions for 16 channels; 3.3 TB/s), reading back by neither it (53 %) nor
+// the bytes (3.2 TB/s): short waves that wait for their codes, then for their stores.
 constexpr int ROWS_TPB = 256;
 
 // Maximum over the aligned group of N lanes.
@@ -46,7 +49,11 @@ __device__ __forceinline__ void load8(const T *p, bool packed, float (&x)[8]) {
     }
 }
 
-// Codes of eight channels (channel j in nibble j), and the head's scale.
+// Codes of eight channels (channel j in nibble j), and the head's scale.  The factor
+// is 6 * (1 / amax), rounded twice: within 2^-23 of 6 / amax, so a code is another
+// than the exact quotient's only where that lies as near to the middle of two levels
+// (25 of the 122944 pairs of bf16 values within 8 octaves of amax; of 6 / amax 10).  It is
+// the format's definition, so that codes are equal wherever they are computed so.
 template <int N>
 __device__ __forceinline__ uint32_t encode8(const float (&x)[8], float &scale) {
     float top = 0.0f, sum = 0.0f;
@@ -618,11 +625,14 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_at
 // order 0-3, 8-11, 4-7, 12-15 of every 16: eight at 16 s + 8 hf are the lane's
 // own.  Rows of LDS are padded by 16 bytes, which spreads eight lanes' 16 bytes
 // over all banks.  A weight enters in one bf16 part: its rounding is as large as
-// the output's own, together 1.4 times that, and a second part would be half as
-// many products again.  Half of a step's scores are scaled under the products of
-// the other half, and the weights of 16 keys are taken under the products of the 16
-// before; without, the wave's vector work and its products take turns (2 x 2047
-// tokens of 40 heads under a window of 4096: 455 us, with it 434, 0.75 PFLOP/s).
+// the output's own, together 1.4 times that (2 x 2047 tokens: 0.0023 of the output's
+// norm off against 0.0017); a second part is half as many products again (532 us
+// against 428).  The sum l takes the weights unrounded.  Half of a step's scores
+// are scaled under the products of the other half, and the weights of 16 keys are
+// taken under the products of the 16 before; without, the wave's vector work and
+// its products take turns (2 x 2047 tokens of 40 heads under a window of 4096: 455
+// us, with it 430, 0.75 PFLOP/s, at 2.38 GHz; a card that idled begins at 2.06 GHz
+// and takes 500).
 // Issue bounds it, with a last round of blocks that leaves half of their places empty.
 constexpr int MANY_WAVES = 4, MANY_ROWS = 32 * MANY_WAVES;
 
@@ -1046,9 +1056,10 @@ Launch plan_attend(const sili_kv4_attend_args &a) {
     // heads of 5 query heads each, chunks at the end of 4096 keys more, us of it and of
     // the other: 1280 blocks 452 and 625, 768 276 and 310, 640 214 and 258, 384 146 and
     // 152, 320 204 and 197 or 151 and 128, 160 142 and 104), in bf16 and at its
-    // head_dim; of fp32 and f16 (2 x 2047 tokens: 1200 and 1013, 873 and 743) and of
-    // head_dim 64 and 256 (1 x 1024: 133 and 98, 394 and 276) a like kernel was slower
-    // everywhere.  192 rows of 2048 keys took 33 us in the few-rows kernel, 51 in the
+    // head_dim.  For fp32 and f16 a like kernel was slower at 1280 blocks (2 x 2047
+    // tokens: 1200 and 1013, 873 and 743).  For head_dim 64 and 256 one was tried at 320
+    // blocks only (133 and 98, 394 and 276), where that of 128 loses too: what it would
+    // do at 512 and more is not known.  192 rows of 2048 keys took 33 us in the few-rows kernel, 51 in the
     // other.
     constexpr int64_t FEW_ROWS = 256;
     const int64_t many_tiles = (rows + MANY_ROWS - 1) / MANY_ROWS;

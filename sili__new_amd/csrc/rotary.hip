@@ -2,7 +2,9 @@
 //
 // Pair i of a head at position p turns by the angle p * step_i, in turns of
 // 2^64: the product wraps modulo one turn, so the fraction keeps its accuracy
-// at any position (32 bits of it are used, 1.5e-9 rad).  Bound by memory: each
+// at any position.  Its upper 32 bits, as a signed part of half a turn, become a
+// float: within 2^-25 of half a turn (9.4e-8 rad) at the largest angles, 1.5e-9 rad
+// at small ones, where sines and cosines are fp32 anyway.  Bound by memory: each
 // element is read and written once.  A thread owns one run of pairs of a token,
 // 16 bytes, takes its sines and cosines once and walks heads with them, four in
 // flight (8192 tokens of 48 bf16 heads of 128, half of each turned: 44 us, 4.6 TB/s;
