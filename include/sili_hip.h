@@ -770,6 +770,131 @@ typedef struct {
 int sili_kv4_attend(const sili_kv4_attend_args *args, void *stream);
 int sili_kv4_attend_workspace(const sili_kv4_attend_args *args, size_t *bytes);
 
+/* ---- drafted tokens ------------------------------------------------------
+ * A step may check several guesses of a request's continuation at once: its new
+ * tokens form a tree, token i following token parents[i] of the same request
+ * (an earlier one, 0 <= parents[i] < i) or, at -1, the request's last cached
+ * token.  At most SILI_TREE_MOST of them a request. */
+enum { SILI_TREE_MOST = 64 };
+
+/* Who descends from whom.  Bit j of ancestors[t], t = q_start[r] + i, is set
+ * where j is i or one that token i descends from; positions[t] = cached_lens[r]
+ * + the number of those - 1 (at most 2^31 - 1), for sili_rotary: the
+ * positions of sili_request_slots count a request's new tokens one after
+ * another.  A parent that is no earlier token of the request counts as -1, a
+ * negative cached length as 0.  max_new (host, at most SILI_TREE_MOST) bounds
+ * the requests' tokens; what q_start holds past it or past `tokens` is left as
+ * it was, as are rows of no request.  Overlapping buffers are refused. */
+typedef struct {
+    const int32_t *parents;     /* [tokens] */
+    const int32_t *q_start;     /* [requests + 1] */
+    const int32_t *cached_lens; /* [requests] */
+    int64_t requests, tokens, max_new;
+    uint64_t *ancestors;        /* [tokens] */
+    int32_t *positions;         /* [tokens] */
+} sili_draft_tree_args;
+int sili_draft_tree(const sili_draft_tree_args *args, void *stream);
+
+/* sili_kv4_attend for such trees.  With n the request's new tokens and base =
+ * kv_lens[r] - n, a query sees the keys before base and key base + j for every
+ * bit j < n of its mask ancestors[t] [tokens] -- any mask, a tree's or not; with
+ * window > 0 the last `window` of those keys.  args as there, `causal` set and
+ * max_new at most SILI_TREE_MOST (ValueError otherwise); workspace of
+ * sili_kv4_attend_tree_workspace(args) bytes. */
+int sili_kv4_attend_tree(const sili_kv4_attend_args *args, const uint64_t *ancestors, void *stream);
+int sili_kv4_attend_tree_workspace(const sili_kv4_attend_args *args, size_t *bytes);
+
+/* ---- dense weights in 4 bits ---------------------------------------------
+ * n_out rows of n_in E2M1 codes (the layers' codec), input 2b in the low and
+ * 2b + 1 in the high nibble of byte b, and a scale a group of `group` inputs
+ * (32, 64 or 128; n_in is a multiple of it) in scale_dtype: weight = scale *
+ * code.  Code 8, which the codec never gives, counts as 0.  codes 16-byte
+ * aligned, codes_stride (bytes a row) a multiple of 16; scales_stride counts
+ * elements. */
+typedef struct {
+    uint8_t *codes;
+    void *scales;
+    int64_t n_out, n_in, group, codes_stride, scales_stride;
+    int32_t scale_dtype;
+} sili_fp4_weights;
+
+/* Weights from rows [n_out][n_in] of `dtype`: scale = amax / 6 of the group,
+ * rounded to scale_dtype, codes fp4_encode(x * (1 / scale)) in fp32.  A group
+ * whose scale rounds to less than 2^-120 is stored as zeros; one with a NaN or
+ * an infinity, or whose scale is past scale_dtype, gets a NaN scale. */
+typedef struct {
+    sili_fp4_weights w;
+    int32_t dtype;
+    const void *rows;
+    int64_t row_stride;
+} sili_fp4_pack_args;
+int sili_fp4_pack(const sili_fp4_pack_args *args, void *stream);
+
+/* y[t][n] = sum over the groups of scale * (sum of code * x[t]), x [tokens]
+ * [n_in] of `dtype`, y [tokens][n_out] of out_dtype.  Any number of tokens; the
+ * weights are read once for up to 16 of them.  x enters the bf16 matrix cores
+ * in as many parts as its type has bits (fp32 three, f16 two, bf16 one), sums
+ * are fp32: the result is that of fp32 arithmetic.  An x that is not finite
+ * makes its own row NaN.  workspace: device memory of
+ * sili_fp4_linear_workspace(args) bytes, 16-byte aligned; calls that overlap
+ * need one each.  The same call gives the same bits. */
+typedef struct {
+    sili_fp4_weights w;
+    int32_t dtype, out_dtype;
+    int64_t tokens;
+    const void *x;
+    int64_t x_stride;
+    void *y;
+    int64_t y_stride;
+    void *workspace;
+    size_t workspace_bytes;
+} sili_fp4_linear_args;
+int sili_fp4_linear(const sili_fp4_linear_args *args, void *stream);
+int sili_fp4_linear_workspace(const sili_fp4_linear_args *args, size_t *bytes);
+
+/* ---- constraints on logits -----------------------------------------------
+ * Penalties for repeated tokens, biases and grammar masks on logits [rows]
+ * [vocab], before a token is chosen.  Request r's rows are q_start[r] ..
+ * q_start[r + 1] - 1 (q_start NULL: row r alone).  Its past is the first
+ * history_lens[r] entries of its history row and, for the row of a drafted
+ * token, the tokens of its own path: tokens[q_start[r] + j] for the bits j of
+ * ancestors[row] (both NULL: none).  With n how often v occurs on the path and
+ * in the history from entry counted_from[r] on (NULL: 0), and "past" whether it
+ * occurs at all:
+ *     past:   z = z > 0 ? z / repetition[r] : z * repetition[r]
+ *     n > 0:  z = z - (frequency[r] n + presence[r])
+ *     z = z + bias[v]           (of request r, or one for all: bias_stride 0)
+ *     z = -infinity             (bit v % 32 of word v / 32 of the row's mask is 0)
+ * in fp32, rounded once to `dtype`.  A row's mask is row allow_row[row] of
+ * allow [n_allow][allow_stride words] (allow_row NULL: row `row`); outside 0 ..
+ * n_allow - 1: no mask.  A mask without a bit leaves a row of -infinity.  Each
+ * of history, the penalties, bias and allow may be NULL.  Tokens outside the
+ * vocabulary count nowhere, bits of ancestors past the request neither; lengths
+ * are cut to their buffers.  out may be logits (same strides), and overlaps it
+ * not otherwise; rows of no request are left as they were. */
+typedef struct {
+    int32_t dtype;
+    int64_t rows, vocab, requests;
+    const void *logits;
+    int64_t logits_stride;
+    void *out;
+    int64_t out_stride;
+    const int32_t *q_start;      /* [requests + 1] */
+    const int32_t *history;      /* [requests][history_stride] */
+    const int32_t *history_lens; /* [requests] */
+    int64_t history_stride;
+    const int32_t *counted_from; /* [requests] */
+    const int32_t *tokens;       /* [rows] */
+    const uint64_t *ancestors;   /* [rows] */
+    const float *repetition, *presence, *frequency; /* [requests] */
+    const float *bias;           /* [vocab] or [requests][bias_stride] */
+    int64_t bias_stride;
+    const uint32_t *allow;
+    const int32_t *allow_row;    /* [rows] */
+    int64_t allow_stride, n_allow;
+} sili_logits_constrain_args;
+int sili_logits_constrain(const sili_logits_constrain_args *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -30,7 +30,7 @@ ARCH = os.environ.get("SILI_OFFLOAD_ARCH", "gfx950")
 
 HIP_SOURCES = ["kernels.hip", "stream.hip", "build.hip", "synapto.hip", "policy.hip", "gen.hip", "train.hip",
                "csr_util.hip", "for_index.hip", "tile_enc.hip", "layout.hip", "b4res.hip", "push.hip", "patch.hip", "staged.hip", "mfma24.hip",
-               "slots.hip", "rotary.hip", "block_norm.hip", "kv4.hip", "capi.hip"]
+               "slots.hip", "rotary.hip", "block_norm.hip", "kv4.hip", "draft.hip", "fp4_linear.hip", "logits.hip", "capi.hip"]
 
 HIP_FLAGS = [
     "-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}",

@@ -1,9 +1,12 @@
 // block_ops.hpp -- the operators between the layers (request slots, rotary
-// positions, block norms, the 4-bit cache): launchers, element types, checks.
+// positions, block norms, the 4-bit cache) and of a step over drafted tokens
+// (trees, 4-bit weights, constraints on logits): launchers, element types, checks.
 #pragma once
 
 #include "../../include/sili_hip.h"
 #include "common.hpp"
+
+#include <algorithm>
 
 namespace sili {
 
@@ -18,12 +21,28 @@ void kv4_append(const sili_kv4_rows_args &a, hipStream_t st);
 void kv4_read(const sili_kv4_rows_args &a, hipStream_t st);
 void kv4_attend(const sili_kv4_attend_args &a, hipStream_t st);
 size_t kv4_attend_workspace(const sili_kv4_attend_args &a);
+void draft_tree(const sili_draft_tree_args &a, hipStream_t st);
+void kv4_attend_tree(const sili_kv4_attend_args &a, const uint64_t *ancestors, hipStream_t st);
+size_t kv4_attend_tree_workspace(const sili_kv4_attend_args &a);
+void fp4_pack(const sili_fp4_pack_args &a, hipStream_t st);
+void fp4_linear(const sili_fp4_linear_args &a, hipStream_t st);
+size_t fp4_linear_workspace(const sili_fp4_linear_args &a);
+void logits_constrain(const sili_logits_constrain_args &a, hipStream_t st);
 
 // Raises SILI_ERR_INVALID with `what` unless ok.
 inline void require(bool ok, const char *what) {
     if (!ok) throw_error(SILI_ERR_INVALID, what);
 }
 inline bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+// The bytes a contiguous buffer takes, and whether two have one in common.
+struct Span {
+    uintptr_t begin, end;
+};
+inline Span span(const void *p, int64_t bytes) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    return {at, at + std::min<uintptr_t>((uintptr_t)bytes, UINTPTR_MAX - at)};
+}
+inline bool meet(const Span &x, const Span &y) { return std::max(x.begin, y.begin) < std::min(x.end, y.end); }
 
 // Element types of activations.  The conversions of __bf16 and _Float16 round
 // to nearest even and keep NaN and infinities.

@@ -1869,6 +1869,55 @@ int sili_kv4_attend_workspace(const sili_kv4_attend_args *args, size_t *bytes) {
     });
 }
 
+int sili_draft_tree(const sili_draft_tree_args *args, void *stream) {
+    return guarded([&] {
+        if (!args) throw_error(SILI_ERR_INVALID, "draft_tree: NULL arguments");
+        draft_tree(*args, reinterpret_cast<hipStream_t>(stream));
+    });
+}
+
+int sili_kv4_attend_tree(const sili_kv4_attend_args *args, const uint64_t *ancestors, void *stream) {
+    return guarded([&] {
+        if (!args) throw_error(SILI_ERR_INVALID, "kv4_attend_tree: NULL arguments");
+        kv4_attend_tree(*args, ancestors, reinterpret_cast<hipStream_t>(stream));
+    });
+}
+
+int sili_kv4_attend_tree_workspace(const sili_kv4_attend_args *args, size_t *bytes) {
+    return guarded([&] {
+        if (!args || !bytes) throw_error(SILI_ERR_INVALID, "kv4_attend_tree_workspace: NULL arguments");
+        *bytes = kv4_attend_tree_workspace(*args);
+    });
+}
+
+int sili_fp4_pack(const sili_fp4_pack_args *args, void *stream) {
+    return guarded([&] {
+        if (!args) throw_error(SILI_ERR_INVALID, "fp4_pack: NULL arguments");
+        fp4_pack(*args, reinterpret_cast<hipStream_t>(stream));
+    });
+}
+
+int sili_fp4_linear(const sili_fp4_linear_args *args, void *stream) {
+    return guarded([&] {
+        if (!args) throw_error(SILI_ERR_INVALID, "fp4_linear: NULL arguments");
+        fp4_linear(*args, reinterpret_cast<hipStream_t>(stream));
+    });
+}
+
+int sili_fp4_linear_workspace(const sili_fp4_linear_args *args, size_t *bytes) {
+    return guarded([&] {
+        if (!args || !bytes) throw_error(SILI_ERR_INVALID, "fp4_linear_workspace: NULL arguments");
+        *bytes = fp4_linear_workspace(*args);
+    });
+}
+
+int sili_logits_constrain(const sili_logits_constrain_args *args, void *stream) {
+    return guarded([&] {
+        if (!args) throw_error(SILI_ERR_INVALID, "logits_constrain: NULL arguments");
+        logits_constrain(*args, reinterpret_cast<hipStream_t>(stream));
+    });
+}
+
 int sili_rotary_steps(int64_t rot_dim, double base, int scaling, double factor, double original_len, double low,
                       double high, uint64_t *steps, float *scale) {
     return guarded([&] {

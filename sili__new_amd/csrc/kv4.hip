@@ -4,6 +4,7 @@
 // A stored head is scale * code[c], code an E2M1 value; its scale is amax / 6,
 // so the largest element takes the largest level.
 #include "block_ops.hpp"
+#include "mma.hpp"
 #include "wave.hpp"
 
 #include <algorithm>
@@ -151,32 +152,6 @@ __global__ __launch_bounds__(ROWS_TPB) void k_kv4_rows(sili_kv4_rows_args a, boo
 // argument 8): until then weights stay below 2^8 and nothing has to be rescaled.
 constexpr float SLACK = 8.0f;
 
-typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
-typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
-typedef __attribute__((ext_vector_type(2))) float f32x2;
-typedef __attribute__((ext_vector_type(4))) float f32x4;
-typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
-
-typedef __attribute__((ext_vector_type(16))) float f32x16;
-
-__device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){x, y}, bf16x2));
-}
-__device__ __forceinline__ float bf16_lo(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
-__device__ __forceinline__ float bf16_hi(uint32_t w) { return __builtin_bit_cast(float, w & 0xFFFF0000u); }
-// Two codes (byte SEL of w) to bf16.
-template <int SEL>
-__device__ __forceinline__ uint32_t codes(uint32_t w) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, SEL));
-}
-// Eight codes of a dword: eight consecutive channels.
-__device__ __forceinline__ u32x4 codes8(uint32_t w) { return (u32x4){codes<0>(w), codes<1>(w), codes<2>(w), codes<3>(w)}; }
 // Four keys of a channel pair (a dword of V) to the even and the odd channel.
 __device__ __forceinline__ void codes_by_channel(uint32_t w, uint32_t (&even)[2], uint32_t (&odd)[2]) {
     const uint32_t a = codes<0>(w), b = codes<1>(w), c = codes<2>(w), d = codes<3>(w);
@@ -201,31 +176,9 @@ __device__ __forceinline__ float lanes_sum(float v) {
     return v + __shfl_xor(v, 32, 64);
 }
 
-// bf16 parts of q: 24 bits of fp32, all 11 of f16, all 8 of bf16.
-template <typename T>
-constexpr int q_parts() { return sizeof(T) == 4 ? 3 : __is_same(T, __bf16) ? 1 : 2; }
-// ... of p: 24 bits for fp32, 16 for f16 and bf16.
+// bf16 parts of p: 24 bits for fp32, 16 for f16 and bf16.
 template <typename T>
 constexpr int p_parts() { return sizeof(T) == 4 ? 3 : 2; }
-// x, y in N parts: part k the bf16 nearest to what the parts before leave.
-template <int N>
-__device__ __forceinline__ void split_bf16(float x, float y, uint32_t (&part)[N]) {
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-        part[k] = pack_bf16(x, y);
-        x -= bf16_lo(part[k]);
-        y -= bf16_hi(part[k]);
-    }
-}
-
-// The part of this lane's column: take[k] is all ones for part k's columns.
-template <int N>
-__device__ __forceinline__ uint32_t pick(const uint32_t (&part)[N], const uint32_t (&take)[N]) {
-    uint32_t w = part[0] & take[0];
-#pragma unroll
-    for (int k = 1; k < N; ++k) w |= part[k] & take[k];
-    return w;
-}
 // Sum over the CP columns of a row, 16 / CP lanes apart in their 16.
 template <int CP>
 __device__ __forceinline__ float columns_sum(float v) {
@@ -250,6 +203,7 @@ struct AttendPlan {
     int32_t many;             // the most rows of a request for the few-rows kernel; more: the other
     float c;                  // |scale| log2(e)
     bool negative;            // scale < 0: the sign goes to q
+    const uint64_t *ancestors;  // trees: the new tokens that a token sees
     float *part_o;            // [tokens * q_heads][splits][D], unnormalised
     float2 *part_ml;          // [tokens * q_heads][splits]: m c, l
 };
@@ -308,6 +262,35 @@ struct KeyRange {
     }
 };
 
+// What a drafted token sees: the keys [begin, context) before the request's new
+// tokens, and base + j for the bits j of mask.  A window drops the earliest.
+struct TreeRange {
+    int32_t base, cap, window, all;
+    __device__ __forceinline__ TreeRange(const KeyRange &kr, const Queries &q) : base(kr.base), cap(kr.cap), window(kr.window), all(q.all) {}
+    __device__ __forceinline__ int32_t context() const { return max(0, min(base, cap)); }
+    // of all of a request's tokens: no key before, none from, the keys that every one sees
+    __device__ __forceinline__ int32_t first() const { return window > 0 ? max(0, context() - window) : 0; }
+    __device__ __forceinline__ int32_t last() const { return min(cap, context() + SILI_TREE_MOST); }
+    __device__ __forceinline__ int32_t all_first() const {
+        return window > 0 ? (int32_t)max((int64_t)0, min((int64_t)cap, (int64_t)base + SILI_TREE_MOST - window)) : 0;
+    }
+    __device__ __forceinline__ int32_t of(uint64_t &mask) const {  // begin; cuts the mask
+        mask &= all < SILI_TREE_MOST ? (uint64_t(1) << max(all, 0)) - 1 : ~uint64_t(0);
+        if (window <= 0) return 0;
+        int32_t n = __popcll(mask);
+        const int64_t from = (int64_t)base + n - window;
+        for (; n > window; --n) mask &= mask - 1;
+        return (int32_t)max((int64_t)0, min((int64_t)cap, from));
+    }
+};
+// Bit j (of 16): the row sees key at + j.
+__device__ __forceinline__ uint32_t seen16(const TreeRange &tr, int32_t begin, uint64_t mask, int32_t at) {
+    auto below = [](int32_t n) { return n >= 16 ? 0xFFFFu : n > 0 ? (1u << n) - 1u : 0u; };
+    const int32_t off = at - tr.base;  // of the mask's bits
+    const uint32_t drafted = off >= SILI_TREE_MOST || off <= -16 ? 0u : (uint32_t)(off >= 0 ? mask >> off : mask << -off);
+    return ((below(tr.context() - at) & ~below(begin - at)) | drafted) & below(tr.cap - at);
+}
+
 // Registers allow this many waves on a SIMD without spilling.
 template <typename T, int D, int CP>
 constexpr int waves_per_simd() {
@@ -329,7 +312,10 @@ constexpr int waves_per_simd() {
 // holds part k of row r.  Scores are summed over a row's columns (rotations
 // within 16 lanes), so every one of them holds the row's weights and takes its
 // own part of them; the outputs are summed once, at the end.
-template <typename T, int D, int WAVES, int CP>
+//
+// TREE: rows are drafted tokens, which see the context and their ancestors.  Steps
+// before the new tokens are as without; the last one or two take a bit a key.
+template <typename T, int D, int WAVES, int CP, bool TREE>
 __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_attend_few(sili_kv4_attend_args a, AttendPlan pl) {
     constexpr int QP = q_parts<T>(), PP = p_parts<T>();
     constexpr int KS = D / 32;   // steps of 32 channels
@@ -361,8 +347,10 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_at
     const int32_t first = tile * RT;
     if (n_rows > pl.many || first >= n_rows) return;
     const int32_t i_first = token_of(pl, first), i_last = token_of(pl, min(first + RT - 1, n_rows - 1));
-    const int32_t lo = kr.begin(i_first) & ~63, hi = kr.end(i_last);
-    const int32_t all_end = kr.end(i_first), all_begin = kr.begin(i_last);  // what every row sees
+    const TreeRange tr(kr, qs);
+    const int32_t lo = (TREE ? tr.first() : kr.begin(i_first)) & ~63, hi = TREE ? tr.last() : kr.end(i_last);
+    // what every row sees
+    const int32_t all_end = TREE ? tr.context() : kr.end(i_first), all_begin = TREE ? tr.all_first() : kr.begin(i_last);
     const int32_t c1 = lo + min(hi - lo, (split + 1) * pl.chunk);
 
     uint32_t take_q[QP], take_p[PP];  // CP > 1: the part this lane's column holds
@@ -373,7 +361,8 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_at
 
     // this lane's rows
     const int32_t my_i = token_of(pl, min(first + my_row, n_rows - 1));
-    const int32_t end = kr.end(my_i), begin = kr.begin(my_i);
+    uint64_t my_mask = TREE ? pl.ancestors[qs.first + my_i] : 0;
+    const int32_t end = kr.end(my_i), begin = TREE ? tr.of(my_mask) : kr.begin(my_i);
     u32x4 q[KS][QM];
     {
         const int32_t row = min(first + my_row, n_rows - 1), i = my_i;
@@ -489,11 +478,18 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_at
             if (QP > 1) v[j] = columns_sum<CP>(v[j]);
         }
         times_scales(v, ks);
+        uint32_t seen = 0;
         if (!whole) {
-            int32_t from = here ? begin - (key + 16 * g) : 16, to = end - (key + 16 * g);
-            stay_branch(from, to);
+            if constexpr (TREE) {
+                seen = here ? seen16(tr, begin, my_mask, key + 16 * g) : 0u;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = j >= from && j < to ? v[j] : -INFINITY;
+                for (int j = 0; j < 16; ++j) v[j] = (seen & (1u << j)) != 0 ? v[j] : -INFINITY;
+            } else {
+                int32_t from = here ? begin - (key + 16 * g) : 16, to = end - (key + 16 * g);
+                stay_branch(from, to);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] = j >= from && j < to ? v[j] : -INFINITY;
+            }
         }
         float top = v[0];
 #pragma unroll
@@ -522,10 +518,15 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_at
         times_scales(w, vs);
         if (!whole) {
             // a key that this row does not see may hold anything
-            int32_t from = here ? begin - (key + 16 * g) : 16, to = end - (key + 16 * g);
-            stay_branch(from, to);
+            if constexpr (TREE) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) w[j] = j >= from && j < to ? w[j] : 0.0f;
+                for (int j = 0; j < 16; ++j) w[j] = (seen & (1u << j)) != 0 ? w[j] : 0.0f;
+            } else {
+                int32_t from = here ? begin - (key + 16 * g) : 16, to = end - (key + 16 * g);
+                stay_branch(from, to);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) w[j] = j >= from && j < to ? w[j] : 0.0f;
+            }
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e)
@@ -988,8 +989,8 @@ void rows(const sili_kv4_rows_args &a, hipStream_t st, const char *what) {
     SILI_HIP(hipGetLastError());
 }
 
-void check_attend(const sili_kv4_attend_args &a) {
-    check_cache(a.cache, "kv4_attend");
+void check_attend(const sili_kv4_attend_args &a, bool tree) {
+    check_cache(a.cache, tree ? "kv4_attend_tree" : "kv4_attend");
     require(a.dtype == SILI_F32 || a.dtype == SILI_BF16 || a.dtype == SILI_F16, "kv4_attend: unknown dtype");
     require(a.requests >= 0 && a.requests <= 65535, "kv4_attend: requests out of range");
     require(a.tokens >= 0 && a.tokens < (int64_t(1) << 31), "kv4_attend: tokens out of range");
@@ -999,6 +1000,7 @@ void check_attend(const sili_kv4_attend_args &a) {
     require(a.table_width >= 0 && a.max_new >= 0 && a.max_len >= 0, "kv4_attend: negative size");
     require(a.max_len <= INT32_MAX && a.max_new <= INT32_MAX && a.table_width <= INT32_MAX, "kv4_attend: bound out of range");
     require(a.window >= 0 && (a.window == 0 || a.causal), "kv4_attend: a window needs the causal mask");
+    require(!tree || (a.causal && a.max_new <= SILI_TREE_MOST), "kv4_attend_tree: not causal, or max_new is past SILI_TREE_MOST");
 }
 
 }  // namespace
@@ -1030,7 +1032,7 @@ struct Launch {
     AttendPlan plan{};
 };
 
-Launch plan_attend(const sili_kv4_attend_args &a) {
+Launch plan_attend(const sili_kv4_attend_args &a, bool tree) {
     Launch L;
     AttendPlan &p = L.plan;
     const int64_t group = a.q_heads / a.cache.kv_heads, heads = a.requests * a.cache.kv_heads;
@@ -1063,7 +1065,7 @@ Launch plan_attend(const sili_kv4_attend_args &a) {
     // other.
     constexpr int64_t FEW_ROWS = 256;
     const int64_t many_tiles = (rows + MANY_ROWS - 1) / MANY_ROWS;
-    if (a.dtype == SILI_BF16 && a.cache.head_dim == MANY_D && rows > FEW_ROWS && heads * many_tiles >= 512) L.many_tiles = many_tiles;
+    if (!tree && a.dtype == SILI_BF16 && a.cache.head_dim == MANY_D && rows > FEW_ROWS && heads * many_tiles >= 512) L.many_tiles = many_tiles;
     p.many = L.many_tiles ? (int32_t)FEW_ROWS : INT32_MAX;
 
     const int parts = a.dtype == SILI_F32 ? 4 : 2;
@@ -1074,7 +1076,7 @@ Launch plan_attend(const sili_kv4_attend_args &a) {
     p.join_rows = (int32_t)std::min(tile_rows, rows);
     // keys a row tile can reach: its rows' windows, aligned to 64
     int64_t reach = p.most;
-    if (p.window > 0) reach = std::min(reach, p.window + (tile_rows - 1) / group + 1 + 63);
+    if (p.window > 0) reach = std::min<int64_t>(reach, int64_t(p.window) + (tree ? SILI_TREE_MOST : (tile_rows - 1) / group + 1) + 63);
     const int64_t blocks = std::max<int64_t>(1, heads * L.tiles);
     // few blocks: as many waves in one as a CU holds, so that fewer splits are left
     // to join (40 heads of 131071 keys, 8 blocks a split: 31 + 5 us against 31 + 7
@@ -1097,7 +1099,7 @@ size_t part_bytes(const sili_kv4_attend_args &a, const AttendPlan &p) {
     return (size_t)a.tokens * (size_t)a.q_heads * (size_t)p.splits * ((size_t)a.cache.head_dim * sizeof(float) + sizeof(float2));
 }
 
-template <typename T, int D>
+template <typename T, int D, bool TREE>
 void run_few(const sili_kv4_attend_args &a, const Launch &L, hipStream_t st) {
     AttendPlan p = L.plan;
     constexpr int PARTS = sizeof(T) == 4 ? 4 : 2;
@@ -1107,11 +1109,11 @@ void run_few(const sili_kv4_attend_args &a, const Launch &L, hipStream_t st) {
     const dim3 grid((unsigned)(L.tiles * a.cache.kv_heads), (unsigned)p.splits, (unsigned)a.requests), block(64 * p.waves);
     const uint32_t lds = p.waves * p.join_rows * (D + 2) * sizeof(float);
     if (p.columns > 1) {
-        if (p.waves == WIDE_P) launch(k_attend_few<T, D, WIDE_P, PARTS>, grid, block, lds, st, a, p);
-        else launch(k_attend_few<T, D, 4, PARTS>, grid, block, lds, st, a, p);
+        if (p.waves == WIDE_P) launch(k_attend_few<T, D, WIDE_P, PARTS, TREE>, grid, block, lds, st, a, p);
+        else launch(k_attend_few<T, D, 4, PARTS, TREE>, grid, block, lds, st, a, p);
     } else {
-        if (p.waves == WIDE) launch(k_attend_few<T, D, WIDE, 1>, grid, block, lds, st, a, p);
-        else launch(k_attend_few<T, D, 4, 1>, grid, block, lds, st, a, p);
+        if (p.waves == WIDE) launch(k_attend_few<T, D, WIDE, 1, TREE>, grid, block, lds, st, a, p);
+        else launch(k_attend_few<T, D, 4, 1, TREE>, grid, block, lds, st, a, p);
     }
     if (p.splits > 1)
         launch(k_attend_join<T, D>, dim3((unsigned)L.rows, (unsigned)a.cache.kv_heads, (unsigned)a.requests), dim3(256), 0, st, a, p);
@@ -1120,16 +1122,26 @@ void run_few(const sili_kv4_attend_args &a, const Launch &L, hipStream_t st) {
 }  // namespace
 
 size_t kv4_attend_workspace(const sili_kv4_attend_args &a) {
-    check_attend(a);
-    return part_bytes(a, plan_attend(a).plan);
+    check_attend(a, false);
+    return part_bytes(a, plan_attend(a, false).plan);
 }
 
-void kv4_attend(const sili_kv4_attend_args &a, hipStream_t st) {
-    check_attend(a);
+size_t kv4_attend_tree_workspace(const sili_kv4_attend_args &a) {
+    check_attend(a, true);
+    return part_bytes(a, plan_attend(a, true).plan);
+}
+
+namespace {
+
+template <bool TREE>
+void attend(const sili_kv4_attend_args &a, const uint64_t *ancestors, hipStream_t st) {
+    check_attend(a, TREE);
     if (a.tokens == 0 || a.requests == 0 || a.max_new == 0) return;
     require(a.q && a.out && a.q_start && a.kv_lens, "kv4_attend: NULL buffer");
     require(a.block_table || a.table_width == 0, "kv4_attend: NULL block_table");
-    const Launch L = plan_attend(a);
+    require(!TREE || ancestors, "kv4_attend_tree: NULL ancestors");
+    Launch L = plan_attend(a, TREE);
+    L.plan.ancestors = ancestors;
     const size_t need = part_bytes(a, L.plan);
     require(need == 0 || (a.workspace && aligned(a.workspace, 16) && a.workspace_bytes >= need),
             "kv4_attend: workspace too small or not 16-byte aligned");
@@ -1140,9 +1152,9 @@ void kv4_attend(const sili_kv4_attend_args &a, hipStream_t st) {
     with_dtype(a.dtype, [&](auto z) {
         using T = decltype(z);
         switch (a.cache.head_dim) {
-            case 64: run_few<T, 64>(a, L, st); break;
-            case 128: run_few<T, 128>(a, L, st); break;
-            default: run_few<T, 256>(a, L, st); break;
+            case 64: run_few<T, 64, TREE>(a, L, st); break;
+            case 128: run_few<T, 128, TREE>(a, L, st); break;
+            default: run_few<T, 256, TREE>(a, L, st); break;
         }
     });
     if (L.many_tiles) {
@@ -1151,5 +1163,10 @@ void kv4_attend(const sili_kv4_attend_args &a, hipStream_t st) {
     }
     SILI_HIP(hipGetLastError());
 }
+
+}  // namespace
+
+void kv4_attend(const sili_kv4_attend_args &a, hipStream_t st) { attend<false>(a, nullptr, st); }
+void kv4_attend_tree(const sili_kv4_attend_args &a, const uint64_t *ancestors, hipStream_t st) { attend<true>(a, ancestors, st); }
 
 }  // namespace sili

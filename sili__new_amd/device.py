@@ -24,6 +24,7 @@ from . import LIB_PATH
 F32, BF16, F16 = 0, 1, 2
 DTYPES = {"float32": F32, "bfloat16": BF16, "float16": F16}
 ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
+TREE_MOST = 64
 ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_BANDS, ROTARY_BASE = 0, 1, 2, 3
 SLOTS_NO_PAGE, SLOTS_TABLE_FULL, SLOTS_TOKENS_FULL, SLOTS_BAD_LENGTH, SLOTS_BAD_PAGE = 1, 2, 4, 8, 16
 
@@ -77,6 +78,29 @@ class Kv4Attend(C.Structure):
                                                "f32: scale; ptr: q; i64: q_token_stride, q_head_stride;"
                                                "ptr: out; i64: out_token_stride, out_head_stride; ptr: lse, workspace;"
                                                "size: workspace_bytes")
+
+
+class DraftTree(C.Structure):
+    _fields_ = _fields("ptr: parents, q_start, cached_lens; i64: requests, tokens, max_new; ptr: ancestors, positions")
+
+
+class Fp4Weights(C.Structure):
+    _fields_ = _fields("ptr: codes, scales; i64: n_out, n_in, group, codes_stride, scales_stride; i32: scale_dtype")
+
+
+class Fp4Pack(C.Structure):
+    _fields_ = [("w", Fp4Weights)] + _fields("i32: dtype; ptr: rows; i64: row_stride")
+
+
+class Fp4Linear(C.Structure):
+    _fields_ = [("w", Fp4Weights)] + _fields("i32: dtype, out_dtype; i64: tokens; ptr: x; i64: x_stride; ptr: y; i64: y_stride;"
+                                             "ptr: workspace; size: workspace_bytes")
+
+
+class LogitsConstrain(C.Structure):
+    _fields_ = _fields("i32: dtype; i64: rows, vocab, requests; ptr: logits; i64: logits_stride; ptr: out; i64: out_stride;"
+                       "ptr: q_start, history, history_lens; i64: history_stride; ptr: counted_from, tokens, ancestors;"
+                       "ptr: repetition, presence, frequency, bias; i64: bias_stride; ptr: allow, allow_row; i64: allow_stride, n_allow")
 
 
 _lib = C.CDLL(LIB_PATH)
@@ -133,6 +157,22 @@ kv4_append = _call("sili_kv4_append", Kv4Rows)
 kv4_read = _call("sili_kv4_read", Kv4Rows)
 kv4_attend = _call("sili_kv4_attend", Kv4Attend)
 kv4_attend_workspace = _bytes("sili_kv4_attend_workspace", Kv4Attend)
+draft_tree = _call("sili_draft_tree", DraftTree)
+kv4_attend_tree_workspace = _bytes("sili_kv4_attend_tree_workspace", Kv4Attend)
+fp4_pack = _call("sili_fp4_pack", Fp4Pack)
+fp4_linear = _call("sili_fp4_linear", Fp4Linear)
+fp4_linear_workspace = _bytes("sili_fp4_linear_workspace", Fp4Linear)
+logits_constrain = _call("sili_logits_constrain", LogitsConstrain)
+
+_lib.sili_kv4_attend_tree.argtypes = [C.POINTER(Kv4Attend), _ptr, _ptr]
+
+
+def kv4_attend_tree(args, ancestors, stream=None):
+    """sili_kv4_attend_tree of include/sili_hip.h: `ancestors` the address of the tokens' masks, on `stream`."""
+    rc = _lib.sili_kv4_attend_tree(args, ancestors, stream)
+    if rc:
+        _raise(rc)
+
 
 _lib.sili_rotary_steps.argtypes = [_i64, C.c_double, C.c_int] + [C.c_double] * 4 + [_ptr, C.POINTER(_f32)]
 
