@@ -65,9 +65,7 @@ __global__ __launch_bounds__(PACK_TPB) void k_fp4_pack(sili_fp4_pack_args a) {
 // y = x W^T on the bf16 matrix cores, x the left operand (rows: tokens), W the
 // right one (columns: outputs).  Codes are exact in bf16 and x enters in bf16
 // parts; a group's products are summed by themselves and then scaled in fp32, a
-// lane's column having one scale.  A wave takes its outputs' rows 128 inputs a
-// step: a lane loads 16 or 32 consecutive bytes, and lanes of a column exchange
-// dwords so that each product has consecutive inputs, of one group.
+// lane's column having one scale.
 constexpr int LINEAR_STEP = 128;
 
 struct LinearPlan {
@@ -88,12 +86,6 @@ __device__ __forceinline__ void cut_bf16(float x, float y, uint32_t (&part)[N]) 
         y -= bf16_hi(part[k]);
     }
 }
-__device__ __forceinline__ void swap32(uint32_t &a, uint32_t &b) {  // upper half of a, lower half of b
-    const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
-    a = r[0];
-    b = r[1];
-}
-
 __device__ __forceinline__ void store_as(void *p, int dtype, int64_t at, float x) {
     if (dtype == SILI_F32) ((float *)p)[at] = x;
     else if (dtype == SILI_BF16) ((__bf16 *)p)[at] = (__bf16)x;
@@ -108,9 +100,9 @@ __device__ __forceinline__ uint32_t load_scale(const sili_fp4_weights &w, int64_
     return w.scale_dtype == SILI_F32 ? ((const uint32_t *)w.scales)[at] : ((const uint16_t *)w.scales)[at];
 }
 
-// Few tokens: rows of one product, 16 in all with their parts, row r + RT k holding
-// part k of token r (RT = 16, 8, 4 for one, two, three parts).  A block cuts x once,
-// in LDS; its waves then run by themselves, 16 outputs each (or a share of their
+// Few tokens, up to 16: rows of one product a part of x (PM of them), or, with
+// 8 (two parts) or 4 (three) at most, of one product in all (PM 1), whose row r + RT k
+// holds part k of token r.  A block cuts x once, in LDS; its waves then run by themselves, 16 outputs each (or a share of their
 // inputs, joined in LDS), in turns of 256 inputs asked for AHEAD turns before.  Eight
 // lanes load 128 bytes of a row of codes, and four its scales, so that the cache is
 // asked for a line and not for a lane at a time; the wave turns them in LDS of its
@@ -127,9 +119,9 @@ struct FewLinear {
     int32_t row_words;  // of x in LDS, a row
 };
 
-template <typename T, int G>
+template <typename T, int G, int PM>
 __global__ __launch_bounds__(64 * FEW_WAVES) void k_linear_few(sili_fp4_linear_args a, LinearPlan pl, FewLinear few) {
-    constexpr int P = q_parts<T>(), RT = P == 1 ? 16 : P == 2 ? 8 : 4;
+    constexpr int P = q_parts<T>(), RT = P == PM ? 16 : P == 2 ? 8 : 4;
     constexpr int GT = FEW_TURN / G, GL = GT >= 4 ? GT / 4 : 1;  // groups a turn; scales a lane loads
     extern __shared__ __align__(16) uint32_t s_few[];
     const int wave = (int)uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, r16 = lane & 15;
@@ -225,8 +217,9 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_linear_few(sili_fp4_linear_a
     }
     __syncthreads();
     // this lane's row of x (tokens past the last: the last again; a fourth part: the third), its column of codes
-    const uint32_t *xs = s_x + (min(r16 / RT, P - 1) * tokens + min(r16 % RT, tokens - 1)) * few.row_words + 4 * g;
+    const uint32_t *xs = s_x + ((P == PM ? 0 : min(r16 / RT, P - 1)) * tokens + min(r16 % RT, tokens - 1)) * few.row_words + 4 * g;
     const uint32_t *ws = s_w + r16 * FEW_ROW + g;
+    const int part_words = tokens * few.row_words;
 
     auto store = [&](int64_t t, int64_t n, float y) {
         if (pl.splits > 1) pl.part[((int64_t)split * tokens + t) * a.w.n_out + n] = y;
@@ -234,7 +227,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_linear_few(sili_fp4_linear_a
     };
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
     auto join_parts = [&] {  // lane: output r16, rows 4 g + j of A
-        if (P == 1) return;
+        if (P == PM) return;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             float y = P == 3 && g == 3 ? 0.0f : acc[j];
@@ -262,9 +255,10 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_linear_few(sili_fp4_linear_a
             f32x4 sum;
 #pragma unroll
             for (int s = 0; s < FEW_TURN / 32; ++s) {
-                const u32x4 av = *reinterpret_cast<const u32x4 *>(x + 16 * s);
                 if (s % (G / 32) == 0) sum = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-                sum = mma(av, codes8(ws[4 * s]), sum);
+                const u32x4 b = codes8(ws[4 * s]);
+#pragma unroll
+                for (int k = 0; k < PM; ++k) sum = mma(*reinterpret_cast<const u32x4 *>(x + k * part_words + 16 * s), b, sum);
                 if ((s + 1) % (G / 32) == 0) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) acc[j] = __builtin_fmaf(sum[j], f[s / (G / 32)], acc[j]);
@@ -308,206 +302,203 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_linear_few(sili_fp4_linear_a
 }
 
 // More tokens: a block's four waves take WN times 64 outputs by 4 / WN times 32 MT
-// tokens, in products of 32 x 32 outputs x 16 inputs.  x is cut into its parts
-// once a block, in LDS (two buffers, KC inputs each: the next ones' loads are under
-// this one's products), rows padded by 16 bytes so that eight lanes' 16 bytes lie
-// in all banks; a wave's 64 outputs take each operand from there twice, which is
-// what the LDS can give the matrix cores.
+// tokens, in products of 32 x 32 outputs x 16 inputs.  LDS holds, twice, a step's
+// codes and scales and KC inputs of x cut into its parts: the next ones' loads are
+// under this one's products, each a line of the cache at a time.  A lane of a product
+// has eight codes of an even (lower half of the wave) or odd word of a row, so a row
+// keeps its even words before its odd ones.  Rows are padded by 16 bytes: 16 lanes'
+// 16 bytes lie in all banks.  A wave's 64 outputs take each operand of x twice,
+// which is what LDS can give the matrix cores.
 template <typename T, int G, int WN, int MT>
 struct ManyLinear {
     static constexpr int P = q_parts<T>(), WM = 4 / WN, BM = 32 * MT * WM, BN = 64 * WN;
-    static constexpr int KC = sizeof(T) == 4 ? 32 : 64, ROW = KC + 8;  // bf16 of a row
-    static constexpr int LDS = 2 * P * BM * ROW * 2;
+    static constexpr int KC = sizeof(T) == 4 ? 32 : 64, ROW = KC + 8;  // bf16 of a row of x
+    static constexpr int GS = LINEAR_STEP / G, C_ROW = LINEAR_STEP / 8 + 4;  // words of a row of codes
+    static constexpr int X_WORDS = P * BM * ROW / 2, W_WORDS = BN * C_ROW, S_WORDS = BN * GS;
+    static constexpr int LDS = 2 * 4 * (X_WORDS + W_WORDS + S_WORDS);
 };
 
 template <typename T, int G, int WN, int MT>
 __global__ __launch_bounds__(256, 2) void k_linear_many(sili_fp4_linear_args a, LinearPlan pl) {
     using M = ManyLinear<T, G, WN, MT>;
-    constexpr int P = M::P, BM = M::BM, KC = M::KC, ROW = M::ROW, GS = LINEAR_STEP / G;
+    constexpr int P = M::P, BM = M::BM, BN = M::BN, KC = M::KC, ROW = M::ROW, GS = M::GS, C_ROW = M::C_ROW;
     constexpr int TPR = KC / 8, PASS = 256 / TPR, PASSES = (BM + PASS - 1) / PASS;  // threads a row of x; rows a pass
-    constexpr int SUB = LINEAR_STEP / KC, KS = KC / 16;  // chunks a step; products a chunk
-    constexpr int US = (G < KC ? G : KC) / 16;           // ... of one scale
-    extern __shared__ __align__(16) uint16_t s_x[];      // [2][P][BM][ROW]
+    constexpr int SUB = LINEAR_STEP / KC, KS = KC / 16;                             // chunks a step; products a chunk
+    constexpr int US = (G < KC ? G : KC) / 16;                                      // ... of one scale
+    static_assert(SUB % 2 == 0, "a step's chunks begin with an even one");
+    constexpr bool WHOLE = P == 1 && G > KC;  // sums go on into the next chunk (more parts: their registers are dearer)
+    constexpr int NW = BN * 4 / 256, NS = BN * GS / 256 > 0 ? BN * GS / 256 : 1;    // loads a thread
+    extern __shared__ __align__(16) uint32_t s_many[];
+    uint32_t *s_w = s_many + 2 * M::X_WORDS;
+    float *s_s = reinterpret_cast<float *>(s_w + 2 * M::W_WORDS);
+    uint16_t *s_x = reinterpret_cast<uint16_t *>(s_many);  // [2][P][BM][ROW]
     const int tid = threadIdx.x, wave = (int)uniform(tid >> 6), lane = tid & 63, hf = lane >> 5, r32 = lane & 31;
     const int wn = wave % WN, wm = wave / WN;
     const int tile = blockIdx.x / pl.token_tiles, t0 = (blockIdx.x - tile * pl.token_tiles) * BM, split = blockIdx.y;
-    const int64_t n0 = (int64_t)tile * M::BN + 64 * wn;
+    const int64_t b0 = (int64_t)tile * BN;
     const int k_end = (int)a.w.n_in;
 
-    const uint8_t *codes[2];
-    int64_t scale_row[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const int64_t n = min(n0 + 32 * t + r32, a.w.n_out - 1);
-        codes[t] = a.w.codes + n * a.w.codes_stride + 32 * hf;
-        scale_row[t] = n * a.w.scales_stride;
-    }
     const T *x[PASSES];
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
         const int64_t token = min((int64_t)t0 + i * PASS + tid / TPR, a.tokens - 1);
-        x[i] = (const T *)a.x + token * a.x_stride + 8 * (tid % TPR);
+        x[i] = (const T *)a.x + token * a.x_stride;
     }
+    const uint8_t *codes[NW];  // 16 bytes: inputs 32 (tid % 4) .. + 31 of a row
+#pragma unroll
+    for (int i = 0; i < NW; ++i) codes[i] = a.w.codes + min(b0 + 64 * i + tid / 4, a.w.n_out - 1) * a.w.codes_stride;
+    int64_t scales[NS];
+#pragma unroll
+    for (int i = 0; i < NS; ++i) scales[i] = min(b0 + (256 * i + tid) / GS, a.w.n_out - 1) * a.w.scales_stride;
 
-    Loose<T, 8> xs[PASSES];
-    auto fetch_x = [&](int k0) {
+    // Every thread asks for the same number of loads whatever the step: the compiler
+    // could else not tell which of them are still under way, and would wait for all.
+    // What lies past the inputs asks for their last ones, and is stored as zeros.
+    Loose<T, 8> xs2[2][PASSES];  // of even and odd chunks
+    auto fetch_x = [&](Loose<T, 8>(&xs)[PASSES], int k0) {
+        const int k = min(k0 + 8 * (tid % TPR), k_end - 8);
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-            if (k0 + 8 * (tid % TPR) < k_end) {
-                xs[i] = *reinterpret_cast<const Loose<T, 8> *>(x[i] + k0);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) xs[i].v[j] = (T)0.0f;
-            }
-        }
+        for (int i = 0; i < PASSES; ++i) xs[i] = *reinterpret_cast<const Loose<T, 8> *>(x[i] + k);
     };
-    auto put_x = [&](int buf) {
+    auto put_x = [&](const Loose<T, 8>(&xs)[PASSES], int k0, int buf) {
+        const uint32_t keep = k0 + 8 * (tid % TPR) < k_end ? ~0u : 0u;
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
             const int row = i * PASS + tid / TPR;
             if (BM % PASS != 0 && row >= BM) continue;
             u32x4 part[P];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t c[P];
-                cut_bf16<P>((float)xs[i].v[2 * j], (float)xs[i].v[2 * j + 1], c);
-#pragma unroll
-                for (int k = 0; k < P; ++k) part[k][j] = c[k];
-            }
-#pragma unroll
-            for (int k = 0; k < P; ++k)
-                *reinterpret_cast<u32x4 *>(s_x + ((buf * P + k) * BM + row) * ROW + 8 * (tid % TPR)) = part[k];
-        }
-    };
-    uint4 w[2][2];
-    uint32_t sc[2][GS];  // two bytes: two a word
-    auto fetch_w = [&](int step) {
-        const int k0 = step * LINEAR_STEP, left = k_end - k0;
-        if (left >= LINEAR_STEP) {
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                w[t][0] = *reinterpret_cast<const uint4 *>(codes[t] + k0 / 2);
-                w[t][1] = *reinterpret_cast<const uint4 *>(codes[t] + k0 / 2 + 16);
-            }
-            if (a.w.scale_dtype == SILI_F32) {
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const auto v = *reinterpret_cast<const Loose<uint32_t, GS> *>((const uint32_t *)a.w.scales + scale_row[t] + step * GS);
-#pragma unroll
-                    for (int i = 0; i < GS; ++i) sc[t][i] = v.v[i];
-                }
-            } else if constexpr (GS == 1) {
-#pragma unroll
-                for (int t = 0; t < 2; ++t) sc[t][0] = ((const uint16_t *)a.w.scales)[scale_row[t] + step];
+            if constexpr (P == 1) {
+                part[0] = __builtin_bit_cast(u32x4, xs[i]);
             } else {
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const auto v = *reinterpret_cast<const LooseWords<GS / 2> *>((const uint16_t *)a.w.scales + scale_row[t] + step * GS);
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t c[P];
+                    cut_bf16<P>((float)xs[i].v[2 * j], (float)xs[i].v[2 * j + 1], c);
 #pragma unroll
-                    for (int i = 0; i < GS / 2; ++i) sc[t][i] = v.v[i];
+                    for (int k = 0; k < P; ++k) part[k][j] = c[k];
                 }
             }
+#pragma unroll
+            for (int k = 0; k < P; ++k) *reinterpret_cast<u32x4 *>(s_x + ((buf * P + k) * BM + row) * ROW + 8 * (tid % TPR)) = part[k] & keep;
+        }
+    };
+    struct Weights {
+        uint4 w[NW];
+        uint32_t sc[NS];
+    } w2[2];  // of even and odd steps
+    const int groups = k_end / G;
+    auto fetch_w = [&](Weights &v, int step) {
+        const int k = min(step * LINEAR_STEP + 32 * (tid % 4), k_end - 32), s = min(step * GS + tid % GS, groups - 1);
+#pragma unroll
+        for (int i = 0; i < NW; ++i) v.w[i] = *reinterpret_cast<const uint4 *>(codes[i] + k / 2);
+        if (a.w.scale_dtype == SILI_F32) {
+#pragma unroll
+            for (int i = 0; i < NS; ++i) v.sc[i] = ((const uint32_t *)a.w.scales)[scales[i] + s];
         } else {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
+            for (int i = 0; i < NS; ++i) v.sc[i] = ((const uint16_t *)a.w.scales)[scales[i] + s];
+        }
+    };
+    auto put_w = [&](const Weights &v, int step, int buf) {
+        const uint32_t keep = step * LINEAR_STEP + 32 * (tid % 4) < k_end ? ~0u : 0u;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    w[t][i] = make_uint4(0, 0, 0, 0);
-                    if (64 * hf + 32 * i < left) w[t][i] = *reinterpret_cast<const uint4 *>(codes[t] + k0 / 2 + 16 * i);
-                }
-            }
+        for (int i = 0; i < NW; ++i) {
+            uint32_t *row = s_w + buf * M::W_WORDS + (64 * i + tid / 4) * C_ROW + 2 * (tid % 4);
+            *reinterpret_cast<uint2 *>(row) = make_uint2(v.w[i].x & keep, v.w[i].z & keep);
+            *reinterpret_cast<uint2 *>(row + LINEAR_STEP / 16) = make_uint2(v.w[i].y & keep, v.w[i].w & keep);
+        }
+        if (BN * GS >= 256 || tid < BN * GS) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-#pragma unroll
-                for (int i = 0; i < GS; ++i) sc[t][i] = 0;
-#pragma unroll
-                for (int i = 0; i < GS; ++i) {
-                    if (G * i >= left) continue;
-                    const uint32_t v = load_scale(a.w, scale_row[t] + step * GS + i);
-                    if (a.w.scale_dtype == SILI_F32 || GS == 1) sc[t][i] = v;
-                    else sc[t][i / 2] |= v << (16 * (i % 2));
-                }
-            }
+            for (int i = 0; i < NS; ++i)
+                s_s[buf * M::S_WORDS + 256 * i + tid] = step * GS + tid % GS < groups ? scale_of(a.w.scale_dtype, v.sc[i]) : 0.0f;
         }
     };
 
-    f32x16 acc[2][MT];
+    f32x16 acc[2][MT], sum[2][MT];
+    const f32x16 zero = {};
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[t][m][i] = 0.0f;
+        for (int m = 0; m < MT; ++m) acc[t][m] = zero;
 
     const int first = split * pl.chunk, last = min(pl.steps, first + pl.chunk);
     if (first < last) {
-        fetch_w(first);
-        fetch_x(first * LINEAR_STEP);
-        put_x(0);
+        fetch_w(w2[0], first);
+        fetch_x(xs2[0], first * LINEAR_STEP);
+        fetch_w(w2[1], first + 1);
+        fetch_x(xs2[1], first * LINEAR_STEP + KC);
+        put_w(w2[0], first, 0);
+        put_x(xs2[0], first * LINEAR_STEP, 0);
     }
-    int buf = 0;
-    for (int step = first; step < last; ++step) {
-        uint32_t ww[2][8];
-        float ss[2][GS];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const uint32_t d[8] = {w[t][0].x, w[t][0].y, w[t][0].z, w[t][0].w, w[t][1].x, w[t][1].y, w[t][1].z, w[t][1].w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {  // product i has dwords 2 i (lower lanes) and 2 i + 1
-                ww[t][i] = d[2 * i];
-                ww[t][4 + i] = d[2 * i + 1];
-                swap32(ww[t][i], ww[t][4 + i]);
-            }
-#pragma unroll
-            for (int i = 0; i < GS; ++i)
-                ss[t][i] = scale_of(a.w.scale_dtype, a.w.scale_dtype == SILI_F32 || GS == 1 ? sc[t][i] : sc[t][i / 2] >> (16 * (i % 2)));
-        }
-        if (step + 1 < last) fetch_w(step + 1);
+    // Step `step`, whose parity is `odd`: asks for the step after the next, and in each
+    // chunk for the chunk after the next.
+    auto run = [&](int step, auto odd) {
+        constexpr int ODD = decltype(odd)::value;
 #pragma unroll
         for (int sub = 0; sub < SUB; ++sub) {
-            const bool more = sub + 1 < SUB || step + 1 < last;
+            constexpr int wbuf = ODD;
+            const int buf = sub & 1;
             __syncthreads();
-            if (more) fetch_x(step * LINEAR_STEP + (sub + 1) * KC);
+            if (sub == 0) fetch_w(w2[ODD], step + 2);
+            const int k0 = step * LINEAR_STEP + sub * KC;
+            fetch_x(xs2[buf], k0 + 2 * KC);
+            uint32_t ww[2][KS];
+            const uint32_t *wr = s_w + wbuf * M::W_WORDS + (64 * wn + r32) * C_ROW + (LINEAR_STEP / 16) * hf + KS * sub;
+            const float *sr = s_s + wbuf * M::S_WORDS + (64 * wn + r32) * GS;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int k = 0; k < KS; ++k) ww[t][k] = wr[32 * t * C_ROW + k];
+            float f[2][US < KS ? KS / US : 1];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < KS / US; ++i) f[t][i] = sr[32 * t * GS + (sub * KS + i * US) / (G / 16)];
             const uint16_t *base = s_x + (buf * P * BM + 32 * MT * wm + r32) * ROW + 8 * hf;
-            // the inputs of a chunk that share a scale
+            // x's operands, FEED products before theirs: the compiler left to itself waits
+            // for each read of LDS
+            constexpr int NQ = KS * P * MT, FEED = WHOLE || MT == 1 ? 4 : 2;
+            u32x4 av[NQ], b[2];
 #pragma unroll
-            for (int s = 0; s < KS; s += US) {
-                const int k = sub * KS + s;  // product of the step
-                u32x4 b[US][2];
+            for (int q = 0; q < NQ + FEED; ++q) {
+                if (q < NQ) {
+                    const int s = q / (P * MT), p = q / MT % P, m = q % MT;
+                    av[q] = *reinterpret_cast<const u32x4 *>(base + (p * BM + 32 * m) * ROW + 16 * s);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if (q < FEED) continue;
+                const int o = q - FEED, s = o / (P * MT), p = o / MT % P, m = o % MT, k = sub * KS + s;  // product of the step
+                const bool begins = WHOLE ? k % (G / 16) == 0 : s % US == 0, ends = WHOLE ? (k + 1) % (G / 16) == 0 : (s + 1) % US == 0;
+                if (p == 0 && m == 0) {
 #pragma unroll
-                for (int u = 0; u < US; ++u)
+                    for (int t = 0; t < 2; ++t) b[t] = codes8(ww[t][s]);
+                }
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) b[u][t] = codes8(ww[t][k + u]);
+                for (int t = 0; t < 2; ++t) sum[t][m] = mma(av[o], b[t], begins && p == 0 ? zero : sum[t][m]);
+                if (ends && p == P - 1 && m == MT - 1) {
 #pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    f32x16 sum[2];
+                    for (int i = 0; i < MT; ++i)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) sum[0][i] = sum[1][i] = 0.0f;
+                        for (int t = 0; t < 2; ++t) {
 #pragma unroll
-                    for (int u = 0; u < US; ++u)
-#pragma unroll
-                        for (int p = 0; p < P; ++p) {
-                            const u32x4 av = *reinterpret_cast<const u32x4 *>(base + (p * BM + 32 * m) * ROW + 16 * (s + u));
-#pragma unroll
-                            for (int t = 0; t < 2; ++t) sum[t] = mma(av, b[u][t], sum[t]);
+                            for (int j = 0; j < 16; ++j) acc[t][i][j] = __builtin_fmaf(sum[t][i][j], f[t][s / US], acc[t][i][j]);
+                            // here: the compiler would keep the sums of several scales until the accumulators' next use
+                            __asm__ volatile("" : "+v"(acc[t][i]));
                         }
-#pragma unroll
-                    for (int t = 0; t < 2; ++t)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) acc[t][m][i] = __builtin_fmaf(sum[t][i], ss[t][k / (G / 16)], acc[t][m][i]);
-                    // here: the compiler would keep the sums of several scales until the accumulators' next use
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) __asm__ volatile("" : "+v"(acc[t][m]));
                 }
             }
-            if (more) put_x(buf ^ 1);
-            buf ^= 1;
+            put_x(xs2[buf ^ 1], k0 + KC, buf ^ 1);
+            if (sub == SUB - 1) put_w(w2[ODD ^ 1], step + 1, wbuf ^ 1);
         }
+    };
+    for (int step = first; step < last; step += 2) {
+        run(step, std::integral_constant<int, 0>{});
+        if (step + 1 < last) run(step + 1, std::integral_constant<int, 1>{});
     }
     // lane: output r32; result 4 i + j of a tile is token 8 i + 4 hf + j
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        const int64_t n = n0 + 32 * t + r32;
+        const int64_t n = b0 + 64 * wn + 32 * t + r32;
         if (n >= a.w.n_out) continue;
 #pragma unroll
         for (int m = 0; m < MT; ++m)
@@ -558,7 +549,7 @@ void check_linear(const sili_fp4_linear_args &a) {
 // How a call is launched.
 struct LinearLaunch {
     int64_t blocks = 0;
-    bool few_tokens = false;
+    bool few_tokens = false, merged = false;
     int wn = 0, mt = 0;  // more tokens: a block's shape
     uint32_t lds = 0;
     LinearPlan plan{};
@@ -566,15 +557,18 @@ struct LinearLaunch {
 };
 
 // Few tokens.  512 blocks of 8 waves fill the GPU twice over.  Fewer (outputs / 128):
-// waves share outputs where x is small (up to 8 rows of 16384 inputs, which every such
+// waves share outputs where x is small (up to 4 rows of 16384 inputs, which every such
 // block holds whole), else blocks split the inputs and are joined.  us of a call, its
-// inputs x outputs, rows of x (tokens times parts); share 1, share 2 .. 8, splits:
+// inputs x outputs, rows of x (tokens times parts); share 1, the best share, the best
+// splits:
 //     5120 x 32768, 3 rows   19.6, 18.7, 21.3      5120 x 5120, 1 row   -, 5.8, 9.0
-//     5120 x 32768, 8 rows   23.0, 26.0, 23.0      5120 x 5120, 8 rows  -, 8.7, 9.3
+//     5120 x 32768, 8 rows   23.0, 26.0, 23.0      5120 x 5120, 8 rows  16.5, 8.7, 9.3
 //     5120 x 32768, 16 rows  27.5, 42.8, 26.5      32768 x 5120, 8 rows -, 31.5, 24.2
 //     5120 x 1000, 3 rows    -, 4.9, 6.5           32768 x 1000, 3 rows -, 9.1, 8.3
-// A block whose waves do not share goes on to other outputs with the x it holds
-// (5120 x 131071, 8 rows: 78 us, 92 with blocks of one tile).
+// (8 rows share well by 4 but not by 8, and lose by 2: they split.)  A block whose
+// waves do not share goes on to other outputs with the x it holds (5120 x 131071, 8
+// rows: 78 us, 92 with blocks of one tile).  More than 16 tokens' kernel took 48 us for
+// 5 fp32 tokens of 5120 x 32768, this one 28.
 void plan_few(const sili_fp4_linear_args &a, int64_t parts, LinearLaunch &L) {
     auto tiles = [](int64_t n, int64_t of) { return (n + of - 1) / of; };
     LinearPlan &p = L.plan;
@@ -582,11 +576,13 @@ void plan_few(const sili_fp4_linear_args &a, int64_t parts, LinearLaunch &L) {
     L.few_tokens = true;
     p.token_tiles = 1;
     p.steps = (int32_t)tiles(a.w.n_in, FEW_TURN);
-    const int64_t turns = std::max<int64_t>(1, p.steps), rows = a.tokens * parts, rt = parts == 1 ? 16 : parts == 2 ? 8 : 4;
+    const int64_t turns = std::max<int64_t>(1, p.steps), rows = a.tokens * parts;
+    L.merged = rows <= (parts == 3 ? 12 : 16);
+    const int64_t rt = !L.merged || parts == 1 ? 16 : parts == 2 ? 8 : 4;
     const int64_t base = tiles(a.w.n_out, 16 * FEW_WAVES), want = std::max<int64_t>(1, 512 / base);
     int64_t splits = 1;
     f.share = 1;
-    if (rows <= 8 && turns <= 64) {
+    if (rows <= 4 && turns <= 64) {
         while (f.share < 8 && f.share * 2 <= std::min(want, turns)) f.share *= 2;
     } else {
         splits = std::clamp<int64_t>(want, 1, std::max<int64_t>(1, turns / 4));
@@ -611,7 +607,7 @@ LinearLaunch plan_linear(const sili_fp4_linear_args &a) {
     LinearPlan &p = L.plan;
     auto tiles = [](int64_t n, int64_t of) { return (n + of - 1) / of; };
     const int64_t parts = a.dtype == SILI_F32 ? 3 : a.dtype == SILI_F16 ? 2 : 1;
-    if (a.tokens <= (parts == 1 ? 16 : parts == 2 ? 8 : 4)) {
+    if (a.tokens <= 16) {
         plan_few(a, parts, L);
         return L;
     }
@@ -636,7 +632,7 @@ void run_linear(const sili_fp4_linear_args &a, const LinearLaunch &L, hipStream_
     const LinearPlan &p = L.plan;
     const dim3 grid((unsigned)L.blocks, (unsigned)p.splits);
     if (L.few_tokens) {
-        launch(k_linear_few<T, G>, grid, dim3(64 * FEW_WAVES), L.lds, st, a, p, L.few);
+        launch(L.merged ? k_linear_few<T, G, 1> : k_linear_few<T, G, q_parts<T>()>, grid, dim3(64 * FEW_WAVES), L.lds, st, a, p, L.few);
     } else if (L.wn == 4) {
         launch(k_linear_many<T, G, 4, 1>, grid, dim3(256), (uint32_t)ManyLinear<T, G, 4, 1>::LDS, st, a, p);
     } else if (L.mt == 1) {
