@@ -64,6 +64,12 @@ template <typename T, int N>
 struct alignas(sizeof(T) * N) Pack {
     T v[N];
 };
+// N elements at any address of an element: one load where the hardware has one
+// for the size (it takes any alignment).
+template <typename T, int N>
+struct __attribute__((packed, aligned(sizeof(T)))) Loose {
+    T v[N];
+};
 template <typename T, int N>
 __device__ __forceinline__ void load_pack(const T *p, float (&x)[N]) {
     const Pack<T, N> k = *reinterpret_cast<const Pack<T, N> *>(p);

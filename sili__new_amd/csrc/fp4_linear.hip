@@ -11,13 +11,6 @@ namespace sili {
 
 namespace {
 
-// N elements at any address of an element: one load where the hardware has one
-// for the size (it takes any alignment).
-template <typename T, int N>
-struct __attribute__((packed, aligned(sizeof(T)))) Loose {
-    T v[N];
-};
-
 // Words at any address of two bytes.
 template <int N>
 struct __attribute__((packed, aligned(2))) LooseWords {
