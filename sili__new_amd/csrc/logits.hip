@@ -2,8 +2,8 @@
 //
 // A block holds a chunk of the vocabulary of one request: it counts the
 // request's history there in LDS (low 31 bits: how often past counted_from; top
-// bit: before it), and then goes over the request's rows, eight tokens a thread
-// and load, whose biases stay in registers.  A bit a token says whether it occurs at
+// bit: before it), and then goes over the request's rows, four or eight tokens a
+// thread and load, whose biases stay in registers.  A bit a token says whether it occurs at
 // all: most eights ask for no count.  A row whose own path has tokens in the chunk
 // adds them to the counts and takes them off again; the others pass without a
 // barrier.  Rows begin at any element (vocabularies are odd): loads of 16 bytes at any
@@ -12,25 +12,28 @@
 #include "block_ops.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace sili {
 
 namespace {
 
-constexpr int LOGITS_TPB = 256, LOGITS_PACK = 8;
 constexpr uint32_t SEEN = 0x80000000u;
 
 struct LogitsPlan {
     int32_t chunks, row_groups;  // blocks of a request
 };
 
-template <typename T, int CHUNK>
-__global__ __launch_bounds__(LOGITS_TPB) void k_logits_constrain(sili_logits_constrain_args a, LogitsPlan pl) {
-    constexpr int N = LOGITS_PACK, IT = CHUNK / (N * LOGITS_TPB) > 0 ? CHUNK / (N * LOGITS_TPB) : 1;
+// N tokens a thread.
+template <typename T, int TPB, int N>
+__global__ __launch_bounds__(TPB, 8) void k_logits_constrain(sili_logits_constrain_args a, LogitsPlan pl) {
+    constexpr int CHUNK = N * TPB;
     __shared__ __align__(16) uint32_t s_count[CHUNK];
     __shared__ uint32_t s_any[CHUNK / 32];
     const int tid = threadIdx.x, lane = tid & 63;
-    const uint32_t block = blockIdx.x / (uint32_t)pl.chunks, chunk = blockIdx.x - block * (uint32_t)pl.chunks;
+    // the first chunks of all requests first: vocabularies begin with their frequent tokens,
+    // which take longest to count
+    const uint32_t groups = (uint32_t)(a.requests * pl.row_groups), chunk = blockIdx.x / groups, block = blockIdx.x - chunk * groups;
     const uint32_t req = block / (uint32_t)pl.row_groups, part = block - req * (uint32_t)pl.row_groups;
     const int32_t c0 = (int32_t)chunk * CHUNK, c1 = (int32_t)min((int64_t)c0 + CHUNK, a.vocab);
 
@@ -43,31 +46,46 @@ __global__ __launch_bounds__(LOGITS_TPB) void k_logits_constrain(sili_logits_con
     const int32_t n = min(all, (int32_t)a.rows - first);
     if ((int32_t)part >= n) return;
 
-    // this thread's tokens: c0 + N tid + N LOGITS_TPB k
-    const int32_t at = N * tid;
-    Loose<T, N> z[IT];
-    auto fetch = [&](int32_t row) {
-        const T *src = (const T *)a.logits + row * a.logits_stride + c0;
-#pragma unroll
-        for (int k = 0; k < IT; ++k) {
-            const int32_t i = at + k * N * LOGITS_TPB;
-            if (c0 + i + N <= c1) {
-                z[k] = *reinterpret_cast<const Loose<T, N> *>(src + i);
-            } else {
-#pragma unroll
-                for (int j = 0; j < N; ++j)
-                    if (c0 + i + j < c1) z[k].v[j] = src[i + j];
-            }
+    // A wave's lanes hold the masks of the block's next 64 rows: their addresses are
+    // there before they are needed.
+    int32_t my_allow = -1;
+    uint32_t path_lo = 0, path_hi = 0;
+    auto look_up = [&](int32_t i) {  // of rows i, i + row_groups, ...
+        const int64_t mine = i + (int64_t)lane * pl.row_groups;
+        if (mine >= n) return;
+        const int32_t row = first + (int32_t)mine;
+        if (a.allow) my_allow = a.allow_row ? a.allow_row[row] : row;
+        if (a.ancestors) {
+            path_lo = (uint32_t)a.ancestors[row];
+            path_hi = (uint32_t)(a.ancestors[row] >> 32);
         }
     };
-    fetch(first + (int32_t)part);
+    look_up((int32_t)part);
+
+    const int32_t at = N * tid, v0 = c0 + at;  // this thread's tokens: v0 .. v0 + N - 1
+    Loose<T, N> z;
+    uint32_t bits = ~0u;  // those allowed
+    auto fetch = [&](int32_t row, int slot) {
+        const int32_t m = (int32_t)__builtin_amdgcn_readlane((uint32_t)my_allow, slot);
+        const bool masked = a.allow && m >= 0 && m < a.n_allow;
+        bits = masked && v0 < c1 ? a.allow[m * a.allow_stride + (v0 >> 5)] >> (v0 & 31) : ~0u;
+        const T *src = (const T *)a.logits + row * a.logits_stride + v0;
+        if (v0 + N <= c1) {
+            z = *reinterpret_cast<const Loose<T, N> *>(src);
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (v0 + j < c1) z.v[j] = src[j];
+        }
+    };
+    fetch(first + (int32_t)part, 0);
 
     const bool counts = a.history != nullptr || a.ancestors != nullptr;
     int32_t mine = -1;  // token `lane` of the request's path, where it is in this chunk
     uint64_t in_chunk = 0;
     if (counts) {
-        for (int i = tid; i < CHUNK / 4; i += LOGITS_TPB) reinterpret_cast<uint4 *>(s_count)[i] = make_uint4(0, 0, 0, 0);
-        for (int i = tid; i < CHUNK / 32; i += LOGITS_TPB) s_any[i] = 0;
+        for (int i = tid; i < CHUNK / 4; i += TPB) reinterpret_cast<uint4 *>(s_count)[i] = make_uint4(0, 0, 0, 0);
+        for (int i = tid; i < CHUNK / 32; i += TPB) s_any[i] = 0;
         if (a.ancestors && lane < min(all, (int32_t)a.rows - first)) {
             const int32_t v = a.tokens[first + lane];
             if (v >= c0 && v < c1) mine = v - c0;
@@ -80,87 +98,91 @@ __global__ __launch_bounds__(LOGITS_TPB) void k_logits_constrain(sili_logits_con
         const int32_t len = (int32_t)max((int64_t)0, min((int64_t)a.history_lens[req], a.history_stride));
         const int32_t since = a.counted_from ? a.counted_from[req] : 0;
         const int32_t *past = a.history + req * a.history_stride;
-        auto count = [&](int32_t i, int32_t v) {
-            if (v < c0 || v >= c1) return;
-            atomicOr(&s_any[(v - c0) >> 5], 1u << ((v - c0) & 31));
-            if (i < since) atomicOr(&s_count[v - c0], SEEN);
-            else atomicAdd(&s_count[v - c0], 1u);
+        // M entries from i on.  A frequent token's atomics run one after another: none where
+        // nothing changes.
+        auto count = [&](int32_t i, const auto &v, auto m) {
+            constexpr int M = decltype(m)::value;
+            uint32_t held[M], word[M];
+#pragma unroll
+            for (int j = 0; j < M; ++j) {
+                const int32_t k = v[j] >= c0 && v[j] < c1 ? v[j] - c0 : 0;
+                held[j] = __hip_atomic_load(&s_count[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                word[j] = __hip_atomic_load(&s_any[k >> 5], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            }
+#pragma unroll
+            for (int j = 0; j < M; ++j) {
+                if (v[j] < c0 || v[j] >= c1) continue;
+                const int32_t k = v[j] - c0;
+                const uint32_t bit = 1u << (k & 31);
+                if ((word[j] & bit) == 0) atomicOr(&s_any[k >> 5], bit);
+                if (i + j >= since) atomicAdd(&s_count[k], 1u);
+                else if ((held[j] & SEEN) == 0) atomicOr(&s_count[k], SEEN);
+            }
         };
         const int32_t whole = len & ~3;
-#pragma unroll 4
-        for (int32_t i = 4 * tid; i < whole; i += 4 * LOGITS_TPB) {
-            const auto v = *reinterpret_cast<const Loose<int32_t, 4> *>(past + i);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) count(i + j, v.v[j]);
-        }
-        if (tid < len - whole) count(whole + tid, past[whole + tid]);
+#pragma unroll 2
+        for (int32_t i = 4 * tid; i < whole; i += 4 * TPB)
+            count(i, reinterpret_cast<const Loose<int32_t, 4> *>(past + i)->v, std::integral_constant<int, 4>{});
+        if (tid < len - whole) count(whole + tid, &past[whole + tid], std::integral_constant<int, 1>{});
     }
     if (counts) __syncthreads();
     const float rep = a.repetition ? a.repetition[req] : 1.0f, freq = a.frequency ? a.frequency[req] : 0.0f,
                 pres = a.presence ? a.presence[req] : 0.0f;
-    Loose<float, N> bias[IT];
-    uint32_t any[IT];
-#pragma unroll
-    for (int k = 0; k < IT; ++k) {
-        const int32_t i = at + k * N * LOGITS_TPB;
-        any[k] = counts && i < CHUNK ? s_any[i >> 5] >> (i & 31) & 0xFFu : 0u;
-        if (!a.bias) continue;
-        const float *src = a.bias + req * a.bias_stride + c0 + i;
-        if (c0 + i + N <= c1) {
-            bias[k] = *reinterpret_cast<const Loose<float, N> *>(src);
+    const uint32_t any = counts ? s_any[at >> 5] >> (at & 31) & ((1u << N) - 1u) : 0u;
+    Loose<float, N> bias = {};
+    if (a.bias) {
+        const float *src = a.bias + req * a.bias_stride + v0;
+        if (v0 + N <= c1) {
+            bias = *reinterpret_cast<const Loose<float, N> *>(src);
         } else {
 #pragma unroll
             for (int j = 0; j < N; ++j)
-                if (c0 + i + j < c1) bias[k].v[j] = src[j];
+                if (v0 + j < c1) bias.v[j] = src[j];
         }
     }
 
+    int slot = 0;  // of the row among those looked up
     for (int32_t i = (int32_t)part; i < n; i += pl.row_groups) {
         const int32_t row = first + i;
-        const uint64_t path = a.ancestors ? a.ancestors[row] & in_chunk : 0;  // uniform
+        const uint32_t lo = __builtin_amdgcn_readlane(path_lo, slot), hi = __builtin_amdgcn_readlane(path_hi, slot);
+        const uint64_t path = ((uint64_t)hi << 32 | lo) & in_chunk;
         const bool adds = tid < 64 && mine >= 0 && (path >> lane & 1) != 0;
         if (path != 0) {
             if (adds) atomicAdd(&s_count[mine], 1u);
             __syncthreads();
         }
-        const int64_t m = !a.allow ? -1 : a.allow_row ? a.allow_row[row] : row;
-        const uint32_t *allow = m >= 0 && m < a.n_allow ? a.allow + m * a.allow_stride : nullptr;
-        T *dst = (T *)a.out + row * a.out_stride + c0;
-        Loose<T, N> out[IT];
+        float x[N];
 #pragma unroll
-        for (int k = 0; k < IT; ++k) {
-            const int32_t e = at + k * N * LOGITS_TPB, v = c0 + e;
-            if (v >= c1) continue;
-            const uint32_t bits = allow ? allow[v >> 5] >> (v & 31) : 0xFFu;
-            float x[N];
-#pragma unroll
-            for (int j = 0; j < N; ++j) x[j] = (float)z[k].v[j];
-            if (any[k] != 0) {
-#pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    const uint32_t c = s_count[e + j];
-                    if (c == 0) continue;
-                    x[j] = x[j] > 0.0f ? x[j] / rep : x[j] * rep;
-                    if ((c & ~SEEN) != 0) x[j] -= freq * (float)(c & ~SEEN) + pres;
-                }
-            }
+        for (int j = 0; j < N; ++j) x[j] = (float)z.v[j];
+        if (any != 0) {
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                if (a.bias) x[j] += bias[k].v[j];
-                out[k].v[j] = (T)((bits >> j & 1) != 0 ? x[j] : -INFINITY);
+                const uint32_t c = s_count[at + j];
+                if (c == 0) continue;
+                x[j] = x[j] > 0.0f ? x[j] / rep : x[j] * rep;
+                if ((c & ~SEEN) != 0) x[j] -= freq * (float)(c & ~SEEN) + pres;
             }
         }
-        if (i + pl.row_groups < n) fetch(row + pl.row_groups);
+        Loose<T, N> out;
 #pragma unroll
-        for (int k = 0; k < IT; ++k) {
-            const int32_t e = at + k * N * LOGITS_TPB, v = c0 + e;
-            if (v + N <= c1) {
-                *reinterpret_cast<Loose<T, N> *>(dst + e) = out[k];
-            } else {
-#pragma unroll
-                for (int j = 0; j < N; ++j)
-                    if (v + j < c1) dst[e + j] = out[k].v[j];
+        for (int j = 0; j < N; ++j) {
+            if (a.bias) x[j] += bias.v[j];
+            out.v[j] = (T)((bits >> j & 1) != 0 ? x[j] : -INFINITY);
+        }
+        if (i + pl.row_groups < n) {
+            if (++slot == 64) {
+                look_up(i + pl.row_groups);
+                slot = 0;
             }
+            fetch(row + pl.row_groups, slot);
+        }
+        T *dst = (T *)a.out + row * a.out_stride + v0;
+        if (v0 + N <= c1) {
+            *reinterpret_cast<Loose<T, N> *>(dst) = out;
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (v0 + j < c1) dst[j] = out.v[j];
         }
         if (path != 0) {
             __syncthreads();
@@ -187,16 +209,22 @@ void logits_constrain(const sili_logits_constrain_args &a, hipStream_t st) {
     require(a.logits && a.out, "logits_constrain: NULL buffer");
     require(a.out != a.logits || a.out_stride == a.logits_stride, "logits_constrain: in place with other strides");
     LogitsPlan p;
-    // small chunks where large ones would leave CUs without a block
-    const int64_t chunk = a.requests * ((a.vocab + 4095) / 4096) < 256 ? 1024 : 4096;
+    // Chunks of 8192 tokens, whose 1024 threads scan a history in few loads (64 requests
+    // of 8 rows of 131071 and histories of 8192: 97 us, with chunks of 4096 and 256
+    // threads 105); of 1024 where those would leave CUs without a block (one row of
+    // 131071: 7.2 us, with 8192 8.4).
+    const bool large = a.requests * ((a.vocab + 8191) / 8192) >= 256;
+    const int64_t chunk = large ? 8192 : 1024;
     p.chunks = (int32_t)((a.vocab + chunk - 1) / chunk);
     // rows of a request share its counts; few requests: their rows go to several blocks
     const int64_t each = (a.rows + a.requests - 1) / a.requests, blocks = a.requests * p.chunks;
     p.row_groups = a.q_start ? (int32_t)std::clamp<int64_t>(1024 / blocks, 1, each) : 1;
-    require(blocks * p.row_groups < (int64_t(1) << 32) / LOGITS_TPB, "logits_constrain: too many requests");
+    require(blocks * p.row_groups < (int64_t(1) << 32) / 1024, "logits_constrain: too many requests");
     const dim3 grid((unsigned)(blocks * p.row_groups));
     with_dtype(a.dtype, [&](auto z) {
-        launch(chunk == 1024 ? k_logits_constrain<decltype(z), 1024> : k_logits_constrain<decltype(z), 4096>, grid, dim3(LOGITS_TPB), 0, st, a, p);
+        using T = decltype(z);
+        if (large) launch(k_logits_constrain<T, 1024, 8>, grid, dim3(1024), 0, st, a, p);
+        else launch(k_logits_constrain<T, 256, 4>, grid, dim3(256), 0, st, a, p);
     });
     SILI_HIP(hipGetLastError());
 }
