@@ -799,8 +799,11 @@ int sili_draft_tree(const sili_draft_tree_args *args, void *stream);
  * kv_lens[r] - n, a query sees the keys before base and key base + j for every
  * bit j < n of its mask ancestors[t] [tokens] -- any mask, a tree's or not; with
  * window > 0 the last `window` of those keys.  args as there, `causal` set and
- * max_new at most SILI_TREE_MOST (ValueError otherwise); workspace of
- * sili_kv4_attend_tree_workspace(args) bytes. */
+ * max_new at most SILI_TREE_MOST (SILI_ERR_INVALID otherwise); workspace of
+ * sili_kv4_attend_tree_workspace(args) bytes.  Parts of q and of the weights as
+ * there, but a bf16 weight in one part where a request may have more than 16 rows
+ * (max_new x query heads a kv head): an error 1.4 times that of the output's own
+ * rounding. */
 int sili_kv4_attend_tree(const sili_kv4_attend_args *args, const uint64_t *ancestors, void *stream);
 int sili_kv4_attend_tree_workspace(const sili_kv4_attend_args *args, size_t *bytes);
 
@@ -832,10 +835,11 @@ int sili_fp4_pack(const sili_fp4_pack_args *args, void *stream);
 
 /* y[t][n] = sum over the groups of scale * (sum of code * x[t]), x [tokens]
  * [n_in] of `dtype`, y [tokens][n_out] of out_dtype.  Any number of tokens; the
- * weights are read once for up to 16 of them.  x enters the bf16 matrix cores
+ * weights are read once for up to 128 of them.  x enters the bf16 matrix cores
  * in as many parts as its type has bits (fp32 three, f16 two, bf16 one), sums
- * are fp32: the result is that of fp32 arithmetic.  An x that is not finite
- * makes its own row NaN.  workspace: device memory of
+ * are fp32, of a group before its scale: the result is that of fp32 arithmetic
+ * where those are finite (768 times the largest x at most) and x is 0 or above
+ * 2^-110.  An x that is not finite makes its own row NaN or infinite.  workspace: device memory of
  * sili_fp4_linear_workspace(args) bytes, 16-byte aligned; calls that overlap
  * need one each.  The same call gives the same bits. */
 typedef struct {

@@ -200,6 +200,8 @@ struct AttendPlan {
     int32_t waves;            // of a block whose waves share rows
     int32_t join_rows;        // rows such a block joins at most
     int32_t columns;          // columns a row takes
+    int32_t row_tiles;        // tiles of 16 rows a wave of the few-rows kernel takes
+    bool one_part;            // of a softmax weight, in bf16
     int32_t many;             // the most rows of a request for the few-rows kernel; more: the other
     float c;                  // |scale| log2(e)
     bool negative;            // scale < 0: the sign goes to q
@@ -292,8 +294,9 @@ __device__ __forceinline__ uint32_t seen16(const TreeRange &tr, int32_t begin, u
 }
 
 // Registers allow this many waves on a SIMD without spilling.
-template <typename T, int D, int CP>
+template <typename T, int D, int CP, int R = 1>
 constexpr int waves_per_simd() {
+    if (R > 1) return D == 64 ? 3 : 2;
     constexpr bool lean = __is_same(T, __bf16) || (CP > 1 && D < 256);  // no more than two parts in registers
     return (D == 64 ? 4 : D == 128 ? 3 : 2) - (lean ? 0 : 1);
 }
@@ -314,13 +317,17 @@ constexpr int waves_per_simd() {
 // own part of them; the outputs are summed once, at the end.
 //
 // TREE: rows are drafted tokens, which see the context and their ancestors.  Steps
-// before the new tokens are as without; the last one or two take a bit a key.
-template <typename T, int D, int WAVES, int CP, bool TREE>
-__global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_attend_few(sili_kv4_attend_args a, AttendPlan pl) {
-    constexpr int QP = q_parts<T>(), PP = p_parts<T>();
+// before the new tokens are as without; the last one or two take a bit a key.  R
+// tiles of rows share a step's turned codes, PP parts hold a weight.  The vector units
+// bound it there (64 requests of 28 tokens x 5 heads over 5.1 K keys: 328 us, 0.54
+// PFLOP/s; 64 % busy with the codes and the softmax, the matrix cores 27 %).
+template <typename T, int D, int WAVES, int CP, bool TREE, int R = 1, int PP = p_parts<T>()>
+__global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP, R>())) void k_attend_few(sili_kv4_attend_args a, AttendPlan pl) {
+    constexpr int QP = q_parts<T>();
     constexpr int KS = D / 32;   // steps of 32 channels
     constexpr int CT = D / 32;   // blocks of 32 output channels
     constexpr int RT = 16 / CP;  // rows of a tile
+    constexpr int BR = R * RT;   // ... of a block
     constexpr int QM = CP > 1 ? 1 : QP, PM = CP > 1 ? 1 : PP;  // products each
     static_assert(CP == 1 || (CP >= QP && CP >= PP), "parts fit the columns");
     extern __shared__ float s_join[];
@@ -344,9 +351,9 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_at
     const Queries qs = queries_of(a, req);
     const KeyRange kr(a, pl, qs, req);
     const int32_t n_rows = qs.n * group;
-    const int32_t first = tile * RT;
+    const int32_t first = tile * BR;
     if (n_rows > pl.many || first >= n_rows) return;
-    const int32_t i_first = token_of(pl, first), i_last = token_of(pl, min(first + RT - 1, n_rows - 1));
+    const int32_t i_first = token_of(pl, first), i_last = token_of(pl, min(first + BR - 1, n_rows - 1));
     const TreeRange tr(kr, qs);
     const int32_t lo = (TREE ? tr.first() : kr.begin(i_first)) & ~63, hi = TREE ? tr.last() : kr.end(i_last);
     // what every row sees
@@ -359,13 +366,16 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_at
 #pragma unroll
     for (int k = 0; k < PP; ++k) take_p[k] = my_part == k ? ~0u : 0u;
 
-    // this lane's rows
-    const int32_t my_i = token_of(pl, min(first + my_row, n_rows - 1));
-    uint64_t my_mask = TREE ? pl.ancestors[qs.first + my_i] : 0;
-    const int32_t end = kr.end(my_i), begin = TREE ? tr.of(my_mask) : kr.begin(my_i);
-    u32x4 q[KS][QM];
-    {
-        const int32_t row = min(first + my_row, n_rows - 1), i = my_i;
+    // this lane's rows, one of each tile
+    uint64_t my_mask[R];
+    int32_t end[R], begin[R];
+    u32x4 q[R][KS][QM];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int32_t row = min(first + r * RT + my_row, n_rows - 1), i = token_of(pl, row);
+        my_mask[r] = TREE ? pl.ancestors[qs.first + i] : 0;
+        end[r] = kr.end(i);
+        begin[r] = TREE ? tr.of(my_mask[r]) : kr.begin(i);
         const T *src = (const T *)a.q + (int64_t)(qs.first + i) * a.q_token_stride + (h * group + (row - i * group)) * a.q_head_stride + g * (D / 4);
         float xs[KS][8];
         if (pl.q_packed) {
@@ -387,15 +397,20 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_at
                 uint32_t part[QP];
                 split_bf16<QP>(x[2 * j], x[2 * j + 1], part);
 #pragma unroll
-                for (int k = 0; k < QM; ++k) q[s][k][j] = CP > 1 && QP > 1 ? pick<QP>(part, take_q) : part[k];
+                for (int k = 0; k < QM; ++k) q[r][s][k][j] = CP > 1 && QP > 1 ? pick<QP>(part, take_q) : part[k];
             }
         }
     }
 
-    float m = -INFINITY, l = 0.0f;  // m in units of c; l of this lane's keys only
-    f32x4 o[CT][2];
+    float m[R], l[R];  // m in units of c; l of this lane's keys only
+    f32x4 o[R][CT][2];
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) o[ct][0] = o[ct][1] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    for (int r = 0; r < R; ++r) {
+        m[r] = -INFINITY;
+        l[r] = 0.0f;
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) o[r][ct][0] = o[r][ct][1] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    }
 
     // The keys of a step as this lane needs them, loaded a step ahead: a part's
     // registers take the next step's as soon as this one's are used.
@@ -451,16 +466,20 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_at
         page = page_of(key + stride);
     }
     for (; key < c1; key += stride) {
-        f32x4 sc[4];
+        f32x4 sc[R][4];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) sc[x] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) sc[r][x] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int x = 0; x < 4; ++x)
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
                 const u32x4 kk = codes8(kw[x][s]);
 #pragma unroll
-                for (int k = 0; k < QM; ++k) sc[x] = mma(kk, q[s][k], sc[x]);
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int k = 0; k < QM; ++k) sc[r][x] = mma(kk, q[r][s][k], sc[r][x]);
             }
         // wave-uniform: every row sees every key of the step
         const bool here = held, whole = key >= all_begin && key + 64 <= all_end && __all(here);
@@ -470,73 +489,76 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_at
             load_k();
             page = page_of(key + 2 * stride);
         }
-        u32x4 p[2][PM];
-        float v[16], w[16];  // scores, then weights, of keys 16 g + 0 .. 15
+        u32x4 p[R][2][PM];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            v[j] = sc[j >> 2][j & 3];
-            if (QP > 1) v[j] = columns_sum<CP>(v[j]);
-        }
-        times_scales(v, ks);
-        uint32_t seen = 0;
-        if (!whole) {
-            if constexpr (TREE) {
-                seen = here ? seen16(tr, begin, my_mask, key + 16 * g) : 0u;
+        for (int r = 0; r < R; ++r) {
+            float v[16], w[16];  // scores, then weights, of keys 16 g + 0 .. 15
 #pragma unroll
-                for (int j = 0; j < 16; ++j) v[j] = (seen & (1u << j)) != 0 ? v[j] : -INFINITY;
-            } else {
-                int32_t from = here ? begin - (key + 16 * g) : 16, to = end - (key + 16 * g);
-                stay_branch(from, to);
-#pragma unroll
-                for (int j = 0; j < 16; ++j) v[j] = j >= from && j < to ? v[j] : -INFINITY;
+            for (int j = 0; j < 16; ++j) {
+                v[j] = sc[r][j >> 2][j & 3];
+                if (QP > 1) v[j] = columns_sum<CP>(v[j]);
             }
-        }
-        float top = v[0];
+            times_scales(v, ks);
+            uint32_t seen = 0;
+            if (!whole) {
+                if constexpr (TREE) {
+                    seen = here ? seen16(tr, begin[r], my_mask[r], key + 16 * g) : 0u;
 #pragma unroll
-        for (int j = 1; j < 16; ++j) top = fmaxf(top, v[j]);
-        top *= pl.c;
-        if (__any(top > m + SLACK)) {
-            const float up = fmaxf(m, lanes_max(top));
-            // a row without a key so far keeps m = -inf, and factor 1 on its zeros
-            const float keep = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - up);
-            m = up;
-            l *= keep;
+                    for (int j = 0; j < 16; ++j) v[j] = (seen & (1u << j)) != 0 ? v[j] : -INFINITY;
+                } else {
+                    int32_t from = here ? begin[r] - (key + 16 * g) : 16, to = end[r] - (key + 16 * g);
+                    stay_branch(from, to);
 #pragma unroll
-            for (int ct = 0; ct < CT; ++ct) {
-                o[ct][0] *= keep;
-                o[ct][1] *= keep;
+                    for (int j = 0; j < 16; ++j) v[j] = j >= from && j < to ? v[j] : -INFINITY;
+                }
             }
-        }
-        const float ref = m == -INFINITY ? 0.0f : m;
-        float sum = 0.0f;
+            float top = v[0];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(v[j], pl.c, -ref));
-            sum += w[j];
-        }
-        l += sum;
-        times_scales(w, vs);
-        if (!whole) {
-            // a key that this row does not see may hold anything
-            if constexpr (TREE) {
+            for (int j = 1; j < 16; ++j) top = fmaxf(top, v[j]);
+            top *= pl.c;
+            if (__any(top > m[r] + SLACK)) {
+                const float up = fmaxf(m[r], lanes_max(top));
+                // a row without a key so far keeps m = -inf, and factor 1 on its zeros
+                const float keep = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[r] - up);
+                m[r] = up;
+                l[r] *= keep;
 #pragma unroll
-                for (int j = 0; j < 16; ++j) w[j] = (seen & (1u << j)) != 0 ? w[j] : 0.0f;
-            } else {
-                int32_t from = here ? begin - (key + 16 * g) : 16, to = end - (key + 16 * g);
-                stay_branch(from, to);
-#pragma unroll
-                for (int j = 0; j < 16; ++j) w[j] = j >= from && j < to ? w[j] : 0.0f;
+                for (int ct = 0; ct < CT; ++ct) {
+                    o[r][ct][0] *= keep;
+                    o[r][ct][1] *= keep;
+                }
             }
-        }
+            const float ref = m[r] == -INFINITY ? 0.0f : m[r];
+            float sum = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t part[PP];
-                split_bf16<PP>(w[8 * e + 2 * j], w[8 * e + 2 * j + 1], part);
-#pragma unroll
-                for (int k = 0; k < PM; ++k) p[e][k][j] = CP > 1 ? pick<PP>(part, take_p) : part[k];
+            for (int j = 0; j < 16; ++j) {
+                w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(v[j], pl.c, -ref));
+                sum += w[j];
             }
+            l[r] += sum;
+            times_scales(w, vs);
+            if (!whole) {
+                // a key that this row does not see may hold anything
+                if constexpr (TREE) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) w[j] = (seen & (1u << j)) != 0 ? w[j] : 0.0f;
+                } else {
+                    int32_t from = here ? begin[r] - (key + 16 * g) : 16, to = end[r] - (key + 16 * g);
+                    stay_branch(from, to);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) w[j] = j >= from && j < to ? w[j] : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t part[PP];
+                    split_bf16<PP>(w[8 * e + 2 * j], w[8 * e + 2 * j + 1], part);
+#pragma unroll
+                    for (int k = 0; k < PM; ++k) p[r][e][k][j] = CP > 1 ? pick<PP>(part, take_p) : part[k];
+                }
+        }
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
@@ -546,42 +568,47 @@ __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP>())) void k_at
                 codes_by_channel(e ? vw[ct].w : vw[ct].y, e1, o1);
                 const u32x4 even = {e0[0], e0[1], e1[0], e1[1]}, odd = {o0[0], o0[1], o1[0], o1[1]};
 #pragma unroll
-                for (int y = 0; y < PM; ++y) {
-                    o[ct][0] = mma(even, p[e][y], o[ct][0]);
-                    o[ct][1] = mma(odd, p[e][y], o[ct][1]);
-                }
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int y = 0; y < PM; ++y) {
+                        o[r][ct][0] = mma(even, p[r][e][y], o[r][ct][0]);
+                        o[r][ct][1] = mma(odd, p[r][e][y], o[r][ct][1]);
+                    }
             }
         if (more) load_v();
     }
-    l = lanes_sum(l);
-
-    // lane: row r16, channels 32 ct + 8 g + 2 i + (even, odd)
+    // lane: row r16 of a tile, channels 32 ct + 8 g + 2 i + (even, odd)
     const int ROWS = pl.join_rows;
     float *s_o = s_join, *s_m = s_join + WAVES * ROWS * D, *s_l = s_m + WAVES * ROWS;
-    f32x4 sum[CT][2];
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            sum[ct][0][i] = columns_sum<CP>(o[ct][0][i]);
-            sum[ct][1][i] = columns_sum<CP>(o[ct][1][i]);
-        }
-    if (first + r16 < n_rows && r16 < RT) {
-        float *dst = s_o + (wave * ROWS + r16) * D + 8 * g;
+    for (int r = 0; r < R; ++r) {
+        const float all = lanes_sum(l[r]);
+        f32x4 sum[CT][2];
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                dst[32 * ct + 2 * i] = sum[ct][0][i];
-                dst[32 * ct + 2 * i + 1] = sum[ct][1][i];
+                sum[ct][0][i] = columns_sum<CP>(o[r][ct][0][i]);
+                sum[ct][1][i] = columns_sum<CP>(o[r][ct][1][i]);
             }
-        if (g == 0) {
-            s_m[wave * ROWS + r16] = m;
-            s_l[wave * ROWS + r16] = l;
+        const int row = r * RT + r16;
+        if (first + row < n_rows && r16 < RT) {
+            float *dst = s_o + (wave * ROWS + row) * D + 8 * g;
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    dst[32 * ct + 2 * i] = sum[ct][0][i];
+                    dst[32 * ct + 2 * i + 1] = sum[ct][1][i];
+                }
+            if (g == 0) {
+                s_m[wave * ROWS + row] = m[r];
+                s_l[wave * ROWS + row] = all;
+            }
         }
     }
     __syncthreads();
-    const int rows = min(RT, n_rows - first);
+    const int rows = min(BR, n_rows - first);
     for (int at = threadIdx.x; at < rows * (D / 4); at += 64 * WAVES) {
         const int row = at / (D / 4), ch = 4 * (at - row * (D / 4));
         float f[WAVES], mm = -INFINITY, ll = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -1011,7 +1038,8 @@ void kv4_read(const sili_kv4_rows_args &a, hipStream_t st) { rows<false>(a, st, 
 namespace {
 
 // Waves of a CU that run the few-rows kernel at once.
-int waves_of(int dtype, int64_t head_dim, int columns) {
+int waves_of(int dtype, int64_t head_dim, int columns, int row_tiles) {
+    if (row_tiles > 1) return 4 * (head_dim == 64 ? waves_per_simd<__bf16, 64, 1, 2>() : waves_per_simd<__bf16, 128, 1, 2>());
     int n = 0;
     with_dtype(dtype, [&](auto z) {
         using T = decltype(z);
@@ -1070,7 +1098,16 @@ Launch plan_attend(const sili_kv4_attend_args &a, bool tree) {
 
     const int parts = a.dtype == SILI_F32 ? 4 : 2;
     p.columns = rows <= 16 / parts ? parts : 1;
-    const int64_t tile_rows = 16 / p.columns;
+    // Trees of bf16 heads: beyond a tile of rows the products bound the call and not the
+    // cache, so a weight enters in one part (us with one and two; 5 query heads a kv head:
+    // 64 requests of 32 tokens 359 and 408, 16 of 8 tokens 37 and 39, 8 of 64 tokens 211 and
+    // 239), and beyond 64 rows a wave takes two tiles with the same turned codes (the first
+    // and the last of these 328 and 189; 40 rows 43 where one tile takes 37, 64 rows 40
+    // and 38).  The kernel of 128 rows a block took 549 and 242 us for those two: its blocks
+    // are not filled by what a tree has.
+    p.one_part = tree && a.dtype == SILI_BF16 && rows > 16;
+    p.row_tiles = p.one_part && a.cache.head_dim <= 128 && rows > 64 ? 2 : 1;
+    const int64_t tile_rows = 16 / p.columns * p.row_tiles;
     L.rows = std::min<int64_t>(rows, p.many);
     L.tiles = (L.rows + tile_rows - 1) / tile_rows;
     p.join_rows = (int32_t)std::min(tile_rows, rows);
@@ -1081,7 +1118,7 @@ Launch plan_attend(const sili_kv4_attend_args &a, bool tree) {
     // few blocks: as many waves in one as a CU holds, so that fewer splits are left
     // to join (40 heads of 131071 keys, 8 blocks a split: 31 + 5 us against 31 + 7
     // with 4 waves; 320 blocks of 2048 keys: 24 us against 22.6, a second round)
-    const int wide = waves_of(a.dtype, a.cache.head_dim, p.columns);
+    const int wide = waves_of(a.dtype, a.cache.head_dim, p.columns, p.row_tiles);
     p.waves = blocks <= 128 ? wide : 4;
     const int64_t step = 64 * p.waves;
     // splits until every SIMD has as many waves as registers allow; fp32, which the
@@ -1111,6 +1148,17 @@ void run_few(const sili_kv4_attend_args &a, const Launch &L, hipStream_t st) {
     if (p.columns > 1) {
         if (p.waves == WIDE_P) launch(k_attend_few<T, D, WIDE_P, PARTS, TREE>, grid, block, lds, st, a, p);
         else launch(k_attend_few<T, D, 4, PARTS, TREE>, grid, block, lds, st, a, p);
+    } else if (p.row_tiles > 1) {
+        if constexpr (TREE && __is_same(T, __bf16) && D <= 128) {
+            constexpr int W2 = 4 * waves_per_simd<T, D, 1, 2>();
+            if (p.waves == W2) launch(k_attend_few<T, D, W2, 1, TREE, 2, 1>, grid, block, lds, st, a, p);
+            else launch(k_attend_few<T, D, 4, 1, TREE, 2, 1>, grid, block, lds, st, a, p);
+        }
+    } else if (p.one_part) {
+        if constexpr (TREE && __is_same(T, __bf16)) {
+            if (p.waves == WIDE) launch(k_attend_few<T, D, WIDE, 1, TREE, 1, 1>, grid, block, lds, st, a, p);
+            else launch(k_attend_few<T, D, 4, 1, TREE, 1, 1>, grid, block, lds, st, a, p);
+        }
     } else {
         if (p.waves == WIDE) launch(k_attend_few<T, D, WIDE, 1, TREE>, grid, block, lds, st, a, p);
         else launch(k_attend_few<T, D, 4, 1, TREE>, grid, block, lds, st, a, p);

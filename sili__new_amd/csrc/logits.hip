@@ -224,7 +224,7 @@ void logits_constrain(const sili_logits_constrain_args &a, hipStream_t st) {
     with_dtype(a.dtype, [&](auto z) {
         using T = decltype(z);
         if (large) launch(k_logits_constrain<T, 1024, 8>, grid, dim3(1024), 0, st, a, p);
-        else launch(k_logits_constrain<T, 256, 4>, grid, dim3(256), 0, st, a, p);
+        else launch(k_logits_constrain<T, 512, 2>, grid, dim3(512), 0, st, a, p);
     });
     SILI_HIP(hipGetLastError());
 }
