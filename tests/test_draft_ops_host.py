@@ -122,6 +122,14 @@ def test_fp4_linear_refuses(bad):
         dev.fp4_linear(changed(linear, **bad))
 
 
+def test_fp4_linear_refuses_what_no_grid_holds():
+    a = changed(linear, w__n_in=1 << 30, w__codes_stride=1 << 29, w__scales_stride=1 << 25, w__n_out=1, tokens=16, workspace=P, workspace_bytes=1 << 60)
+    with pytest.raises(ValueError, match="too many"):
+        dev.fp4_linear(a)
+    with pytest.raises(ValueError, match="too many"):
+        dev.fp4_linear(changed(linear, tokens=(1 << 31) - 1, w__n_out=(1 << 31) - 1, workspace=P, workspace_bytes=1 << 62))
+
+
 def test_fp4_linear_refuses_a_short_workspace():
     a = changed(linear, w__n_in=1 << 16, w__codes_stride=1 << 15, w__scales_stride=1 << 11)
     need = dev.fp4_linear_workspace(a)

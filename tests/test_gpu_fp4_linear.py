@@ -126,6 +126,19 @@ def test_sizes(hip, n_out, n_in, group, tokens, dtype):
     assert torch.equal(s["y"], again["y"])
 
 
+@pytest.mark.parametrize("n_out,n_in,group,tokens", [(131071, 96, 32, 3), (131071, 64, 64, 16), (110000, 256, 128, 1), (40, 16384, 64, 1), (1500, 16384, 128, 1),
+                                                     (20, 32768, 128, 16), (300, 6144 - 32, 32, 11), (33000, 640, 64, 9), (8200, 1280, 32, 4)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_few_tokens_over_many_outputs_and_inputs(hip, n_out, n_in, group, tokens, dtype):
+    """Blocks that go on to other outputs, waves that share outputs, inputs that LDS does not hold at once."""
+    codes, scales = random_weights(n_out, n_in, group, F32, n_out)
+    gen = torch.Generator(device="cuda").manual_seed(n_in)
+    x = torch.randn(tokens, n_in, generator=gen, device="cuda").to(dtype)
+    s = linear(weights(codes, scales, group), x, F32)
+    check(s, codes, scales, group)
+    assert torch.equal(s["y"], linear(weights(codes, scales, group), x, F32)["y"])
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("tokens", [1, 6, 50, 140])
 def test_strides(hip, tokens, dtype):

@@ -177,6 +177,18 @@ def test_a_token_that_is_often_repeated(hip):
     check(constrain(z, **kw), z, **kw)
 
 
+def test_more_rows_of_a_request_than_a_wave_has_lanes(hip):
+    """A block that goes over 150 rows, each with a mask of its own, beside a thousand requests of a row."""
+    new = [150] + [1] * 600 + [0] * 423
+    rng, kw = case(12, [1] * len(new), 37, 20)
+    rows = int(np.sum(new))
+    kw.update(q_start=np.concatenate([[0], np.cumsum(new)]), tokens=rng.integers(0, 37, rows), allow_row=rng.integers(-1, 4, rows),
+              masks=[int(rng.integers(0, 2 ** 63)) for _ in range(150)] + [1] * 600)
+    for dtype in (torch.float32, torch.bfloat16):
+        z = logits(rng, rows, 37, dtype)
+        check(constrain(z, **kw), z, **kw)
+
+
 def test_a_large_vocabulary_and_a_long_history(hip):
     rng, kw = case(9, [2], 131071, 20000, masks=1, bias="one")
     z = logits(rng, 2, 131071, torch.bfloat16)
