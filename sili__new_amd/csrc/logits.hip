@@ -148,6 +148,7 @@ __global__ __launch_bounds__(TPB, 8) void k_logits_constrain(sili_logits_constra
         const uint64_t path = ((uint64_t)hi << 32 | lo) & in_chunk;
         const bool adds = tid < 64 && mine >= 0 && (path >> lane & 1) != 0;
         if (path != 0) {
+            __syncthreads();  // waves may still be at a row before it, which has no barrier of its own
             if (adds) atomicAdd(&s_count[mine], 1u);
             __syncthreads();
         }

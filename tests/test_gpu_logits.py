@@ -177,6 +177,20 @@ def test_a_token_that_is_often_repeated(hip):
     check(constrain(z, **kw), z, **kw)
 
 
+@pytest.mark.parametrize("vocab,requests,nodes", [(30000, 70, 8), (9000, 140, 5), (5000, 20, 12)])
+def test_rows_with_and_without_a_path_in_a_chunk(hip, vocab, requests, nodes):
+    """A path's tokens lie in few chunks, so a block's rows with barriers follow rows without; large and small chunks."""
+    rng = np.random.default_rng(requests)
+    for dtype in (torch.float32, torch.bfloat16):
+        _, kw = case(int(rng.integers(1000)), [nodes] * requests, vocab, 40, bias="one")
+        kw["tokens"] = rng.integers(0, vocab, requests * nodes)
+        z = logits(rng, requests * nodes, vocab, dtype)
+        t = constrain(z, **kw)
+        check(t, z, **kw)
+        for _ in range(3):
+            assert torch.equal(t["out"], constrain(z, **kw)["out"])
+
+
 def test_more_rows_of_a_request_than_a_wave_has_lanes(hip):
     """A block that goes over 150 rows, each with a mask of its own, beside a thousand requests of a row."""
     new = [150] + [1] * 600 + [0] * 423
