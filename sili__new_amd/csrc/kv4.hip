@@ -1125,7 +1125,11 @@ Launch plan_attend(const sili_kv4_attend_args &a, bool tree) {
     // vector units bound, two at most (320 blocks of 2048 keys: 22.7 us, with a
     // second split 21.4 + 4.7 to join)
     const int64_t fill = 256 * std::max(1, std::min(wide, a.dtype == SILI_F32 ? 8 : wide) / p.waves);
-    const int64_t want = std::clamp<int64_t>(fill / blocks, 1, std::max<int64_t>(1, (reach + 255) / 256));
+    // A split takes 256 keys at least; of a tree whose blocks half fill the GPU 1280, for a
+    // join costs 5 us (240 blocks of 1151 keys at head_dim 64: 11.5 us, three splits 17.0;
+    // 128 of 1024 at 256: 20.0 and 22.4; 80 of 1500 at 128: 14.5 and 13.2).
+    const int64_t least = tree && blocks >= 128 ? 1280 : 256;
+    const int64_t want = std::clamp<int64_t>(fill / blocks, 1, std::max<int64_t>(1, (reach + least - 1) / least));
     p.chunk = (int32_t)std::max(step, ((reach + want - 1) / want + step - 1) / step * step);
     p.splits = (int32_t)std::max<int64_t>(1, (reach + p.chunk - 1) / p.chunk);
     return L;
