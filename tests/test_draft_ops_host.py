@@ -154,6 +154,13 @@ def test_logits_constrain_refuses(bad):
         dev.logits_constrain(changed(logits, **bad))
 
 
+@pytest.mark.parametrize("bad", [dict(vocab=(1 << 31) - 8192, bias=None, allow=None), dict(history_stride=(1 << 31) - 8192)])
+def test_logits_constrain_refuses_what_an_int32_cannot_step_past(bad):
+    """A thread's next token or entry lies up to 8192 past the last one."""
+    with pytest.raises(ValueError, match="out of range"):
+        dev.logits_constrain(changed(logits, **bad))
+
+
 def test_empty_calls_do_nothing():
     """No tokens, rows or outputs: nothing is launched, so nothing needs a GPU or a buffer."""
     for kw in (dict(requests=0), dict(tokens=0), dict(max_new=0)):
