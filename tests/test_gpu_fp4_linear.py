@@ -243,3 +243,23 @@ def test_replayed_in_two_graphs_with_workspaces_of_their_own(hip, tokens):
         for s in calls:
             check(s, codes, scales, group)
             assert torch.equal(s["y"], linear(w, s["x"], F32)["y"])
+
+
+def test_two_calls_at_once_on_streams_of_their_own(hip):
+    """Split calls of few and of many tokens, with a workspace each, in turn on two streams."""
+    n_out, n_in, group = 80, 8192, 64
+    codes, scales = random_weights(n_out, n_in, group, F32, 4)
+    w = weights(codes, scales, group)
+    calls = [(linear(w, torch.randn(tokens, n_in, device="cuda").to(dtype), F32), torch.cuda.Stream())
+             for tokens, dtype in ((8, BF16), (100, F16), (3, F32), (40, F32))]
+    want = [s["y"].clone() for s, _ in calls]
+    for s, _ in calls:
+        check(s, codes, scales, group)
+        s["y"].fill_(7)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s, st in calls:
+            dev.fp4_linear(s["args"], st.cuda_stream)
+    torch.cuda.synchronize()
+    for (s, _), y in zip(calls, want):
+        assert torch.equal(s["y"], y)

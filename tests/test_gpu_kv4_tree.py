@@ -108,6 +108,45 @@ def test_a_long_axis_is_split_and_joined(hip, window, dtype, group, d):
     assert torch.equal(s["out"], again["out"]) and torch.equal(s["lse"], again["lse"])
 
 
+@pytest.mark.parametrize("dtype,d", [(torch.float32, 128), (torch.bfloat16, 256), (torch.float16, 64)])
+@pytest.mark.parametrize("longest", [1280, 1281, 2600])
+def test_many_blocks_over_contexts_about_a_split(hip, longest, dtype, d):
+    """128 and 120 (request, kv head) pairs of one tile of rows: whole, and split from one length on."""
+    rng = np.random.default_rng(longest)
+    for requests in (16, 15):
+        new = rng.integers(1, 8, requests)
+        lens = rng.integers(8, longest + 1, requests)
+        lens[3], lens[4] = longest, longest - 1
+        host, gpu, table = filled(lens, 8, 16, d, 5)
+        masks = tree_masks(rng, new)
+        q = queries(int(new.sum()), 16, d, dtype, 3)
+        for window in (0, 1217):
+            check(host, attend(gpu, q, masks, starts(new), lens, table, window), masks, starts(new), lens, table, window)
+
+
+def test_two_calls_at_once_on_streams_of_their_own(hip):
+    """Split calls with a workspace each, in turn on two streams, against the same calls one after another."""
+    rng = np.random.default_rng(6)
+    new, lens = np.array([13, 64, 1]), np.array([9001, 2777, 5056])
+    host, gpu, table = filled(lens, 2, 16, 128, 3)
+    calls = []
+    for seed in (5, 6):
+        masks = tree_masks(rng, new)
+        q = queries(int(new.sum()), 10, 128, torch.bfloat16, seed)
+        calls.append((attend(gpu, q, masks, starts(new), lens, table), torch.cuda.Stream()))
+    want = [(s["out"].clone(), s["lse"].clone()) for s, _ in calls]
+    for s, _ in calls:
+        s["out"].fill_(7)
+        s["lse"].fill_(7)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s, st in calls:
+            dev.kv4_attend_tree(s["args"], s["masks"].data_ptr(), st.cuda_stream)
+    torch.cuda.synchronize()
+    for (s, _), (out, lse) in zip(calls, want):
+        assert torch.equal(s["out"], out) and torch.equal(s["lse"], lse)
+
+
 def test_many_requests_of_large_trees(hip):
     """Enough blocks of many rows to fill the GPU, requests without tokens and of one among them; hidden pages."""
     rng = np.random.default_rng(8)
