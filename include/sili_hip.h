@@ -801,9 +801,7 @@ int sili_draft_tree(const sili_draft_tree_args *args, void *stream);
  * window > 0 the last `window` of those keys.  args as there, `causal` set and
  * max_new at most SILI_TREE_MOST (SILI_ERR_INVALID otherwise); workspace of
  * sili_kv4_attend_tree_workspace(args) bytes.  Parts of q and of the weights as
- * there, but a bf16 weight in one part where a request may have more than 16 rows
- * (max_new x query heads a kv head): an error 1.4 times that of the output's own
- * rounding. */
+ * there, a bf16 weight in two whatever the request's rows. */
 int sili_kv4_attend_tree(const sili_kv4_attend_args *args, const uint64_t *ancestors, void *stream);
 int sili_kv4_attend_tree_workspace(const sili_kv4_attend_args *args, size_t *bytes);
 

@@ -201,7 +201,6 @@ struct AttendPlan {
     int32_t join_rows;        // rows such a block joins at most
     int32_t columns;          // columns a row takes
     int32_t row_tiles;        // tiles of 16 rows a wave of the few-rows kernel takes
-    bool one_part;            // of a softmax weight, in bf16
     int32_t many;             // the most rows of a request for the few-rows kernel; more: the other
     float c;                  // |scale| log2(e)
     bool negative;            // scale < 0: the sign goes to q
@@ -296,7 +295,7 @@ __device__ __forceinline__ uint32_t seen16(const TreeRange &tr, int32_t begin, u
 // Registers allow this many waves on a SIMD without spilling.
 template <typename T, int D, int CP, int R = 1>
 constexpr int waves_per_simd() {
-    if (R > 1) return D == 64 ? 3 : 2;
+    if (R > 1) return 2;
     constexpr bool lean = __is_same(T, __bf16) || (CP > 1 && D < 256);  // no more than two parts in registers
     return (D == 64 ? 4 : D == 128 ? 3 : 2) - (lean ? 0 : 1);
 }
@@ -318,12 +317,12 @@ constexpr int waves_per_simd() {
 //
 // TREE: rows are drafted tokens, which see the context and their ancestors.  Steps
 // before the new tokens are as without; the last one or two take a bit a key.  R
-// tiles of rows share a step's turned codes, PP parts hold a weight.  The vector units
-// bound it there (64 requests of 28 tokens x 5 heads over 5.1 K keys: 328 us, 0.54
-// PFLOP/s; 64 % busy with the codes and the softmax, the matrix cores 27 %).
-template <typename T, int D, int WAVES, int CP, bool TREE, int R = 1, int PP = p_parts<T>()>
+// tiles of rows share a step's turned codes.  The vector units
+// bound it there (64 requests of 28 tokens x 5 heads over 5.1 K keys: 381 us, 0.46
+// PFLOP/s; 69 % busy with the codes and the softmax, the matrix cores 37 %).
+template <typename T, int D, int WAVES, int CP, bool TREE, int R = 1>
 __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP, R>())) void k_attend_few(sili_kv4_attend_args a, AttendPlan pl) {
-    constexpr int QP = q_parts<T>();
+    constexpr int QP = q_parts<T>(), PP = p_parts<T>();
     constexpr int KS = D / 32;   // steps of 32 channels
     constexpr int CT = D / 32;   // blocks of 32 output channels
     constexpr int RT = 16 / CP;  // rows of a tile
@@ -1038,8 +1037,7 @@ void kv4_read(const sili_kv4_rows_args &a, hipStream_t st) { rows<false>(a, st, 
 namespace {
 
 // Waves of a CU that run the few-rows kernel at once.
-int waves_of(int dtype, int64_t head_dim, int columns, int row_tiles) {
-    if (row_tiles > 1) return 4 * (head_dim == 64 ? waves_per_simd<__bf16, 64, 1, 2>() : waves_per_simd<__bf16, 128, 1, 2>());
+int waves_of(int dtype, int64_t head_dim, int columns) {
     int n = 0;
     with_dtype(dtype, [&](auto z) {
         using T = decltype(z);
@@ -1098,15 +1096,17 @@ Launch plan_attend(const sili_kv4_attend_args &a, bool tree) {
 
     const int parts = a.dtype == SILI_F32 ? 4 : 2;
     p.columns = rows <= 16 / parts ? parts : 1;
-    // Trees of bf16 heads: beyond a tile of rows the products bound the call and not the
-    // cache, so a weight enters in one part (us with one and two; 5 query heads a kv head:
-    // 64 requests of 32 tokens 359 and 408, 16 of 8 tokens 37 and 39, 8 of 64 tokens 211 and
-    // 239), and beyond 64 rows a wave takes two tiles with the same turned codes (the first
-    // and the last of these 328 and 189; 40 rows 43 where one tile takes 37, 64 rows 40
-    // and 38).  The kernel of 128 rows a block took 549 and 242 us for those two: its blocks
-    // are not filled by what a tree has.
-    p.one_part = tree && a.dtype == SILI_BF16 && rows > 16;
-    p.row_tiles = p.one_part && a.cache.head_dim <= 128 && rows > 64 ? 2 : 1;
+    // Trees of many rows in bf16, at head_dim 128: a wave takes two tiles of rows with the
+    // same turned codes where that leaves 2048 blocks of 4096 keys and more (us with one
+    // and two, 8 kv heads x 5, requests x rows of keys: 64 x 160 of 8192 441 and 397, of 4096
+    // 228 and 214, of 300 60 and 66; 64 x 320 of 8192 742 and 657; 64 x 105 304 and 333, half
+    // of the last pair being empty; 16 x 160 131 and 139; 8 x 160 96 and 112; 4 x 320 91 and
+    // 98).  At head_dim 64 it gains nothing (64 x 160 of 8192: 279 and 281); of f16 and fp32,
+    // whose q takes more registers, none was built.
+    const int64_t reach_most = p.window > 0 ? std::min(p.most, p.window) : p.most;
+    const bool paired = tree && a.dtype == SILI_BF16 && a.cache.head_dim == 128 && rows > 128 && heads * ((rows + 31) / 32) >= 2048 &&
+                        reach_most >= 4096;
+    p.row_tiles = paired ? 2 : 1;
     const int64_t tile_rows = 16 / p.columns * p.row_tiles;
     L.rows = std::min<int64_t>(rows, p.many);
     L.tiles = (L.rows + tile_rows - 1) / tile_rows;
@@ -1118,7 +1118,7 @@ Launch plan_attend(const sili_kv4_attend_args &a, bool tree) {
     // few blocks: as many waves in one as a CU holds, so that fewer splits are left
     // to join (40 heads of 131071 keys, 8 blocks a split: 31 + 5 us against 31 + 7
     // with 4 waves; 320 blocks of 2048 keys: 24 us against 22.6, a second round)
-    const int wide = waves_of(a.dtype, a.cache.head_dim, p.columns, p.row_tiles);
+    const int wide = waves_of(a.dtype, a.cache.head_dim, p.columns);
     p.waves = blocks <= 128 ? wide : 4;
     const int64_t step = 64 * p.waves;
     // splits until every SIMD has as many waves as registers allow; fp32, which the
@@ -1153,16 +1153,7 @@ void run_few(const sili_kv4_attend_args &a, const Launch &L, hipStream_t st) {
         if (p.waves == WIDE_P) launch(k_attend_few<T, D, WIDE_P, PARTS, TREE>, grid, block, lds, st, a, p);
         else launch(k_attend_few<T, D, 4, PARTS, TREE>, grid, block, lds, st, a, p);
     } else if (p.row_tiles > 1) {
-        if constexpr (TREE && __is_same(T, __bf16) && D <= 128) {
-            constexpr int W2 = 4 * waves_per_simd<T, D, 1, 2>();
-            if (p.waves == W2) launch(k_attend_few<T, D, W2, 1, TREE, 2, 1>, grid, block, lds, st, a, p);
-            else launch(k_attend_few<T, D, 4, 1, TREE, 2, 1>, grid, block, lds, st, a, p);
-        }
-    } else if (p.one_part) {
-        if constexpr (TREE && __is_same(T, __bf16)) {
-            if (p.waves == WIDE) launch(k_attend_few<T, D, WIDE, 1, TREE, 1, 1>, grid, block, lds, st, a, p);
-            else launch(k_attend_few<T, D, 4, 1, TREE, 1, 1>, grid, block, lds, st, a, p);
-        }
+        if constexpr (TREE && __is_same(T, __bf16) && D == 128) launch(k_attend_few<T, D, 4, 1, TREE, 2>, grid, block, lds, st, a, p);
     } else {
         if (p.waves == WIDE) launch(k_attend_few<T, D, WIDE, 1, TREE>, grid, block, lds, st, a, p);
         else launch(k_attend_few<T, D, 4, 1, TREE>, grid, block, lds, st, a, p);
