@@ -666,6 +666,7 @@ void fp4_pack(const sili_fp4_pack_args &a, hipStream_t st) {
 
 size_t fp4_linear_workspace(const sili_fp4_linear_args &a) {
     check_linear(a);
+    if (a.tokens == 0 || a.w.n_out == 0) return 0;  // nothing to plan
     return linear_bytes(a, plan_linear(a).plan);
 }
 
