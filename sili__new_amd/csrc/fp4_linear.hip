@@ -552,15 +552,17 @@ struct LinearLaunch {
 };
 
 // Few tokens.  512 blocks of 8 waves fill the GPU twice over.  Fewer (outputs / 128):
-// waves share outputs where x is small (up to 4 rows of 16384 inputs, which every such
-// block holds whole), else blocks split the inputs and are joined.  us of a call, its
+// waves share outputs where x is small (up to 4 rows of up to 16384 inputs, of which a
+// block holds all), else blocks split the inputs and are joined.  us of a call, its
 // inputs x outputs, rows of x (tokens times parts); share 1, the best share, the best
 // splits:
 //     5120 x 32768, 3 rows   19.6, 18.7, 21.3      5120 x 5120, 1 row   -, 5.8, 9.0
 //     5120 x 32768, 8 rows   23.0, 26.0, 23.0      5120 x 5120, 8 rows  16.5, 8.7, 9.3
 //     5120 x 32768, 16 rows  27.5, 42.8, 26.5      32768 x 5120, 8 rows -, 31.5, 24.2
 //     5120 x 1000, 3 rows    -, 4.9, 6.5           32768 x 1000, 3 rows -, 9.1, 8.3
-// (8 rows share well by 4 but not by 8, and lose by 2: they split.)  A block whose
+// (8 rows share well by 4 but not by 8, and lose by 2: they split.  Inputs that LDS does
+// not hold split only: 4 rows of 16384 x 5120 14.0, shared and split 25.9, 3 rows 14.0 and
+// 17.3; x 1000 8.2 and 10.6.)  A block whose
 // waves do not share goes on to other outputs with the x it holds (5120 x 131071, 8
 // rows: 78 us, 92 with blocks of one tile).  More than 16 tokens' kernel took 48 us for
 // 5 fp32 tokens of 5120 x 32768, this one 28.
@@ -577,15 +579,16 @@ void plan_few(const sili_fp4_linear_args &a, int64_t parts, LinearLaunch &L) {
     const int64_t base = tiles(a.w.n_out, 16 * FEW_WAVES), want = std::max<int64_t>(1, 512 / base);
     int64_t splits = 1;
     f.share = 1;
-    if (rows <= 4 && turns <= 64) {
+    // words of LDS beside x, what x may take of 112 KiB, and the turns of x that it holds
+    const int64_t words = FEW_WAVES * 16 * (FEW_ROW + FEW_TURN / a.w.group), room = (112 << 8) - words;
+    const int64_t held = std::max<int64_t>(1, (room / rows - 4) / (FEW_TURN / 2));
+    if (rows <= 4 && turns <= std::min<int64_t>(64, held)) {
         while (f.share < 8 && f.share * 2 <= std::min(want, turns)) f.share *= 2;
     } else {
         splits = std::clamp<int64_t>(want, 1, std::max<int64_t>(1, turns / 4));
     }
     f.tiles = (int32_t)tiles(a.w.n_out, 16 * FEW_WAVES / f.share);
-    // words of LDS beside x, and what x may take of 112 KiB
-    const int64_t words = FEW_WAVES * 16 * (FEW_ROW + FEW_TURN / a.w.group), room = (112 << 8) - words;
-    splits = std::max(splits, tiles(turns, std::max<int64_t>(1, (room / rows - 4) / (FEW_TURN / 2))));
+    splits = std::max(splits, tiles(turns, held));
     p.chunk = (int32_t)tiles(turns, splits);
     p.splits = (int32_t)tiles(turns, p.chunk);
     f.row_words = p.chunk * (FEW_TURN / 2) + 4;

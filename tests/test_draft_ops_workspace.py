@@ -22,3 +22,23 @@ def test_an_empty_call_needs_none():
             "    for dtype in (dev.F32, dev.BF16, dev.F16): assert dev.kv4_attend_tree_workspace(changed(attend, dtype=dtype, **kw)) == 0, kw\n")
     r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True)
     assert r.returncode == 0, (r.returncode, r.stderr)
+
+
+def few(tokens, n_out, n_in, group=128, dtype=dev.BF16):
+    """The bytes of a call with those weights."""
+    return dev.fp4_linear_workspace(changed(linear, tokens=tokens, dtype=dtype, w__n_out=n_out, w__n_in=n_in, w__group=group, w__codes_stride=n_in // 2,
+                                            w__scales_stride=n_in // group))
+
+
+def test_waves_share_outputs_only_where_a_block_holds_all_of_x():
+    """4 rows of x (tokens times parts) at most: a block either holds all their inputs, and needs no workspace, or the inputs go
+    to blocks that are joined, as many as 5 rows' do."""
+    for dtype, parts in ((dev.BF16, 1), (dev.F16, 2), (dev.F32, 3)):
+        for group in (32, 128):
+            for tokens in range(1, 4 // parts + 1):
+                for n_in in range(1024, 16385, 1024):
+                    need = few(tokens, 1500, n_in, group, dtype)
+                    if need:
+                        assert need // tokens == few(5, 1500, n_in, group, dev.BF16) // 5, (dtype, group, tokens, n_in)
+                    else:  # 112 KiB hold them beside 8 waves' codes and scales
+                        assert tokens * parts * n_in * 2 <= (112 << 10) - 8 * 16 * (36 + 256 // group) * 4

@@ -1,0 +1,24 @@
+"""GPU: 4-bit weights about the sizes from which a call is cut another way.
+
+Tolerances as in test_gpu_fp4_linear.py."""
+import pytest
+import torch
+
+from tests.test_gpu_fp4_linear import BF16, F16, F32, check, linear, random_weights, weights
+
+pytestmark = pytest.mark.gpu
+
+
+def run(n_out, n_in, group, tokens, dtype):
+    codes, scales = random_weights(n_out, n_in, group, BF16, n_out + tokens)
+    x = torch.randn(tokens, n_in, generator=torch.Generator(device="cuda").manual_seed(n_in), device="cuda").to(dtype)
+    s = linear(weights(codes, scales, group), x, F32)
+    check(s, codes, scales, group)
+    assert torch.equal(s["y"], linear(weights(codes, scales, group), x, F32)["y"])
+
+
+@pytest.mark.parametrize("dtype,tokens", [(BF16, 3), (BF16, 4), (F16, 1), (F16, 2), (F32, 1)])
+@pytest.mark.parametrize("n_in", [11264, 11520, 15104, 15360, 16384, 16640])
+def test_a_few_rows_of_x_that_a_block_holds_or_not(hip, n_in, dtype, tokens):
+    for n_out, group in ((300, 128), (5120, 32)):
+        run(n_out, n_in, group, tokens, dtype)
