@@ -611,8 +611,17 @@ LinearLaunch plan_linear(const sili_fp4_linear_args &a) {
     }
     p.steps = (int32_t)tiles(a.w.n_in, LINEAR_STEP);
     const int64_t steps = std::max<int64_t>(1, p.steps);
+    // A block's waves lie side by side over 256 outputs, or in two rows over 128 (us, inputs
+    // 5120, groups of 128: 32 bf16 tokens x 32768 outputs 37 and 44, x 5120 14.3 and 16.0,
+    // fp32 55 and 87; 33 tokens 52 and 45, 18.4 and 16.1, 89 and 88).  In bf16 a wave takes 64
+    // tokens where two tiles of 32 each are filled in pairs and 512 blocks are left (one tile
+    // and two: 128 tokens x 131071 278 and 237, 65 264 and 228, 256 tokens x 32768 140 and
+    // 117; 192 x 131071 403 and 421; fewer blocks, 128 x 16384 45.6 and 46.7, x 5120 25.5 and
+    // 27.0, 1024 inputs x 32768 20.8 and 31.4).  In f16 and fp32 it loses at every size (128 x
+    // 32768 110 and 138, 163 and 188).
+    const int64_t pairs = tiles(a.tokens, 128);
     L.wn = a.tokens <= 32 ? 4 : 2;
-    L.mt = a.tokens <= 64 ? 1 : 2;
+    L.mt = a.dtype == SILI_BF16 && tiles(a.tokens, 64) == 2 * pairs && tiles(a.w.n_out, 128) * pairs >= 512 ? 2 : 1;
     p.token_tiles = (int32_t)tiles(a.tokens, 32 * L.mt * (4 / L.wn));
     L.blocks = tiles(a.w.n_out, 64 * L.wn) * p.token_tiles;
     const int64_t want = std::clamp<int64_t>(512 / std::max<int64_t>(1, L.blocks), 1, std::max<int64_t>(1, steps / 4));
@@ -636,7 +645,7 @@ void run_linear(const sili_fp4_linear_args &a, const LinearLaunch &L, hipStream_
     } else if (L.mt == 1) {
         launch(k_linear_many<T, G, 2, 1>, grid, dim3(256), (uint32_t)ManyLinear<T, G, 2, 1>::LDS, st, a, p);
     } else {
-        launch(k_linear_many<T, G, 2, 2>, grid, dim3(256), (uint32_t)ManyLinear<T, G, 2, 2>::LDS, st, a, p);
+        if constexpr (__is_same(T, __bf16)) launch(k_linear_many<T, G, 2, 2>, grid, dim3(256), (uint32_t)ManyLinear<T, G, 2, 2>::LDS, st, a, p);
     }
 }
 

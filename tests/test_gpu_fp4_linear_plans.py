@@ -22,3 +22,19 @@ def run(n_out, n_in, group, tokens, dtype):
 def test_a_few_rows_of_x_that_a_block_holds_or_not(hip, n_in, dtype, tokens):
     for n_out, group in ((300, 128), (5120, 32)):
         run(n_out, n_in, group, tokens, dtype)
+
+
+@pytest.mark.parametrize("tokens", [64, 65, 128, 129, 192, 193, 256])
+@pytest.mark.parametrize("n_out", [32640, 32641, 65408, 65409])
+def test_tiles_of_tokens_in_pairs(hip, n_out, tokens):
+    """About 512 blocks of 128 outputs, by the 128 tokens."""
+    for group, n_in in ((128, 384), (64, 320)):
+        run(n_out, n_in, group, tokens, BF16)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("tokens", [65, 128, 200])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_more_tokens_than_a_tile(hip, group, tokens, dtype):
+    for n_out, n_in in ((70000, 256), (700, 3200)):
+        run(n_out, n_in, group, tokens, dtype)
