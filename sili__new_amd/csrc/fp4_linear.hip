@@ -103,6 +103,11 @@ __device__ __forceinline__ uint32_t load_scale(const sili_fp4_weights &w, int64_
 // joined through the workspace.
 constexpr int FEW_TURN = 2 * LINEAR_STEP;  // inputs
 constexpr int FEW_ROW = FEW_TURN / 8 + 4;  // words of a row of codes in LDS: 16 rows in all banks
+// Waves of a block, us with 4, 8 and 16: 1 fp32 token of 5120 x 32768 29.1, 21.8, 25.5; 8 bf16
+// of 32768 x 5120 40.0, 23.7, 27.5; 16 fp32 of 5120 x 32768 46.9, 38.8, 36.7.  Turns ahead, us
+// with 1, 2 and 3: the first of these 20.5, 21.8, 22.7 (its scales bf16) and with fp32 scales,
+// which take the most loads, 26.3 with 1 and 23.0 with 2; the others 23.3, 23.7, 24.5 and 38.2,
+// 38.8, 39.8.
 constexpr int FEW_WAVES = 8;
 constexpr int AHEAD = 2;
 
@@ -451,7 +456,9 @@ __global__ __launch_bounds__(256, 2) void k_linear_many(sili_fp4_linear_args a, 
                 for (int i = 0; i < KS / US; ++i) f[t][i] = sr[32 * t * GS + (sub * KS + i * US) / (G / 16)];
             const uint16_t *base = s_x + (buf * P * BM + 32 * MT * wm + r32) * ROW + 8 * hf;
             // x's operands, FEED products before theirs: the compiler left to itself waits
-            // for each read of LDS
+            // for each read of LDS.  Two and four before theirs take the same time within 1 %
+            // (128 tokens of 5120 x 131071: 239 and 237 us); four do not fit the registers of two
+            // tiles beside a chunk's own sums (128 of 5120 x 32768, groups of 32: 84 and 128 us).
             constexpr int NQ = KS * P * MT, FEED = WHOLE || MT == 1 ? 4 : 2;
             u32x4 av[NQ], b[2];
 #pragma unroll
@@ -562,7 +569,9 @@ struct LinearLaunch {
 //     5120 x 1000, 3 rows    -, 4.9, 6.5           32768 x 1000, 3 rows -, 9.1, 8.3
 // (8 rows share well by 4 but not by 8, and lose by 2: they split.  Inputs that LDS does
 // not hold split only: 4 rows of 16384 x 5120 14.0, shared and split 25.9, 3 rows 14.0 and
-// 17.3; x 1000 8.2 and 10.6.)  A block whose
+// 17.3; x 1000 8.2 and 10.6.)  A split takes four turns at least: 8 bf16 tokens, us with 2, 4
+// and 8, 1024 x 5120 6.9, 5.6, -; 4096 x 1000 6.5, 8.6, 10.4, x 5120 8.6, 9.4, 11.3; 16384 x 1000
+// 8.3, 8.8, 11.1; 32768 x 1000 12.3, 10.5, 11.7.  A block whose
 // waves do not share goes on to other outputs with the x it holds (5120 x 131071, 8
 // rows: 78 us, 92 with blocks of one tile).  More than 16 tokens' kernel took 48 us for
 // 5 fp32 tokens of 5120 x 32768, this one 28.
@@ -624,6 +633,8 @@ LinearLaunch plan_linear(const sili_fp4_linear_args &a) {
     L.mt = a.dtype == SILI_BF16 && tiles(a.tokens, 64) == 2 * pairs && tiles(a.w.n_out, 128) * pairs >= 512 ? 2 : 1;
     p.token_tiles = (int32_t)tiles(a.tokens, 32 * L.mt * (4 / L.wn));
     L.blocks = tiles(a.w.n_out, 64 * L.wn) * p.token_tiles;
+    // A split takes four steps at least: 64 bf16 tokens, us with 2, 4 and 8, 1024 x 1000 9.3,
+    // 10.3, 12.6; 4096 x 1000 10.6, 11.0, 14.1, x 5120 17.2, 16.1, 16.5; 16384 x 1000 17.4, 14.4, 15.9.
     const int64_t want = std::clamp<int64_t>(512 / std::max<int64_t>(1, L.blocks), 1, std::max<int64_t>(1, steps / 4));
     p.chunk = (int32_t)tiles(steps, want);
     p.splits = (int32_t)tiles(steps, p.chunk);

@@ -2,7 +2,7 @@
 //
 // A block holds a chunk of the vocabulary of one request: it counts the
 // request's history there in LDS (low 31 bits: how often past counted_from; top
-// bit: before it), and then goes over the request's rows, four or eight tokens a
+// bit: before it), and then goes over the request's rows, two or eight tokens a
 // thread and load, whose biases stay in registers.  A bit a token says whether it occurs at
 // all: most eights ask for no count.  A row whose own path has tokens in the chunk
 // adds them to the counts and takes them off again; the others pass without a
