@@ -554,6 +554,7 @@ struct LinearLaunch {
     bool few_tokens = false, merged = false;
     int wn = 0, mt = 0;  // more tokens: a block's shape
     uint32_t lds = 0;
+    int64_t most_splits = 1;  // few tokens: what plan.splits is rounded down from; no less for more tokens
     LinearPlan plan{};
     FewLinear few{};
 };
@@ -598,6 +599,7 @@ void plan_few(const sili_fp4_linear_args &a, int64_t parts, LinearLaunch &L) {
     }
     f.tiles = (int32_t)tiles(a.w.n_out, 16 * FEW_WAVES / f.share);
     splits = std::max(splits, tiles(turns, held));
+    L.most_splits = splits;
     p.chunk = (int32_t)tiles(turns, splits);
     p.splits = (int32_t)tiles(turns, p.chunk);
     f.row_words = p.chunk * (FEW_TURN / 2) + 4;
@@ -641,8 +643,26 @@ LinearLaunch plan_linear(const sili_fp4_linear_args &a) {
     return L;
 }
 
+// A workspace for the call and for those of fewer tokens, which may split where it does
+// not: tokens x splits at most, over the plans that plan_linear takes up to a.tokens.
+// Blocks of 64 tokens and 128 outputs split into 512 / blocks at most, so those of more than
+// 32 tokens need 64 x 512 / (outputs / 128) rows of sums however many they are.
 size_t linear_bytes(const sili_fp4_linear_args &a, const LinearPlan &p) {
-    return p.splits == 1 ? 0 : (size_t)a.tokens * (size_t)a.w.n_out * (size_t)p.splits * sizeof(float);
+    auto tiles = [](int64_t n, int64_t of) { return (n + of - 1) / of; };
+    sili_fp4_linear_args few = a;
+    few.tokens = std::min<int64_t>(a.tokens, 16);
+    LinearLaunch L;
+    plan_few(few, a.dtype == SILI_F32 ? 3 : a.dtype == SILI_F16 ? 2 : 1, L);
+    int64_t rows = L.most_splits > 1 ? few.tokens * L.most_splits : 0;
+    const int64_t steps = tiles(a.w.n_in, LINEAR_STEP) / 4;
+    auto more = [&](int64_t tokens, int64_t blocks, int64_t most) {
+        const int64_t splits = std::min(512 / blocks, steps);
+        if (splits > 1) rows = std::max(rows, std::min(tokens * splits, most));
+    };
+    if (a.tokens > 16) more(std::min<int64_t>(a.tokens, 32), tiles(a.w.n_out, 256), INT64_MAX);
+    if (a.tokens > 32) more(a.tokens, tiles(a.w.n_out, 128), 64 * 512 / tiles(a.w.n_out, 128));
+    if (p.splits > 1) rows = std::max(rows, a.tokens * p.splits);
+    return (size_t)rows * (size_t)a.w.n_out * sizeof(float);
 }
 
 template <typename T, int G>
@@ -689,8 +709,7 @@ void fp4_pack(const sili_fp4_pack_args &a, hipStream_t st) {
 
 size_t fp4_linear_workspace(const sili_fp4_linear_args &a) {
     check_linear(a);
-    if (a.tokens == 0 || a.w.n_out == 0) return 0;  // nothing to plan
-    return linear_bytes(a, plan_linear(a).plan);
+    return a.tokens == 0 || a.w.n_out == 0 ? 0 : linear_bytes(a, plan_linear(a).plan);
 }
 
 void fp4_linear(const sili_fp4_linear_args &a, hipStream_t st) {

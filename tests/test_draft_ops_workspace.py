@@ -3,6 +3,8 @@ import os
 import subprocess
 import sys
 
+import pytest
+
 from sili__new_amd import device as dev
 from tests.test_draft_ops_host import attend, changed, linear
 
@@ -42,3 +44,15 @@ def test_waves_share_outputs_only_where_a_block_holds_all_of_x():
                         assert need // tokens == few(5, 1500, n_in, group, dev.BF16) // 5, (dtype, group, tokens, n_in)
                     else:  # 112 KiB hold them beside 8 waves' codes and scales
                         assert tokens * parts * n_in * 2 <= (112 << 10) - 8 * 16 * (36 + 256 // group) * 4
+
+
+@pytest.mark.parametrize("dtype", [dev.F32, dev.BF16, dev.F16])
+@pytest.mark.parametrize("group", [32, 128])
+def test_more_tokens_never_need_less(dtype, group):
+    """A buffer for the most tokens does for fewer, which may split the inputs where those do not."""
+    counts = list(range(0, 400)) + [511, 512, 513, 1000, 4096, 5000, 16384, 16385, 70000, (1 << 31) - 1]
+    for n_out in (1, 16, 127, 129, 1000, 1500, 5120, 8192, 16384, 32768, 33000, 65536, 131071):
+        for n_in in (group, 128, 640, 1024, 5120, 11264, 12288, 16384, 32768):
+            sizes = [few(t, n_out, n_in, group, dtype) for t in counts]
+            assert sizes == sorted(sizes), (n_out, n_in)
+            assert sizes[-1] <= max(sizes[16], 16 << 20)  # of more than 16 tokens 512 blocks split at most

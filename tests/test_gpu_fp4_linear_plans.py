@@ -4,6 +4,7 @@ Tolerances as in test_gpu_fp4_linear.py."""
 import pytest
 import torch
 
+from sili__new_amd import device as dev
 from tests.test_gpu_fp4_linear import BF16, F16, F32, check, linear, random_weights, weights
 
 pytestmark = pytest.mark.gpu
@@ -38,3 +39,23 @@ def test_tiles_of_tokens_in_pairs(hip, n_out, tokens):
 def test_more_tokens_than_a_tile(hip, group, tokens, dtype):
     for n_out, n_in in ((70000, 256), (700, 3200)):
         run(n_out, n_in, group, tokens, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("n_out,n_in", [(1000, 4096), (5120, 1024), (300, 16384)])
+def test_one_workspace_for_every_step(hip, n_out, n_in, dtype):
+    """A server's: asked for once, for the most tokens that a step may have."""
+    group, most = 64, 700
+    codes, scales = random_weights(n_out, n_in, group, BF16, 3)
+    x = torch.randn(most, n_in, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(dtype)
+    s = linear(weights(codes, scales, group), x, F32)
+    a, y = s["args"], s["y"]
+    check(s, codes, scales, group)
+    for tokens in (1, 2, 5, 16, 17, 32, 33, 64, 65, 128, 129, 300, 699):
+        y.fill_(7)
+        a.tokens = tokens
+        torch.cuda.synchronize()
+        dev.fp4_linear(a)
+        torch.cuda.synchronize()
+        assert bool((s["work"][a.workspace_bytes:] == 255).all()) and bool((y[tokens:] == 7).all())
+        check(dict(x=x[:tokens], y=y[:tokens]), codes, scales, group)
