@@ -748,8 +748,9 @@ int sili_kv4_read(const sili_kv4_rows_args *args, void *stream);
  * calls with 512 blocks of 128 such rows or more (requests x kv_heads x
  * ceil(rows of the longest request / 128)): the error against exact arithmetic
  * is 1.4 times that of the output's own rounding there.  workspace: device
- * memory of sili_kv4_attend_workspace(args) bytes, 16-byte aligned; calls that
- * overlap need one each. */
+ * memory of sili_kv4_attend_workspace(args) bytes, 16-byte aligned, to be asked for
+ * with each call's sizes (fewer requests or keys may be cut into more pieces);
+ * calls that overlap need one each. */
 typedef struct {
     sili_kv4_cache cache;
     int32_t dtype, causal;
@@ -800,7 +801,9 @@ int sili_draft_tree(const sili_draft_tree_args *args, void *stream);
  * bit j < n of its mask ancestors[t] [tokens] -- any mask, a tree's or not; with
  * window > 0 the last `window` of those keys.  args as there, `causal` set and
  * max_new at most SILI_TREE_MOST (SILI_ERR_INVALID otherwise); workspace of
- * sili_kv4_attend_tree_workspace(args) bytes.  Parts of q and of the weights as
+ * sili_kv4_attend_tree_workspace(args) bytes, enough also for calls of fewer requests,
+ * tokens (requests x max_new of them at most), max_new or max_len with these heads,
+ * types, cache and window.  Parts of q and of the weights as
  * there, a bf16 weight in two whatever the request's rows. */
 int sili_kv4_attend_tree(const sili_kv4_attend_args *args, const uint64_t *ancestors, void *stream);
 int sili_kv4_attend_tree_workspace(const sili_kv4_attend_args *args, size_t *bytes);

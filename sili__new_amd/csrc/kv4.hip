@@ -1051,6 +1051,9 @@ int waves_of(int dtype, int64_t head_dim, int columns) {
     return n;
 }
 
+constexpr int64_t LEAST_KEYS = 256;  // of a split
+constexpr int64_t FILL = 256 * 4;    // blocks of 4 waves that the GPU takes at once, at most
+
 // How a call is launched: requests of up to plan.many rows go to the few-rows
 // kernel, `tiles` row tiles a (request, kv head), those of more to the other.
 struct Launch {
@@ -1128,16 +1131,25 @@ Launch plan_attend(const sili_kv4_attend_args &a, bool tree) {
     // A split takes 256 keys at least; of a tree whose blocks half fill the GPU 1280, for a
     // join costs 5 us (240 blocks of 1151 keys at head_dim 64: 11.5 us, three splits 17.0;
     // 128 of 1024 at 256: 20.0 and 22.4; 80 of 1500 at 128: 14.5 and 13.2).
-    const int64_t least = tree && blocks >= 128 ? 1280 : 256;
+    const int64_t least = tree && blocks >= 128 ? 1280 : LEAST_KEYS;
     const int64_t want = std::clamp<int64_t>(fill / blocks, 1, std::max<int64_t>(1, (reach + least - 1) / least));
     p.chunk = (int32_t)std::max(step, ((reach + want - 1) / want + step - 1) / step * step);
     p.splits = (int32_t)std::max<int64_t>(1, (reach + p.chunk - 1) / p.chunk);
     return L;
 }
 
-size_t part_bytes(const sili_kv4_attend_args &a, const AttendPlan &p) {
-    if (p.splits == 1) return 0;
-    return (size_t)a.tokens * (size_t)a.q_heads * (size_t)p.splits * ((size_t)a.cache.head_dim * sizeof(float) + sizeof(float2));
+size_t part_bytes(const sili_kv4_attend_args &a, const AttendPlan &p, bool tree) {
+    const size_t each = (size_t)a.cache.head_dim * sizeof(float) + sizeof(float2), rows = (size_t)a.tokens * (size_t)a.q_heads;
+    const size_t own = p.splits == 1 ? 0 : rows * (size_t)p.splits * each;
+    if (!tree) return own;
+    // Fewer requests, tokens or keys may be split where these are not.  With requests x
+    // max_new tokens at most, blocks x a tile's rows are no less than the tokens' rows, and a
+    // call splits into FILL / blocks pieces and into one for 256 keys: rows x splits is
+    // bounded whatever the call.
+    const int64_t reach = p.window > 0 ? std::min<int64_t>(p.most, int64_t(p.window) + SILI_TREE_MOST + 63) : p.most;
+    if (reach <= LEAST_KEYS) return own;
+    const size_t pieces = (size_t)((reach + LEAST_KEYS - 1) / LEAST_KEYS);
+    return std::max(own, std::min(rows * pieces, (size_t)FILL * (16 / p.columns)) * each);
 }
 
 template <typename T, int D, bool TREE>
@@ -1166,12 +1178,12 @@ void run_few(const sili_kv4_attend_args &a, const Launch &L, hipStream_t st) {
 
 size_t kv4_attend_workspace(const sili_kv4_attend_args &a) {
     check_attend(a, false);
-    return part_bytes(a, plan_attend(a, false).plan);
+    return part_bytes(a, plan_attend(a, false).plan, false);
 }
 
 size_t kv4_attend_tree_workspace(const sili_kv4_attend_args &a) {
     check_attend(a, true);
-    return part_bytes(a, plan_attend(a, true).plan);
+    return part_bytes(a, plan_attend(a, true).plan, true);
 }
 
 namespace {
@@ -1185,7 +1197,7 @@ void attend(const sili_kv4_attend_args &a, const uint64_t *ancestors, hipStream_
     require(!TREE || ancestors, "kv4_attend_tree: NULL ancestors");
     Launch L = plan_attend(a, TREE);
     L.plan.ancestors = ancestors;
-    const size_t need = part_bytes(a, L.plan);
+    const size_t need = part_bytes(a, L.plan, TREE);
     require(need == 0 || (a.workspace && aligned(a.workspace, 16) && a.workspace_bytes >= need),
             "kv4_attend: workspace too small or not 16-byte aligned");
     const int64_t most = (int64_t(1) << 32) - 1;  // threads of a grid's x

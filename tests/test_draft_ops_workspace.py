@@ -1,5 +1,7 @@
 """CPU: what the operators over drafted tokens ask for as workspace."""
+import math
 import os
+import random
 import subprocess
 import sys
 
@@ -56,3 +58,28 @@ def test_more_tokens_never_need_less(dtype, group):
             sizes = [few(t, n_out, n_in, group, dtype) for t in counts]
             assert sizes == sorted(sizes), (n_out, n_in)
             assert sizes[-1] <= max(sizes[16], 16 << 20)  # of more than 16 tokens 512 blocks split at most
+
+
+@pytest.mark.parametrize("dtype", [dev.F32, dev.BF16, dev.F16])
+@pytest.mark.parametrize("window", [0, 1, 1000])
+def test_smaller_trees_never_need_more(dtype, window):
+    """A buffer for the largest step does for every step of fewer requests, tokens or keys."""
+    rng = random.Random(window)
+    log = lambda n: int(math.exp(rng.uniform(0, math.log(n + 1))))  # noqa: E731
+    split = 0
+    for _ in range(300):
+        kv, group, d = rng.choice([1, 2, 5, 8, 40]), rng.choice([1, 2, 5, 16]), rng.choice([64, 128, 256])
+
+        def need(r, n, t, length):
+            return dev.kv4_attend_tree_workspace(changed(attend, dtype=dtype, window=window, cache__kv_heads=kv, q_heads=kv * group, cache__head_dim=d,
+                                                         cache__n_pages=1 << 17, table_width=1 << 13, requests=r, max_new=n, tokens=t, max_len=length))
+
+        r, n, length = log(256), log(64), log(131072)
+        largest = need(r, n, r * n, length)
+        for _ in range(20):
+            fewer, less, shorter = rng.randint(1, r), rng.randint(1, n), rng.choice([length, log(length)])
+            bytes_ = need(fewer, less, rng.randint(1, fewer * less), shorter)
+            assert bytes_ <= largest, (kv, group, d, r, n, length, fewer, less, shorter)
+            split += bytes_ > 0
+        assert largest <= 20 << 20
+    assert split > 300 or window == 1
