@@ -196,9 +196,9 @@ __global__ __launch_bounds__(TPB, 8) void k_logits_constrain(sili_logits_constra
 }  // namespace
 
 void logits_constrain(const sili_logits_constrain_args &a, hipStream_t st) {
-    constexpr int64_t MOST = (int64_t(1) << 31) - 1, STEP = 8192;  // what a thread's next token or entry may lie past the last one
+    constexpr int64_t MOST = (int64_t(1) << 31) - 1, STEP = 8192;  // what a thread's next token, entry or row may lie past the last one
     require(a.dtype == SILI_F32 || a.dtype == SILI_BF16 || a.dtype == SILI_F16, "logits_constrain: unknown dtype");
-    require(a.rows >= 0 && a.rows <= MOST, "logits_constrain: rows out of range");
+    require(a.rows >= 0 && a.rows <= MOST - STEP, "logits_constrain: rows out of range");
     require(a.vocab >= 0 && a.vocab <= MOST - STEP, "logits_constrain: vocab out of range");
     require(a.requests >= 0 && a.requests <= MOST, "logits_constrain: requests out of range");
     require(!a.history || (a.history_stride >= 0 && a.history_stride <= MOST - STEP), "logits_constrain: history_stride out of range");

@@ -1,0 +1,13 @@
+"""CPU: bounds of the operators over drafted tokens, refused before any device call."""
+import pytest
+
+from sili__new_amd import device as dev
+from tests.test_draft_ops_host import changed, logits
+
+
+@pytest.mark.parametrize("vocab", [1, 100])
+@pytest.mark.parametrize("rows", [(1 << 31) - 8192, (1 << 31) - 1024, (1 << 31) - 1])
+def test_logits_constrain_refuses_rows_that_an_int32_cannot_step_past(rows, vocab):
+    """A block's next row lies up to 1024 past its last one."""
+    with pytest.raises(ValueError, match="rows out of range"):
+        dev.logits_constrain(changed(logits, rows=rows, vocab=vocab, requests=1))
