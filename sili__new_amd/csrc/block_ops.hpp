@@ -44,6 +44,9 @@ inline Span span(const void *p, int64_t bytes) {
 }
 inline bool meet(const Span &x, const Span &y) { return std::max(x.begin, y.begin) < std::min(x.end, y.end); }
 
+// Rows of n elements, `stride` apart, of which none has a byte of another.
+inline bool apart(int64_t rows, int64_t n, int64_t stride) { return rows <= 1 || stride >= n || stride <= -n; }
+
 // Element types of activations.  The conversions of __bf16 and _Float16 round
 // to nearest even and keep NaN and infinities.
 inline int64_t dtype_size(int dtype) { return dtype == SILI_F32 ? 4 : 2; }

@@ -209,6 +209,7 @@ void logits_constrain(const sili_logits_constrain_args &a, hipStream_t st) {
     if (a.rows == 0 || a.vocab == 0 || a.requests == 0) return;
     require(a.logits && a.out, "logits_constrain: NULL buffer");
     require(a.out != a.logits || a.out_stride == a.logits_stride, "logits_constrain: in place with other strides");
+    require(apart(a.rows, a.vocab, a.out_stride), "logits_constrain: rows of out overlap");
     LogitsPlan p;
     // Chunks of 8192 tokens, whose 1024 threads scan a history in few loads (64 requests
     // of 8 rows of 131071 and histories of 8192: 97 us, with chunks of 4096 and 256

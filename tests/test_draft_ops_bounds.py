@@ -2,7 +2,7 @@
 import pytest
 
 from sili__new_amd import device as dev
-from tests.test_draft_ops_host import changed, logits
+from tests.test_draft_ops_host import P, changed, logits
 
 
 @pytest.mark.parametrize("vocab", [1, 100])
@@ -11,3 +11,10 @@ def test_logits_constrain_refuses_rows_that_an_int32_cannot_step_past(rows, voca
     """A block's next row lies up to 1024 past its last one."""
     with pytest.raises(ValueError, match="rows out of range"):
         dev.logits_constrain(changed(logits, rows=rows, vocab=vocab, requests=1))
+
+
+@pytest.mark.parametrize("stride", [99, 1, 0, -1, -99])
+def test_logits_constrain_refuses_rows_of_out_that_overlap(stride):
+    for kw in (dict(), dict(out=P, logits_stride=stride)):
+        with pytest.raises(ValueError, match="logits_constrain: rows of out overlap"):
+            dev.logits_constrain(changed(logits, out_stride=stride, **kw))
