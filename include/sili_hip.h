@@ -877,8 +877,8 @@ int sili_fp4_linear_workspace(const sili_fp4_linear_args *args, size_t *bytes);
  * of history, the penalties, bias and allow may be NULL.  Tokens outside the
  * vocabulary count nowhere, bits of ancestors past the request neither; lengths
  * are cut to their buffers; rows, vocab and history_stride are 2^31 - 8193 at most.
- * out may be logits (same strides), and overlaps it not otherwise; rows of no
- * request are left as they were. */
+ * out may be logits (same strides), and has no byte of it or of another input
+ * otherwise (refused); rows of no request are left as they were. */
 typedef struct {
     int32_t dtype;
     int64_t rows, vocab, requests;

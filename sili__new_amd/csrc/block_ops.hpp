@@ -5,6 +5,7 @@
 
 #include "../../include/sili_hip.h"
 #include "common.hpp"
+#include "overlap.hpp"
 
 #include <algorithm>
 
@@ -44,6 +45,11 @@ inline Span span(const void *p, int64_t bytes) {
 }
 inline bool meet(const Span &x, const Span &y) { return std::max(x.begin, y.begin) < std::min(x.end, y.end); }
 
+// n elements of `bytes` bytes one after another, or `rows` times that.
+inline Rows row(const void *p, int64_t n, int64_t bytes) { return {p, 1, (__int128)n * bytes, 0}; }
+inline Rows rows_of(const void *p, int64_t rows, int64_t n, int64_t stride, int64_t bytes) {
+    return {p, rows, (__int128)n * bytes, (__int128)stride * bytes};
+}
 // Rows of n elements, `stride` apart, of which none has a byte of another.
 inline bool apart(int64_t rows, int64_t n, int64_t stride) { return rows <= 1 || stride >= n || stride <= -n; }
 

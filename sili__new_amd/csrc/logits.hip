@@ -210,6 +210,22 @@ void logits_constrain(const sili_logits_constrain_args &a, hipStream_t st) {
     require(a.logits && a.out, "logits_constrain: NULL buffer");
     require(a.out != a.logits || a.out_stride == a.logits_stride, "logits_constrain: in place with other strides");
     require(apart(a.rows, a.vocab, a.out_stride), "logits_constrain: rows of out overlap");
+    const int64_t es = dtype_size(a.dtype), words = (a.vocab + 31) / 32;
+    const Rows out = rows_of(a.out, a.rows, a.vocab, a.out_stride, es);
+    const Rows read[] = {a.out == a.logits ? Rows{} : rows_of(a.logits, a.rows, a.vocab, a.logits_stride, es),
+                         row(a.q_start, a.requests + 1, 4),
+                         rows_of(a.history, a.requests, a.history_stride, a.history_stride, 4),
+                         row(a.history_lens, a.requests, 4),
+                         row(a.counted_from, a.requests, 4),
+                         row(a.tokens, a.rows, 4),
+                         row(a.ancestors, a.rows, 8),
+                         row(a.repetition, a.requests, 4),
+                         row(a.presence, a.requests, 4),
+                         row(a.frequency, a.requests, 4),
+                         rows_of(a.bias, a.bias_stride == 0 ? 1 : a.requests, a.vocab, a.bias_stride, 4),
+                         rows_of(a.allow, a.n_allow, words, a.allow_stride, 4),
+                         row(a.allow_row, a.rows, 4)};
+    for (const Rows &r : read) require(!meet(out, r), "logits_constrain: out overlaps an input");
     LogitsPlan p;
     // Chunks of 8192 tokens, whose 1024 threads scan a history in few loads (64 requests
     // of 8 rows of 131071 and histories of 8192: 97 us, with chunks of 4096 and 256
