@@ -722,6 +722,7 @@ void fp4_linear(const sili_fp4_linear_args &a, hipStream_t st) {
             "fp4_linear: workspace too small or not 16-byte aligned");
     L.plan.part = static_cast<float *>(a.workspace);
     require(L.blocks * 512 < (int64_t(1) << 32) && L.plan.splits <= 65535, "fp4_linear: too many tokens, outputs or inputs");
+    require(apart(a.tokens, a.w.n_out, a.y_stride), "fp4_linear: rows of y overlap");
     with_dtype(a.dtype, [&](auto z) {
         with_group(a.w.group, [&](auto g) { run_linear<decltype(z), decltype(g)::value>(a, L, st); });
     });
