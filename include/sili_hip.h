@@ -840,7 +840,8 @@ int sili_fp4_pack(const sili_fp4_pack_args *args, void *stream);
  * in as many parts as its type has bits (fp32 three, f16 two, bf16 one), sums
  * are fp32, of a group before its scale: the result is that of fp32 arithmetic
  * where those are finite (768 times the largest x at most) and x is 0 or above
- * 2^-110.  An x that is not finite makes its own row NaN or infinite.  workspace: device memory of
+ * 2^-110.  An x that is not finite makes its own row NaN or infinite.  y has no byte
+ * of an input (refused).  workspace: device memory of
  * sili_fp4_linear_workspace(args) bytes, 16-byte aligned, enough also for calls
  * of fewer tokens with these weights and types; calls that overlap need one each.
  * The same call gives the same bits. */

@@ -541,6 +541,9 @@ void check_weights(const sili_fp4_weights &w, const char *what) {
     need(w.n_out <= 1 || (w.codes_stride >= w.n_in / 2 && w.scales_stride >= w.n_in / w.group), "rows of codes or scales overlap");
 }
 
+Rows codes_of(const sili_fp4_weights &w) { return rows_of(w.codes, w.n_out, w.n_in / 2, w.codes_stride, 1); }
+Rows scales_of(const sili_fp4_weights &w) { return rows_of(w.scales, w.n_out, w.n_in / w.group, w.scales_stride, dtype_size(w.scale_dtype)); }
+
 void check_linear(const sili_fp4_linear_args &a) {
     check_weights(a.w, "fp4_linear");
     require(a.dtype == SILI_F32 || a.dtype == SILI_BF16 || a.dtype == SILI_F16, "fp4_linear: unknown dtype");
@@ -723,6 +726,10 @@ void fp4_linear(const sili_fp4_linear_args &a, hipStream_t st) {
     L.plan.part = static_cast<float *>(a.workspace);
     require(L.blocks * 512 < (int64_t(1) << 32) && L.plan.splits <= 65535, "fp4_linear: too many tokens, outputs or inputs");
     require(apart(a.tokens, a.w.n_out, a.y_stride), "fp4_linear: rows of y overlap");
+    const Rows y = rows_of(a.y, a.tokens, a.w.n_out, a.y_stride, dtype_size(a.out_dtype)), work = row(a.workspace, (int64_t)need, 1);
+    for (const Rows &r : {rows_of(a.x, a.tokens, a.w.n_in, a.x_stride, dtype_size(a.dtype)), codes_of(a.w), scales_of(a.w)})
+        require(!meet(y, r) && !meet(work, r), "fp4_linear: y or the workspace overlaps an input");
+    require(!meet(y, work), "fp4_linear: y overlaps the workspace");
     with_dtype(a.dtype, [&](auto z) {
         with_group(a.w.group, [&](auto g) { run_linear<decltype(z), decltype(g)::value>(a, L, st); });
     });

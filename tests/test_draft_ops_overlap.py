@@ -2,7 +2,7 @@
 import pytest
 
 from sili__new_amd import device as dev
-from tests.test_draft_ops_host import P, changed, logits
+from tests.test_draft_ops_host import P, changed, linear, logits
 
 
 @pytest.mark.parametrize("bad", [dict(out=P + 4), dict(out=P - 4), dict(out=P + 400), dict(out=P + 1596), dict(out=P - 1596), dict(out=P + 4, logits_stride=120),
@@ -14,3 +14,25 @@ from tests.test_draft_ops_host import P, changed, logits
 def test_logits_constrain(bad):
     with pytest.raises(ValueError, match="logits_constrain: out overlaps an input"):
         dev.logits_constrain(changed(logits, **bad))
+
+
+def product(**kw):
+    """A call that needs a workspace, its buffers apart."""
+    a = changed(linear, w__n_in=1 << 16, w__codes_stride=1 << 15, w__scales_stride=1 << 11, w__codes=P << 4, w__scales=P << 5, x=P << 6, x_stride=1 << 16,
+                y=P << 7, workspace=P << 8)
+    a.workspace_bytes = dev.fp4_linear_workspace(a)
+    return changed(lambda: a, **kw)
+
+
+@pytest.mark.parametrize("bad", [dict(y=(P << 6) + 4), dict(y=(P << 6) - 572), dict(y=(P << 6) + (3 << 18) - 4), dict(y=(P << 6) + (1 << 18), tokens=2),
+                                 dict(y=(P << 6) + 1024, y_stride=1 << 16), dict(y=(P << 4) + (48 << 15) - 4), dict(y=(P << 5) - 4), dict(y=(P << 5) + (48 << 13) - 4),
+                                 dict(workspace=P << 6), dict(workspace=(P << 4) + 16), dict(workspace=(P << 5) - 16), dict(y=(P << 6) + (3 << 18) + 188, y_stride=-48)])
+def test_fp4_linear(bad):
+    with pytest.raises(ValueError, match="fp4_linear: y or the workspace overlaps an input"):
+        dev.fp4_linear(product(**bad))
+
+
+@pytest.mark.parametrize("at", [-572, 0, 4, 1 << 10])
+def test_fp4_linear_on_its_workspace(at):
+    with pytest.raises(ValueError, match="fp4_linear: y overlaps the workspace"):
+        dev.fp4_linear(product(y=(P << 8) + at))
