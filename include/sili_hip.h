@@ -825,7 +825,8 @@ typedef struct {
 /* Weights from rows [n_out][n_in] of `dtype`: scale = amax / 6 of the group,
  * rounded to scale_dtype, codes fp4_encode(x * (1 / scale)) in fp32.  A group
  * whose scale rounds to less than 2^-120 is stored as zeros; one with a NaN or
- * an infinity, or whose scale is past scale_dtype, gets a NaN scale. */
+ * an infinity, or whose scale is past scale_dtype, gets a NaN scale.  Codes, scales
+ * and rows have no byte in common (refused). */
 typedef struct {
     sili_fp4_weights w;
     int32_t dtype;

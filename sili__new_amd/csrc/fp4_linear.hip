@@ -699,6 +699,8 @@ void fp4_pack(const sili_fp4_pack_args &a, hipStream_t st) {
     require(a.dtype == SILI_F32 || a.dtype == SILI_BF16 || a.dtype == SILI_F16, "fp4_pack: unknown dtype");
     if (a.w.n_out == 0 || a.w.n_in == 0) return;
     require(a.rows, "fp4_pack: NULL buffer");
+    const Rows in = rows_of(a.rows, a.w.n_out, a.w.n_in, a.row_stride, dtype_size(a.dtype)), codes = codes_of(a.w), scales = scales_of(a.w);
+    require(!meet(codes, in) && !meet(scales, in) && !meet(codes, scales), "fp4_pack: outputs overlap the rows or each other");
     const int64_t blocks = std::min<int64_t>((a.w.n_out * (a.w.n_in / 8) + PACK_TPB - 1) / PACK_TPB, 1 << 20);
     with_dtype(a.dtype, [&](auto z) {
         with_dtype(a.w.scale_dtype, [&](auto s) {

@@ -2,7 +2,7 @@
 import pytest
 
 from sili__new_amd import device as dev
-from tests.test_draft_ops_host import P, changed, linear, logits
+from tests.test_draft_ops_host import P, changed, linear, logits, pack
 
 
 @pytest.mark.parametrize("bad", [dict(out=P + 4), dict(out=P - 4), dict(out=P + 400), dict(out=P + 1596), dict(out=P - 1596), dict(out=P + 4, logits_stride=120),
@@ -36,3 +36,12 @@ def test_fp4_linear(bad):
 def test_fp4_linear_on_its_workspace(at):
     with pytest.raises(ValueError, match="fp4_linear: y overlaps the workspace"):
         dev.fp4_linear(product(y=(P << 8) + at))
+
+
+@pytest.mark.parametrize("bad", [dict(w__codes=(P << 6) + 48 * 1024 - 16), dict(w__codes=P << 6), dict(w__codes=(P << 6) - 48 * 128 + 16), dict(w__scales=P << 6),
+                                 dict(w__scales=(P << 6) + 48 * 1024 - 4), dict(w__scales=(P << 6) - 48 * 32 + 4), dict(w__scales=P), dict(w__scales=P + 48 * 128 - 4),
+                                 dict(w__scales=P - 48 * 32 + 4), dict(w__codes=(P << 6) + 512, w__codes_stride=1024), dict(w__scales=P + 124, w__codes_stride=160, w__scales_stride=40)])
+def test_fp4_pack(bad):
+    apart = changed(pack, rows=P << 6, w__scales=P << 5)
+    with pytest.raises(ValueError, match="fp4_pack: outputs overlap the rows or each other"):
+        dev.fp4_pack(changed(lambda: apart, **bad))
