@@ -803,7 +803,8 @@ int sili_draft_tree(const sili_draft_tree_args *args, void *stream);
  * max_new at most SILI_TREE_MOST (SILI_ERR_INVALID otherwise); workspace of
  * sili_kv4_attend_tree_workspace(args) bytes, enough also for calls of fewer requests,
  * tokens (requests x max_new of them at most), max_new or max_len with these heads,
- * types, cache and window.  Parts of q and of the weights as
+ * types, cache and window.  out may be q (same strides); it, lse and the workspace
+ * have no byte of another buffer otherwise (refused).  Parts of q and of the weights as
  * there, a bf16 weight in two whatever the request's rows. */
 int sili_kv4_attend_tree(const sili_kv4_attend_args *args, const uint64_t *ancestors, void *stream);
 int sili_kv4_attend_tree_workspace(const sili_kv4_attend_args *args, size_t *bytes);

@@ -1054,6 +1054,38 @@ int waves_of(int dtype, int64_t head_dim, int columns) {
 constexpr int64_t LEAST_KEYS = 256;  // of a split
 constexpr int64_t FILL = 256 * 4;    // blocks of 4 waves that the GPU takes at once, at most
 
+// [tokens][heads][d] elements as rows: tokens of heads, or heads of tokens where those are
+// further apart.
+Rows heads_of(const void *p, int64_t tokens, int64_t heads, int64_t d, int64_t token_stride, int64_t head_stride, int64_t bytes) {
+    auto size = [](__int128 v) { return v < 0 ? -v : v; };
+    const __int128 ts = (__int128)token_stride * bytes, hs = (__int128)head_stride * bytes;
+    const bool by_token = tokens > 1 && (heads == 1 || size(ts) >= size(hs));
+    const int64_t n = by_token ? tokens : heads, inner = by_token ? heads : tokens;
+    const __int128 pitch = by_token ? ts : hs, step = by_token ? hs : ts, reach = (inner - 1) * step;
+    return {(const char *)p + (int64_t)std::min<__int128>(0, reach), n, size(reach) + (__int128)d * bytes, pitch};
+}
+
+// Blocks read q, masks and lengths while others write.
+void check_overlap(const sili_kv4_attend_args &a, const uint64_t *ancestors, size_t work_bytes) {
+    const int64_t es = dtype_size(a.dtype), d = a.cache.head_dim, heads = a.cache.n_pages * a.cache.kv_heads, ps = a.cache.page_size;
+    const Rows out = heads_of(a.out, a.tokens, a.q_heads, d, a.out_token_stride, a.out_head_stride, es);
+    const Rows lse = row(a.lse, a.tokens * a.q_heads, 4), work = row(a.workspace, (int64_t)work_bytes, 1);
+    const bool in_place = a.q == a.out && a.q_token_stride == a.out_token_stride && a.q_head_stride == a.out_head_stride;
+    const Rows q = heads_of(a.q, a.tokens, a.q_heads, d, a.q_token_stride, a.q_head_stride, es);
+    const Rows read[] = {row(ancestors, a.tokens, 8),
+                         row(a.q_start, a.requests + 1, 4),
+                         row(a.kv_lens, a.requests, 4),
+                         row(a.block_table, a.requests, a.table_width * 4),
+                         rows_of(a.cache.k, heads, ps * (d / 2), ps * (d / 2), 1),
+                         rows_of(a.cache.v, heads, ps * (d / 2), ps * (d / 2), 1),
+                         rows_of(a.cache.k_scale, heads, ps, ps, 4),
+                         rows_of(a.cache.v_scale, heads, ps, ps, 4)};
+    bool ok = (in_place || !meet(out, q)) && !meet(lse, q) && !meet(work, q);
+    for (const Rows &r : read) ok = ok && !meet(out, r) && !meet(lse, r) && !meet(work, r);
+    require(ok, "kv4_attend_tree: out, lse or the workspace overlaps an input");
+    require(!meet(out, lse) && !meet(out, work) && !meet(lse, work), "kv4_attend_tree: out, lse and the workspace overlap");
+}
+
 // How a call is launched: requests of up to plan.many rows go to the few-rows
 // kernel, `tiles` row tiles a (request, kv head), those of more to the other.
 struct Launch {
@@ -1204,6 +1236,7 @@ void attend(const sili_kv4_attend_args &a, const uint64_t *ancestors, hipStream_
     require(L.tiles * a.cache.kv_heads * 64 * L.plan.waves <= most && L.many_tiles * a.cache.kv_heads * 64 * MANY_WAVES <= most &&
                 L.rows * (L.plan.splits > 1 ? 256 : 1) <= most && L.plan.splits <= 65535,
             "kv4_attend: too many rows or keys");
+    if (TREE) check_overlap(a, ancestors, need);
     with_dtype(a.dtype, [&](auto z) {
         using T = decltype(z);
         switch (a.cache.head_dim) {
