@@ -628,14 +628,15 @@ LinearLaunch plan_linear(const sili_fp4_linear_args &a) {
     // A block's waves lie side by side over 256 outputs, or in two rows over 128 (us, inputs
     // 5120, groups of 128: 32 bf16 tokens x 32768 outputs 37 and 44, x 5120 14.3 and 16.0,
     // fp32 55 and 87; 33 tokens 52 and 45, 18.4 and 16.1, 89 and 88).  In bf16 a wave takes 64
-    // tokens where two tiles of 32 each are filled in pairs and 512 blocks are left (one tile
-    // and two: 128 tokens x 131071 278 and 237, 65 264 and 228, 256 tokens x 32768 140 and
-    // 117; 192 x 131071 403 and 421; fewer blocks, 128 x 16384 45.6 and 46.7, x 5120 25.5 and
-    // 27.0, 1024 inputs x 32768 20.8 and 31.4).  In f16 and fp32 it loses at every size (128 x
-    // 32768 110 and 138, 163 and 188).
+    // tokens where tiles of 64 are filled in pairs and 8192 steps of 128 x 128 x 128 are left,
+    // 32 a CU (us with one tile and two: 5120 x 131071 128 tokens 278 and 237, 65 264 and 228,
+    // 192 403 and 421; x 32768 128 76.0 and 76.6, 256 140 and 117; 2048 x 65536 128 59 and 53;
+    // 32768 x 5120 128 87 and 78, 256 165 and 132; and of fewer steps 8192 x 8192 128 38 and 40,
+    // 2048 x 32768 33 and 41, 5120 x 5120 25.5 and 27.0, 1024 x 32768 20.8 and 31.4).  In f16 and
+    // fp32 it loses at every size (128 of 5120 x 32768 110 and 138, 163 and 188).
     const int64_t pairs = tiles(a.tokens, 128);
     L.wn = a.tokens <= 32 ? 4 : 2;
-    L.mt = a.dtype == SILI_BF16 && tiles(a.tokens, 64) == 2 * pairs && tiles(a.w.n_out, 128) * pairs >= 512 ? 2 : 1;
+    L.mt = a.dtype == SILI_BF16 && tiles(a.tokens, 64) == 2 * pairs && tiles(a.w.n_out, 128) * pairs * steps >= 8192 ? 2 : 1;
     p.token_tiles = (int32_t)tiles(a.tokens, 32 * L.mt * (4 / L.wn));
     L.blocks = tiles(a.w.n_out, 64 * L.wn) * p.token_tiles;
     // A split takes four steps at least: 64 bf16 tokens, us with 2, 4 and 8, 1024 x 1000 9.3,
@@ -648,8 +649,8 @@ LinearLaunch plan_linear(const sili_fp4_linear_args &a) {
 
 // A workspace for the call and for those of fewer tokens, which may split where it does
 // not: tokens x splits at most, over the plans that plan_linear takes up to a.tokens.
-// Blocks of 64 tokens and 128 outputs split into 512 / blocks at most, so those of more than
-// 32 tokens need 64 x 512 / (outputs / 128) rows of sums however many they are.
+// Blocks of 64 or 128 tokens and 128 outputs split into 512 / blocks at most, so those of more
+// than 32 tokens need 128 x 512 / (outputs / 128) rows of sums however many they are.
 size_t linear_bytes(const sili_fp4_linear_args &a, const LinearPlan &p) {
     auto tiles = [](int64_t n, int64_t of) { return (n + of - 1) / of; };
     sili_fp4_linear_args few = a;
@@ -663,7 +664,7 @@ size_t linear_bytes(const sili_fp4_linear_args &a, const LinearPlan &p) {
         if (splits > 1) rows = std::max(rows, std::min(tokens * splits, most));
     };
     if (a.tokens > 16) more(std::min<int64_t>(a.tokens, 32), tiles(a.w.n_out, 256), INT64_MAX);
-    if (a.tokens > 32) more(a.tokens, tiles(a.w.n_out, 128), 64 * 512 / tiles(a.w.n_out, 128));
+    if (a.tokens > 32) more(a.tokens, tiles(a.w.n_out, 128), 128 * 512 / tiles(a.w.n_out, 128));
     if (p.splits > 1) rows = std::max(rows, a.tokens * p.splits);
     return (size_t)rows * (size_t)a.w.n_out * sizeof(float);
 }

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from sili__new_amd import device as dev
+from tests import block_ref
 from tests.test_gpu_fp4_linear import BF16, F16, F32, check, linear, random_weights, weights
 
 pytestmark = pytest.mark.gpu
@@ -26,11 +27,18 @@ def test_a_few_rows_of_x_that_a_block_holds_or_not(hip, n_in, dtype, tokens):
 
 
 @pytest.mark.parametrize("tokens", [64, 65, 128, 129, 192, 193, 256])
-@pytest.mark.parametrize("n_out", [32640, 32641, 65408, 65409])
-def test_tiles_of_tokens_in_pairs(hip, n_out, tokens):
-    """About 512 blocks of 128 outputs, by the 128 tokens."""
-    for group, n_in in ((128, 384), (64, 320)):
-        run(n_out, n_in, group, tokens, BF16)
+@pytest.mark.parametrize("n_out,n_in,group", [(65408, 2048, 128), (65409, 2048, 64), (131000, 992, 32), (260, 349952, 128), (2049, 65600, 64)])
+def test_tiles_of_tokens_in_pairs(hip, n_out, n_in, group, tokens):
+    """About 8192 steps of 128 outputs, 128 tokens and 128 inputs; the products in 64 bits on the GPU."""
+    codes, scales = random_weights(n_out, n_in, group, BF16, n_out + tokens)
+    x = torch.randn(tokens, n_in, generator=torch.Generator(device="cuda").manual_seed(n_in), device="cuda").to(BF16)
+    s = linear(weights(codes, scales, group), x, F32)
+    levels = torch.from_numpy(block_ref.LEVELS).cuda()
+    w = torch.stack([levels[(codes & 15).long()], levels[(codes >> 4).long()]], -1).view(n_out, n_in // group, group) * scales.double()[..., None]
+    w = w.view(n_out, n_in).t().contiguous()
+    want, size = x.double() @ w, x.double().abs() @ w.abs()
+    tol = 2.0 ** -18 * size
+    assert bool(((s["y"].double() - want).abs() <= tol + 2.0 ** -24 * (want.abs() + tol)).all())
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])
