@@ -27,7 +27,9 @@ __device__ __forceinline__ float group_max(float v) {
     return v;
 }
 
-// A thread takes 8 inputs, group / 8 neighbours a group.
+// A thread takes 8 inputs, group / 8 neighbours a group.  Bound by the codec's arithmetic, 286
+// vector instructions for the 8 in any type: 32768 x 5120 139 us from fp32 (5.5 TB/s), 132 from
+// bf16, 128 from f16 (3.3 TB/s, floor 83); 131071 x 5120 570, 491, 493.
 template <typename T, typename S, int G>
 __global__ __launch_bounds__(PACK_TPB) void k_fp4_pack(sili_fp4_pack_args a) {
     const int64_t per_row = a.w.n_in / 8, total = a.w.n_out * per_row;

@@ -1161,8 +1161,12 @@ Launch plan_attend(const sili_kv4_attend_args &a, bool tree) {
     // second split 21.4 + 4.7 to join)
     const int64_t fill = 256 * std::max(1, std::min(wide, a.dtype == SILI_F32 ? 8 : wide) / p.waves);
     // A split takes 256 keys at least; of a tree whose blocks half fill the GPU 1280, for a
-    // join costs 5 us (240 blocks of 1151 keys at head_dim 64: 11.5 us, three splits 17.0;
-    // 128 of 1024 at 256: 20.0 and 22.4; 80 of 1500 at 128: 14.5 and 13.2).
+    // join costs 5 us (14 rows a block, us with 256 and 1280: head_dim 64 in f16 160 blocks of
+    // 700 keys 12.4 and 7.3, of 1300 14.3 and 15.6, of 2600 18.5 and 17.5, 240 14.1 and 7.8, 16.1 and
+    // 16.8, 20.6 and 20.7; head_dim 128 in fp32 192 of 700 18.8 and 12.7, of 1300 22.5 and 22.4;
+    // 256 in bf16 256 of 700 25.5 and 16.9, 160 of 1300 23.3 and 27.9; with 2560 keys 700 the same,
+    // 1300 less, 2600 more: 11.5 and 20.6 at the first of these; below 128 blocks 64 of 2600 at
+    // head_dim 64 12.6 and 14.4).
     const int64_t least = tree && blocks >= 128 ? 1280 : LEAST_KEYS;
     const int64_t want = std::clamp<int64_t>(fill / blocks, 1, std::max<int64_t>(1, (reach + least - 1) / least));
     p.chunk = (int32_t)std::max(step, ((reach + want - 1) / want + step - 1) / step * step);
