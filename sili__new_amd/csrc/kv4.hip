@@ -1233,7 +1233,7 @@ void attend(const sili_kv4_attend_args &a, const uint64_t *ancestors, hipStream_
     require(!TREE || ancestors, "kv4_attend_tree: NULL ancestors");
     Launch L = plan_attend(a, TREE);
     L.plan.ancestors = ancestors;
-    const size_t need = part_bytes(a, L.plan, TREE);
+    const size_t need = L.plan.splits == 1 ? 0 : part_bytes(a, L.plan, TREE);  // what other calls need is theirs
     require(need == 0 || (a.workspace && aligned(a.workspace, 16) && a.workspace_bytes >= need),
             "kv4_attend: workspace too small or not 16-byte aligned");
     const int64_t most = (int64_t(1) << 32) - 1;  // threads of a grid's x

@@ -67,3 +67,17 @@ def test_one_workspace_for_every_step(hip, n_out, n_in, dtype):
         torch.cuda.synchronize()
         assert bool((s["work"][a.workspace_bytes:] == 255).all()) and bool((y[tokens:] == 7).all())
         check(dict(x=x[:tokens], y=y[:tokens]), codes, scales, group)
+
+
+def test_a_call_that_is_not_split_needs_none(hip):
+    """Enough blocks to fill the GPU: no workspace, though fewer tokens would need one."""
+    codes, scales = random_weights(5120, 1024, 64, BF16, 3)
+    s = linear(weights(codes, scales, 64), torch.randn(1000, 1024, device="cuda").to(BF16), F32)
+    a, want = s["args"], s["y"].clone()
+    assert a.workspace_bytes > 0
+    a.workspace, a.workspace_bytes = None, 0
+    s["y"].fill_(7)
+    torch.cuda.synchronize()
+    dev.fp4_linear(a)
+    torch.cuda.synchronize()
+    assert torch.equal(s["y"], want)

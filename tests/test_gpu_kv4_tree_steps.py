@@ -38,3 +38,20 @@ def test_one_workspace_for_every_step(hip, dtype, group, d):
         torch.cuda.synchronize()
         assert torch.equal(s["out"], want) and bool((work[size:] == 255).all())
         check(host, s, masks, starts(count), have, table[:n])
+
+
+def test_a_call_that_is_not_split_needs_none(hip):
+    """Enough blocks to fill the GPU: no workspace, though smaller steps would need one."""
+    rng = np.random.default_rng(1)
+    new, lens = np.full(70, 3), rng.integers(200, 400, 70)
+    host, gpu, table = filled(lens, 8, 16, 64, 5)
+    masks = tree_masks(rng, new)
+    s = attend(gpu, queries(210, 8, 64, torch.bfloat16, 3), masks, starts(new), lens, table)
+    a, want = s["args"], s["out"].clone()
+    assert a.workspace_bytes > 0
+    a.workspace, a.workspace_bytes = None, 0
+    s["out"].fill_(7)
+    torch.cuda.synchronize()
+    dev.kv4_attend_tree(a, s["masks"].data_ptr())
+    torch.cuda.synchronize()
+    assert torch.equal(s["out"], want)
