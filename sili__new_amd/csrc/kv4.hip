@@ -317,8 +317,8 @@ constexpr int waves_per_simd() {
 //
 // TREE: rows are drafted tokens, which see the context and their ancestors.  Steps
 // before the new tokens are as without; the last one or two take a bit a key.  R
-// tiles of rows share a step's turned codes.  The vector units
-// bound it there (64 requests of 28 tokens x 5 heads over 5.1 K keys: 381 us, 0.46
+// tiles of rows share a step's turned codes.  The vector units bound it
+// there (64 requests of 28 tokens x 5 heads over 5.1 K keys: 377 us, 0.47
 // PFLOP/s; 69 % busy with the codes and the softmax, the matrix cores 37 %).
 template <typename T, int D, int WAVES, int CP, bool TREE, int R = 1>
 __global__ __launch_bounds__(64 * WAVES, (waves_per_simd<T, D, CP, R>())) void k_attend_few(sili_kv4_attend_args a, AttendPlan pl) {
